@@ -5,8 +5,9 @@ test/test_quantize_bench.py:7; `from ac4k_kernel.ops import linear, quantize`,
 test/test_linear_bench.py:4; `from ac4k_kernel.ops import attention`, test/test_attention_bench.py:4)
 keep their import lines.  Only the NVFP4 path exists here: the meta API of
 python/ac4k_kernel/__init__.py:58-74, the quantize / linear operators of
-python/ac4k_kernel/ops/__init__.py:5-26 and `attention` (both precisions, head dims up to 128).  The RoPE and
-sparse-attention names of the reference are absent, and asking for them raises AttributeError / ImportError.
+python/ac4k_kernel/ops/__init__.py:5-26 and `attention` (both precisions, head dims up to 128).  The
+sparse-attention names of the reference and `rope3d` are absent (`rope` takes three axes among others), and asking for them raises
+AttributeError / ImportError.
 """
 import sys as _sys
 

@@ -12,6 +12,12 @@ from . import build as _build
 
 _i64, _f32, _int, _vp, _cp = ctypes.c_int64, ctypes.c_float, ctypes.c_int, ctypes.c_void_p, ctypes.c_char_p
 
+
+class RopeTensor(ctypes.Structure):
+    """ac4k_rope_tensor"""
+    _fields_ = ([("input", _vp), ("out", _vp)] + [(n, _i64) for n in ("in_b", "in_n", "in_h", "out_b", "out_n", "out_h", "heads")])
+
+
 # name -> (restype, argtypes); must list every function of include/ac4k_nvfp4.h
 SIGNATURES = {
     "ac4k_arch": (_cp, []),
@@ -55,6 +61,15 @@ SIGNATURES = {
     "ac4k_attention_nvfp4_workspace_bytes": (_i64, [_i64] * 6),
     "ac4k_attention_nvfp4_bf16": (_int, [_vp] + [_i64] * 4 + ([_vp] + [_i64] * 3) * 3 + [_i64] * 6 + [_f32, _f32, _vp, _i64, _vp]),
     "ac4k_quantize_int8_token_block_bf16": (_int, [_vp, _vp, _vp] + [_i64] * 7 + [_int, _vp]),
+    "ac4k_rms_norm_workspace_bytes": (_i64, [_i64, _i64, _int, _int, _int]),
+    "ac4k_rms_norm": (_int, [_vp, _i64, _vp, _vp, _int, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _int, _i64, _i64, _int, _int,
+                             ctypes.c_double, _vp, _i64, _vp]),
+    "ac4k_dequantize": (_int, [_vp, _int, _vp, _vp, _vp] + [_i64] * 5 + [_int, _vp]),
+    "ac4k_rope": (_int, [ctypes.POINTER(RopeTensor), _int, _int, _i64, _i64, _i64, _vp, _i64, _i64, ctypes.POINTER(_i64), _int,
+                         _vp, _int, _i64, _i64, _i64, ctypes.POINTER(_i64), _int, _int, _vp]),
+    "ac4k_linear_grouped_nvfp4_workspace_bytes": (_i64, [_i64] * 4 + [_int]),
+    "ac4k_linear_grouped_nvfp4": (_int, [_vp, _int, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _int, _vp] + [_i64] * 4
+                                  + [_vp, _i64, _vp]),
 }
 
 _lib = None

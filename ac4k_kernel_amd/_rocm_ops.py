@@ -454,3 +454,255 @@ def quantize_int8_token_block(y, scale, x_bhnd, block: int) -> None:
         return
     _lib.check(_L.ac4k_quantize_int8_token_block_bf16(y.data_ptr(), scale.data_ptr(), x_bhnd.data_ptr(), B, H, N, D,
                                                       x_bhnd.stride(0), x_bhnd.stride(1), x_bhnd.stride(2), int(block), _stream()))
+
+
+_PRECISIONS = {None: 0, "fp8e4m3": 1, "int8": 2, "nvfp4": 3}
+_EIGHT_BITS = {torch.float8_e4m3fn: 1, torch.int8: 2}
+
+
+def _check_float(t, name: str) -> int:
+    _check(isinstance(t, torch.Tensor), "{} must be a tensor", name)
+    _check(t.is_cuda, "{} must be a CUDA tensor", name)
+    _check(t.dtype in _DTYPE_TAG, "{} must be bfloat16, half or float", name)
+    return _DTYPE_TAG[t.dtype]
+
+
+def _same_device(dev: int, **tensors) -> None:
+    """Kernels run on the current device and its stream: every operand has to be there."""
+    _check(dev == _current_device(), "operands on device {}, the current device is {}", dev, _current_device())
+    for name, t in tensors.items():
+        _check(t is None or t.get_device() == dev, "{} is on another device than the first operand", name)
+
+
+def _rows_view(t, name: str):
+    """t [.., K] as rows: (rows, K, elements between rows) of the tensor itself, or None if no single row stride describes it."""
+    shape, stride = t.shape, t.stride()
+    _check(t.dim() >= 1 and shape[-1] >= 1, "{} must have a last dim of at least one element", name)
+    rows, step = 1, 0
+    if shape[-1] > 1 and stride[-1] != 1:
+        return None
+    for n, s in zip(reversed(shape[:-1]), reversed(stride[:-1])):
+        if n == 1:
+            continue
+        if rows > 1 and s != step * rows:
+            return None
+        if rows == 1:
+            step = s
+        rows *= n
+    return rows, shape[-1], step
+
+
+def _may_overlap(a, b) -> bool:
+    """Whether the memory between the first and the last element of two tensors meets."""
+    def ends(t):
+        first = t.data_ptr()
+        return first, first + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
+    (a0, a1), (b0, b1) = ends(a), ends(b)
+    return a0 < b1 and b0 < a1
+
+
+def _same_rows(a, b) -> bool:
+    return a.data_ptr() == b.data_ptr() and a.stride() == b.stride()
+
+
+def rms_norm(out, sf, global_scale, given_scale: bool, x, weight, residual, residual_out, precision, eps: float) -> None:
+    """out (and sf, global_scale) <- norm of the rows of x, or of x + residual, which residual_out receives."""
+    tag = _check_float(x, "x")
+    view = _rows_view(x, "x")
+    _check(view is not None, "x must have rows of contiguous elements, evenly apart")
+    rows, K, x_step = view
+    _check(precision in _PRECISIONS, "precision must be one of {}", list(_PRECISIONS))
+    _same_device(x.get_device(), weight=weight, residual=residual, residual_out=residual_out, out=out, sf=sf, global_scale=global_scale)
+    if weight is not None:
+        _check(_check_float(weight, "weight") == tag or weight.dtype == torch.float32, "weight must have the type of x or be float")
+        _check(weight.dim() == 1 and weight.size(0) == K and weight.is_contiguous(), "weight must be contiguous of [{}]", K)
+    _check((residual is None) == (residual_out is None), "a residual comes with residual_out, and the other way round")
+    steps = [0, 0]
+    if residual is not None:
+        for i, (t, name) in enumerate(((residual, "residual"), (residual_out, "residual_out"))):
+            _check(_check_float(t, name) == tag and t.shape == x.shape, "{} must have the type and shape of x", name)
+            v = _rows_view(t, name)
+            _check(v is not None, "{} must have rows of contiguous elements, evenly apart", name)
+            steps[i] = v[2]
+        _check(rows <= 1 or abs(steps[1]) >= K, "residual_out must have rows of its own")
+        for t in (x, residual):
+            _check(_same_rows(t, residual_out) or not _may_overlap(t, residual_out),
+                   "residual_out may be x or residual itself, but not overlap them otherwise")
+    out_step = 0
+    if precision is None:
+        _check(_check_float(out, "out") == tag and out.shape == x.shape, "out must have the type and shape of x")
+        v = _rows_view(out, "out")
+        _check(v is not None and (rows <= 1 or abs(v[2]) >= K), "out must have rows of contiguous elements, evenly apart")
+        out_step = v[2]
+        _check(_same_rows(out, x) or not _may_overlap(out, x), "out may be x itself, but not overlap it otherwise")
+        for t in (residual, residual_out):
+            _check(t is None or not _may_overlap(out, t), "out must not overlap residual or residual_out")
+    else:
+        nvfp4 = precision == "nvfp4"
+        _check_tensor(out, torch.uint8 if nvfp4 else torch.float8_e4m3fn if precision == "fp8e4m3" else torch.int8, "out")
+        _check(list(out.shape) == [rows, _align_up(K, 64) // 2 if nvfp4 else _align_up(K, 16)], "meet invalid out shape")
+        _check_tensor(sf, torch.float8_e4m3fn if nvfp4 else torch.float32, "sf")
+        _check(list(sf.shape) == ([_align_up(K, 64) // 64, _align_up(rows, 16), 4] if nvfp4 else [_align_up(rows, 16)]), "meet invalid sf shape")
+        if nvfp4:
+            _check_tensor(global_scale, torch.float32, "global_scale")
+            _check(global_scale.dim() == 0, "global_scale must be a scalar")
+    if rows == 0:
+        return
+    nbytes = _L.ac4k_rms_norm_workspace_bytes(rows, K, tag, _PRECISIONS[precision], int(given_scale))
+    ws = x.new_empty((nbytes,), dtype=torch.uint8) if nbytes > 0 else None
+    _lib.check(_L.ac4k_rms_norm(out.data_ptr(), out_step, None if sf is None else sf.data_ptr(),
+                                None if global_scale is None else global_scale.data_ptr(), int(given_scale), x.data_ptr(), x_step,
+                                None if residual is None else residual.data_ptr(), steps[0],
+                                None if residual is None else residual_out.data_ptr(), steps[1],
+                                None if weight is None else weight.data_ptr(), tag if weight is None else _DTYPE_TAG[weight.dtype],
+                                rows, K, tag, _PRECISIONS[precision], float(eps), None if ws is None else ws.data_ptr(), nbytes,
+                                _stream()))
+
+
+def dequantize(out, q, sf, global_scale=None) -> None:
+    """out [.., R, cols] <- the values of q, sf (and global_scale, for nvfp4) as `quantize` returns them without swizzle."""
+    tag = _check_float(out, "out")
+    _check(isinstance(q, torch.Tensor) and q.dim() >= 2, "q must have at least two dims")
+    nvfp4 = q.dtype == torch.uint8
+    _check(nvfp4 or q.dtype in _EIGHT_BITS, "q must be uint8 (nvfp4), float8_e4m3fn or int8")
+    _check_tensor(q, q.dtype, "q")
+    _same_device(q.get_device(), out=out, sf=sf, global_scale=global_scale)
+    lead, R, W = list(q.shape[:-2]), q.size(-2), q.size(-1) * (2 if nvfp4 else 1)
+    _check(W % (64 if nvfp4 else 16) == 0, "rows of q must be whole pieces of {} elements", 64 if nvfp4 else 16)
+    _check_tensor(sf, torch.float8_e4m3fn if nvfp4 else torch.float32, "sf")
+    _check(list(sf.shape) == lead + ([W // 64, _align_up(R, 16), 4] if nvfp4 else [_align_up(R, 16)]), "meet invalid sf shape")
+    planes = 1
+    for n in lead:
+        planes *= n
+    gs_step = 0
+    if nvfp4:
+        _check_tensor(global_scale, torch.float32, "global_scale")
+        _check(global_scale.dim() == 0 or list(global_scale.shape) == lead, "global_scale must be a scalar or have the leading dims of q")
+        gs_step = int(global_scale.dim() > 0)
+    else:
+        _check(global_scale is None, "only nvfp4 has a global scale")
+    _check(out.is_contiguous() and list(out.shape[:-1]) == lead + [R] and out.size(-1) <= W, "out must be contiguous of [.., {}, up to {}]", R, W)
+    if out.numel() == 0:
+        return
+    _lib.check(_L.ac4k_dequantize(out.data_ptr(), tag, q.data_ptr(), sf.data_ptr(), None if global_scale is None else global_scale.data_ptr(),
+                                  gs_step, planes, R, W, out.size(-1), 3 if nvfp4 else _EIGHT_BITS[q.dtype], _stream()))
+
+
+def rope(outs, xs, table, sections, positions, grid, bnhd: bool, interleaved: bool, inverse: bool) -> None:
+    """outs <- xs (one or two tensors) turned by the angles of their tokens' positions."""
+    _check(len(xs) in (1, 2) and len(outs) == len(xs), "rope takes one or two tensors, and as many outputs")
+    x = xs[0]
+    tag = _check_float(x, "x")
+    _check(x.dim() == 4, "x must be a 4D tensor")
+    B, D = x.size(0), x.size(3)
+    N = x.size(1 if bnhd else 2)
+    _check_tensor(table, torch.float32, "table")
+    _check(table.dim() == 3 and table.size(2) == 2 and table.size(0) >= 1 and table.size(1) >= 1, "table must be [length, pairs, 2]")
+    length, pairs = table.size(0), table.size(1)
+    _check(2 * pairs <= D, "{} pairs do not fit a head of {}", pairs, D)
+    axes = len(sections)
+    _check(1 <= axes <= 8 and sum(sections) == pairs and min(sections) >= 0, "sections must be 1 to 8 counts of pairs, {} in all", pairs)
+    _check((positions is None) != (grid is None), "positions or a grid, one of them")
+    _same_device(x.get_device(), table=table, positions=positions)
+    args = (_lib.RopeTensor * len(xs))()
+    n_dim, h_dim = (1, 2) if bnhd else (2, 1)
+    empty = B == 0 or N == 0
+    for i, (t, o) in enumerate(zip(xs, outs)):
+        _check(_check_float(t, "x") == tag and _check_float(o, "out") == tag, "all tensors must have one type")
+        _check(t.dim() == 4 and t.size(0) == B and t.size(n_dim) == N and t.size(3) == D, "all tensors must have the same batch, tokens and head dim")
+        _check(o.shape == t.shape, "out must have the shape of x")
+        _same_device(x.get_device(), x=t, out=o)
+        _check(t.stride(3) == 1 and o.stride(3) == 1, "heads must be contiguous")
+        _check(_same_rows(t, o) or not _may_overlap(t, o), "out may be x itself, but not overlap it otherwise")
+        empty = empty or t.size(h_dim) == 0
+        args[i] = _lib.RopeTensor(t.data_ptr(), o.data_ptr(), t.stride(0), t.stride(n_dim), t.stride(h_dim), o.stride(0), o.stride(n_dim),
+                                  o.stride(h_dim), t.size(h_dim))
+    if len(xs) == 2:
+        _check(not any(_may_overlap(o, t) for o, t in ((outs[0], xs[1]), (outs[1], xs[0]), (outs[0], outs[1])) if o.numel() and t.numel())
+               or _interleaved_heads(outs, xs), "the two tensors must not overlap each other")
+    pos_ptr, pos_bytes, pos_strides, grid_arg = None, 0, (0, 0, 0), None
+    if positions is not None:
+        _check(isinstance(positions, torch.Tensor) and positions.is_cuda and positions.dtype in (torch.int32, torch.int64), "positions must be a CUDA tensor of int32 or int64")
+        _check(list(positions.shape) == [axes, B, N], "positions must be [{}, {}, {}]", axes, B, N)
+        pos_ptr, pos_bytes, pos_strides = positions.data_ptr(), positions.element_size(), positions.stride()
+    else:
+        _check(len(grid) == axes and all(1 <= g for g in grid), "grid must have one size of at least 1 for each axis")
+        _check(max(grid) <= length, "the table has {} positions, the grid {}", length, max(grid))
+        grid_arg = (_lib._i64 * axes)(*grid)
+    if empty:
+        return
+    _lib.check(_L.ac4k_rope(args, len(xs), tag, B, N, D, table.data_ptr(), length, pairs, (_lib._i64 * axes)(*sections), axes, pos_ptr,
+                            pos_bytes, *pos_strides, grid_arg, int(interleaved), int(inverse), _stream()))
+
+
+def _interleaved_heads(outs, xs) -> bool:
+    """Whether two tensors are slices of the heads of one (q and k of a packed projection): same strides, apart by whole heads that neither
+    reaches into, and each output its input or memory of its own."""
+    (a, b), (c, d) = xs, outs
+    for p, q in ((a, b), (c, d), (c, b), (a, d)):
+        if not _may_overlap(p, q):
+            continue
+        if p.stride() != q.stride():
+            return False
+        away = (q.data_ptr() - p.data_ptr()) // p.element_size()
+        lo, hi = (p, q) if away >= 0 else (q, p)
+        away = abs(away)
+        # rows of the outermost strides stay apart when a row of `lo` ends before `hi` begins and `hi` ends before the next row of `lo`
+        dims = sorted((s, n) for s, n in zip(lo.stride(), lo.shape) if n > 1)
+        reach, step = 1, None
+        for s, n in dims:
+            if s > away:
+                step = s
+                break
+            reach = max(reach, (n - 1) * s + reach)
+        if step is None or reach > away:
+            return False
+        reach_hi = 1
+        for s, n in sorted((s, n) for s, n in zip(hi.stride(), hi.shape) if n > 1):
+            if s >= step:
+                break
+            reach_hi += (n - 1) * s
+        if away + reach_hi > step:
+            return False
+    return True
+
+
+def linear_grouped_nvfp4(D, A, A_sf, A_global_scale, B, B_sf, B_global_scale, offsets, rows=None, bias=None) -> None:
+    """D[i] = linear of row rows[i] (row i without rows) of A on the weight of the expert whose range of offsets holds i."""
+    M, N, tag = _check_output(D)
+    _check(isinstance(A, torch.Tensor) and A.dim() == 2, "a must be a 2d matrix")
+    T = A.size(0)
+    K = _check_linear_operand(A, A_sf, A_global_scale, T, "a")
+    _check(K >= 64 and K % 64 == 0, "K must be a multiple of 64 but see {}", K)
+    _check(isinstance(B, torch.Tensor) and B.dim() == 3, "b must be [experts, N, K/2]")
+    E = B.size(0)
+    _check(B.size(1) == N, "b size(1) must be {}", N)
+    _check(B.size(2) * 2 == K, "b size(2) must equal a size(1)")
+    _check_tensor(B, torch.uint8, "b")
+    _check_tensor(B_sf, torch.float8_e4m3fn, "scale_b")
+    _check(list(B_sf.shape) == [E, K // 64, _align_up(N, 16), 4], "scale_b has an invalid shape")
+    _check_tensor(B_global_scale, torch.float32, "global_scale_b")
+    _check(B_global_scale.dim() == 0 or list(B_global_scale.shape) == [E], "b_global_scale must be a scalar or one per expert")
+    _check_tensor(offsets, torch.int32, "offsets")
+    _check(list(offsets.shape) == [E + 1], "offsets must be [{}]", E + 1)
+    if rows is None:
+        _check(T == M, "A size(0) must be {}", M)
+    else:
+        _check_tensor(rows, torch.int32, "rows")
+        _check(list(rows.shape) == [M], "rows must be [{}]", M)
+    bias_ptr, bias_tag = None, 0
+    if bias is not None:
+        bias_tag = _check_float(bias, "bias")
+        _check(bias.is_contiguous() and list(bias.shape) == [E, N], "bias must be contiguous of [{}, {}]", E, N)
+        bias_ptr = bias.data_ptr()
+    _same_device(D.get_device(), a=A, scale_a=A_sf, global_scale_a=A_global_scale, b=B, scale_b=B_sf, global_scale_b=B_global_scale,
+                 offsets=offsets, rows=rows, bias=bias)
+    if M == 0 or N == 0 or E == 0:
+        return
+    _check(T > 0, "rows of an empty a")
+    nbytes = _L.ac4k_linear_grouped_nvfp4_workspace_bytes(M, N, K, E, int(rows is not None))
+    ws = D.new_empty((nbytes,), dtype=torch.uint8) if nbytes > 0 else None
+    _lib.check(_L.ac4k_linear_grouped_nvfp4(D.data_ptr(), tag, A.data_ptr(), A_sf.data_ptr(), A_global_scale.data_ptr(), T,
+                                            None if rows is None else rows.data_ptr(), B.data_ptr(), B_sf.data_ptr(),
+                                            B_global_scale.data_ptr(), int(B_global_scale.dim() > 0), bias_ptr, bias_tag,
+                                            offsets.data_ptr(), M, N, K, E, None if ws is None else ws.data_ptr(), nbytes, _stream()))

@@ -314,6 +314,70 @@ int ac4k_attention_nvfp4_bf16(void *O, int64_t o_b_stride, int64_t o_h_stride, i
                               float max_scale, float sm_scale, void *workspace, int64_t workspace_bytes,
                               ac4k_stream_t stream);
 
+/* Operators around the quantized linears and the attention of a transformer layer; the reference holds none of the first three.
+ *
+ * Formats of ac4k_rms_norm's output and of ac4k_dequantize's input: those of the quantizers above. */
+enum { AC4K_PRECISION_NONE = 0, AC4K_PRECISION_FP8 = 1, AC4K_PRECISION_INT8 = 2, AC4K_PRECISION_NVFP4 = 3 };
+#define AC4K_NORM_MAX_COLS 65536
+
+/* Root-mean-square norm of the rows of x [rows, K] (dtype: one of the tags above; strides in elements, elements of a row contiguous):
+ *   h = x, or x + residual rounded to dtype, which is written to `sum` (which may be x or residual itself);
+ *   y = h * fp32(1 / sqrt(mean(h^2) + eps)) * weight, weight [K] of dtype or fp32, or NULL; the sum of squares in 64 bits.
+ * precision NONE: out [rows, K] of dtype (out_stride; it may be x).  Otherwise y in fp32 goes straight into the format of a quantizer:
+ *   FP8 / INT8: out [rows, align_up(K,16)], sf fp32 [align_up(rows,16)] = max|y| / 448 or 127;
+ *   NVFP4: out [rows, align_up(K,64)/2], sf [align_up(K,64)/64, align_up(rows,16), 4]; *global_scale is read where given_scale != 0, otherwise
+ *   written: max|y| / 2688 over all rows.
+ * Every byte of out and sf is written, zeros in the padding.  A row (nvfp4: a tensor) whose max|y| is under 2^-100 gives zero codes and
+ * scales, and so does a given scale under 2^-112.  K <= AC4K_NORM_MAX_COLS.  `workspace`: ac4k_rms_norm_workspace_bytes, on 4 bytes, contents irrelevant, NULL when that is 0
+ * (it is for everything but nvfp4 whose scale is to be found). */
+int64_t ac4k_rms_norm_workspace_bytes(int64_t rows, int64_t K, int dtype, int precision, int given_scale);
+int ac4k_rms_norm(void *out, int64_t out_stride, void *sf, float *global_scale, int given_scale, const void *x, int64_t x_stride,
+                  const void *residual, int64_t residual_stride, void *sum, int64_t sum_stride, const void *weight,
+                  int weight_dtype, int64_t rows, int64_t K, int dtype, int precision, double eps, void *workspace,
+                  int64_t workspace_bytes, ac4k_stream_t stream);
+
+/* Values of quantized rows (no swizzle): out [lead, R, cols] of dtype = q * sf, for nvfp4 times global_scale[l * global_scale_stride] (stride 0: one
+ * scale for all).  W: elements of a quantized row, padding included (nvfp4: a multiple of 64, 8 bits: of 16); cols <= W of them are written.
+ * q [lead, R, W/2] and sf [lead, W/64, align_up(R,16), 4] for nvfp4, q [lead, R, W] and sf fp32 [lead, align_up(R,16)] for 8 bits. */
+int ac4k_dequantize(void *out, int dtype, const void *q, const void *sf, const float *global_scale, int64_t global_scale_stride,
+                    int64_t lead, int64_t R, int64_t W, int64_t cols, int precision, ac4k_stream_t stream);
+
+/* Rotary positions with several axes, for one or two tensors [B, N, heads, D] (any strides of the first three dims, in elements; a
+ * head contiguous) that share their tokens' positions; out may be in.  Takes the place of ac4k::rope3d (lib/cuda/sm120/rope3d.cu:23-129)
+ * and of tables with any number of axes besides.
+ *   table: fp32 [length, pairs, 2], cosine and sine of the angle of a pair at a position (on 8 bytes);
+ *   sections [axes] (host): pairs of each axis, in order, `pairs` in all; pair j is elements (2j, 2j+1) of a head, or with
+ *   interleaved == 0 (j, j + pairs); elements from 2 * pairs on are copied;
+ *   positions: int32 or int64 (positions_bytes) with strides (axis, b, n) in elements, or NULL with a grid [axes] (host) instead:
+ *   token n then sits at the n-th place of the grid in row-major order, and tokens behind its last place stay as they are.
+ * A token with a negative position along any axis stays as it is; a position of `length` or more gives NaN in the pairs of its axis.
+ * inverse != 0 turns the other way: the gradient. */
+#define AC4K_ROPE_MAX_AXES 8
+#define AC4K_ROPE_MAX_DIM 1024
+typedef struct {
+  const void *in;
+  void *out;
+  int64_t in_b_stride, in_n_stride, in_h_stride, out_b_stride, out_n_stride, out_h_stride;
+  int64_t heads;
+} ac4k_rope_tensor;
+int ac4k_rope(const ac4k_rope_tensor *tensors, int count, int dtype, int64_t B, int64_t N, int64_t D, const float *table,
+              int64_t length, int64_t pairs, const int64_t *sections, int axes, const void *positions, int positions_bytes,
+              int64_t pos_axis_stride, int64_t pos_b_stride, int64_t pos_n_stride, const int64_t *grid, int interleaved,
+              int inverse, ac4k_stream_t stream);
+
+/* Linears grouped by expert (no counterpart in the reference; beside ac4k_linear_nvfp4):
+ *   D[i] = (A[rows[i]] . B[e]^T) * (*A_gs * B_gs[e * B_gs_stride]) + bias[e]   for offsets[e] <= i < offsets[e+1].
+ * D [M,N] (d_dtype); A [T,K/2] with A_sf [K/64,align_up(T,16),4]; rows int32 [M] (device), or NULL: row i itself, T == M;
+ * B [E,N,K/2] with B_sf [E,K/64,align_up(N,16),4]; B_gs: one scale (stride 0) or one per expert (stride 1); bias [E,N] or NULL;
+ * offsets int32 [E+1] (device), rising.  Rows of D that no range holds stay as they are.  The library never waits for
+ * the offsets.  Offsets are clamped to [0, M] and row indexes to [0, T): wrong ones give wrong rows, never an access out of range.
+ * K % 64 == 0; A and B on 16 bytes.  `workspace`: ac4k_linear_grouped_nvfp4_workspace_bytes(M, N, K, E, rows != NULL), on 16 bytes. */
+int64_t ac4k_linear_grouped_nvfp4_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t E, int has_rows);
+int ac4k_linear_grouped_nvfp4(void *D, int d_dtype, const void *A, const void *A_sf, const float *A_gs, int64_t T,
+                              const int32_t *rows, const void *B, const void *B_sf, const float *B_gs, int64_t B_gs_stride,
+                              const void *bias, int bias_dtype, const int32_t *offsets, int64_t M, int64_t N, int64_t K,
+                              int64_t E, void *workspace, int64_t workspace_bytes, ac4k_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
