@@ -700,7 +700,7 @@ def linear_grouped_nvfp4(D, A, A_sf, A_global_scale, B, B_sf, B_global_scale, of
     if M == 0 or N == 0 or E == 0:
         return
     _check(T > 0, "rows of an empty a")
-    nbytes = _L.ac4k_linear_grouped_nvfp4_workspace_bytes(M, N, K, E, int(rows is not None))
+    nbytes = _L.ac4k_linear_grouped_nvfp4_workspace_bytes(T, M, N, K, E, int(rows is not None))
     ws = D.new_empty((nbytes,), dtype=torch.uint8) if nbytes > 0 else None
     _lib.check(_L.ac4k_linear_grouped_nvfp4(D.data_ptr(), tag, A.data_ptr(), A_sf.data_ptr(), A_global_scale.data_ptr(), T,
                                             None if rows is None else rows.data_ptr(), B.data_ptr(), B_sf.data_ptr(),

@@ -6,7 +6,9 @@
 // The sizes of the groups are on the GPU and nothing waits for them: launches are made for the largest number of tiles that the row and
 // expert counts allow, and workgroups without a tile end at once.  Offsets are taken as clamped to [0, rows] and rising, row indexes as
 // clamped to x: a wrong table gives wrong rows, not an access outside of the operands.  Output rows that no group holds stay as they are.
-#include "linear_common.h"
+#include <math.h>
+
+#include "linear_tile.h"
 
 namespace ac4k {
 
@@ -128,8 +130,141 @@ __global__ __launch_bounds__(64 * R16_WAVES, 2) void linear_grouped_rows16_kerne
   }
 }
 
+// ===========================================================================
+// The tile kernel of the linears on the tiles of all groups.  A group's tiles start at a multiple of four rows, at or in front of its first one (a
+// transfer of scales is four rows), and go up to its end; the tiles of all groups are one sequence, dealt to the XCDs and walked in bands as
+// those of one matrix are.  Every workgroup finds its tile by itself: the tile counts of 64 experts a step, one a lane, summed over the wave.
+// ===========================================================================
+template <int BM>
+__device__ __forceinline__ int group_tiles(const Group &g) {
+  return g.count == 0 ? 0 : ((g.first & 3) + g.count + BM - 1) / BM;
+}
+__device__ __forceinline__ int wave_prefix(int v) {  // inclusive
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int o = __shfl_up(v, d, 64);
+    v += lane >= d ? o : 0;
+  }
+  return v;
+}
+
+struct GroupTile {
+  int e, first, count, tile, tn;  // tile: index inside the group; e < 0: none
+};
+template <int BM, int BN>
+__device__ __forceinline__ GroupTile tile_of_groups(const GroupedArgs &a) {
+  const int lane = threadIdx.x & 63, E = (int)a.E;
+  const uint32_t tiles_n = (uint32_t)ceil_div(a.N, BN);
+  int64_t sum = 0;
+  Group grp{0, 0};
+  int incl = 0;
+  for (int base = 0; base < E; base += 64) {
+    grp = base + lane < E ? group_of(a.offsets, base + lane, a.M) : Group{0, 0};
+    incl = wave_prefix(group_tiles<BM>(grp));
+    sum += __builtin_amdgcn_readlane(incl, 63);
+  }
+  // (offsets that overlap could name more tiles than the launch has)
+  const uint32_t most = gridDim.x / tiles_n;
+  const uint32_t total = (uint32_t)__builtin_amdgcn_readfirstlane((int)(sum < most ? sum : most));
+  if (blockIdx.x >= total * tiles_n) return {-1, 0, 0, 0, 0};
+  const TileCoord tc = tile_of_workgroup<4>(blockIdx.x, total, tiles_n);
+  const int tm = __builtin_amdgcn_readfirstlane((int)tc.m);
+  int before = 0, base = 0;
+  if (E > 64) {
+    for (; base < E; base += 64) {
+      grp = base + lane < E ? group_of(a.offsets, base + lane, a.M) : Group{0, 0};
+      incl = wave_prefix(group_tiles<BM>(grp));
+      const int here = __builtin_amdgcn_readlane(incl, 63);
+      if (tm < before + here) break;  // (some step has it: tm < total)
+      before += here;
+    }
+  }
+  const int l = __builtin_ctzll(__ballot(before + incl > tm));
+  const int tiles = __builtin_amdgcn_readlane(group_tiles<BM>(grp), l);
+  return {base + l, __builtin_amdgcn_readlane(grp.first, l), __builtin_amdgcn_readlane(grp.count, l), tm - (before + __builtin_amdgcn_readlane(incl, l) - tiles),
+          __builtin_amdgcn_readfirstlane((int)tc.n)};
+}
+
+template <int D_DT, int BIAS_DT, int MI, int NJ, int PS, int KW, bool EARLY, int PER_CU>
+__global__ __launch_bounds__(256, PER_CU) void linear_grouped_tile_kernel(GroupedArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char plds[];
+  constexpr int BM = 64 * MI, BN = 64 * NJ;
+  const GroupTile t = tile_of_groups<BM, BN>(a);
+  if (t.e < 0) return;
+  const int64_t kb = a.K >> 1, e = t.e;
+  LinearArgs la{a.D, a.A, a.B + e * a.N * kb, a.A_sf, a.B_sf + e * (a.K >> 6) * a.Np, a.A_gs, a.B_gs + e * a.B_gs_stride, nullptr,
+                t.first + t.count, a.N, a.K, a.Tp, a.Np};
+  if constexpr (BIAS_DT != BIAS_NONE) la.bias = static_cast<const typename Elem<BIAS_DT>::T *>(a.bias) + e * a.N;
+  tile256p<D_DT, BIAS_DT, MI, NJ, PS, KW, EARLY, true>(la, SplitK{nullptr, 1}, plds, TileRows{(t.first & ~3) + (int64_t)t.tile * BM, t.first, a.rows, a.T}, t.tn);
+}
+
+// Scales of gathered rows, a column for each row of the output: the tile kernel fetches those of four neighbours at once.
+__global__ __launch_bounds__(256) void gather_scales_kernel(uint32_t *out, const uint32_t *sf, const int32_t *rows, int64_t M, int64_t Mp, int64_t T,
+                                                            int64_t Tp) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, chunk = blockIdx.y;
+  if (i >= Mp) return;
+  int64_t row = i < M ? rows[i] : 0;
+  row = row < 0 ? 0 : row < T ? row : T - 1;
+  out[chunk * Mp + i] = i < M ? sf[chunk * Tp + row] : 0u;
+}
+
+enum GroupedKind { GROUPED_ROWS16, GROUPED_64_128, GROUPED_64_256, GROUPED_256_256 };
+
+// (the tile kernel's 32-bit lane offsets: whole of x where rows are gathered, the rows of a tile and of a band otherwise)
+static bool grouped_tiles_fit(int64_t T, int64_t N, int64_t K, bool gather) {
+  return K >= P_BK && N >= 128 && (K >> 1) * 260 < (1ll << 31) && (!gather || T * (K >> 1) < (1ll << 32) - 64) && N < (1ll << 27);
+}
+// Which kernel, by the time that each is expected to take (us), fitted to 100 shapes of 8 to 128 experts, N of 1003 to 14336, K of 2048 to 14336 and 1 to
+// 2048 rows an expert.  What is known on the host are the counts; the groups are taken for those of rows dealt out evenly at random.  A tile of a
+// shape takes so long for each 4096 of K, and so long besides, with its CU full of them; tiles go to the CUs in whole rounds while these
+// are few.  64 x 256 and 64 x 128 tiles are two to a CU: memory latency and the exchange at the end of one lie under the other's work.
+// Measured, us (256 x 256 / 64 x 256 / 64 x 128 / 16 rows):  8 experts of 14336 x 4096, 2 rows each 162 / 57 / 66 / 80, 128 157 / 137 / 147 / 570,
+// 2048 1291 / 1498 / 1795; 8 of 4096 x 14336, 8 rows 236 / 92 / 69 / 73; 16 of 4096 x 4096, 512 rows 237 / 235 / 274; 128 x 128 tiles, one or two to a CU,
+// were nowhere more than 6 % ahead of the best of these.
+static GroupedKind grouped_kind(int64_t T, int64_t M, int64_t N, int64_t K, int64_t E, bool gather) {
+  if (!grouped_tiles_fit(T, N, K, gather)) return GROUPED_ROWS16;
+  const int cu = device_cu_count();
+  const double cus = cu > 0 ? cu : 256, k = (double)K / 4096;
+  const double groups = (double)E * -expm1((double)M * log1p(-1.0 / ((double)E + 1e-9)));  // that have rows
+  auto tiles = [&](int bm, int bn) {  // a CU
+    const double m = (double)M / bm + groups / 2;
+    return (m > groups ? m : groups) * (double)ceil_div(N, bn) / cus;
+  };
+  auto rounds = [](double x) { return x <= 3 ? ceil(x) : x + 0.25; };
+  const double launch = 6, t256 = launch + rounds(tiles(256, 256)) * (76 * k + 10.5), t64 = launch + rounds(tiles(64, 256)) * (24.3 * k + 2.5);
+  const double x = tiles(64, 128), t128 = launch + (x <= 1 ? 19 * k + 1 : rounds(x) * (14 * k + 1.7));
+  GroupedKind kind = t256 < t64 ? GROUPED_256_256 : GROUPED_64_256;
+  double best = t256 < t64 ? t256 : t64;
+  if (t128 < best) kind = GROUPED_64_128, best = t128;
+  if ((double)M <= 16 * groups && 8 + groups * (double)N * (double)K * 0.5625 / 3.5e6 < best) kind = GROUPED_ROWS16;  // bytes of the weights
+  return kind;
+}
+
+template <int D_DT, int BIAS_DT, int MI, int NJ, int KW, int PS, int PER_CU>
+static int launch_grouped_tile(const GroupedArgs &a, hipStream_t st) {
+  constexpr int BM = 64 * MI;
+  const bool early = a.K % P_BK != 0;
+  auto *kern = early ? linear_grouped_tile_kernel<D_DT, BIAS_DT, MI, NJ, PS, KW, true, PER_CU> : linear_grouped_tile_kernel<D_DT, BIAS_DT, MI, NJ, PS, KW, false, PER_CU>;
+  using PL = PLayout<BM, 64 * NJ, PS>;
+  static std::atomic<uint32_t> lds_ok[2];
+  if (int rc = allow_dynamic_lds(kern, lds_ok[early], PL::LDS_BYTES)) return rc;
+  // rows in tiles, and at most one tile more for each group that has rows
+  const int64_t groups = a.E < a.M ? a.E : a.M;
+  const int64_t tiles = (a.M + groups * (BM + 2)) / BM * ceil_div(a.N, 64 * NJ);
+  AC4K_REQUIRE(tiles < (1ll << 24), "problem too large");  // 2^32 threads a launch
+  hipLaunchKernelGGL(kern, dim3((unsigned)tiles), dim3(256), PL::LDS_BYTES, st, a);
+  return 0;
+}
+
 template <int D_DT, int BIAS_DT>
-static int launch_grouped(const GroupedArgs &a, hipStream_t st) {
+static int launch_grouped(const GroupedArgs &a, GroupedKind kind, hipStream_t st) {
+  switch (kind) {
+    case GROUPED_256_256: return launch_grouped_tile<D_DT, BIAS_DT, 4, 4, 1, 3, 1>(a, st);
+    case GROUPED_64_256: return launch_grouped_tile<D_DT, BIAS_DT, 1, 4, 2, 3, 2>(a, st);
+    case GROUPED_64_128: return launch_grouped_tile<D_DT, BIAS_DT, 1, 2, 2, 5, 2>(a, st);
+    case GROUPED_ROWS16: break;
+  }
   const dim3 grid((unsigned)ceil_div(a.N, R16_ROWS), (unsigned)a.E);
   if (a.M <= 16 * a.E) hipLaunchKernelGGL((linear_grouped_rows16_kernel<D_DT, BIAS_DT, 1>), grid, dim3(64 * R16_WAVES), 0, st, a);
   else hipLaunchKernelGGL((linear_grouped_rows16_kernel<D_DT, BIAS_DT, 2>), grid, dim3(64 * R16_WAVES), 0, st, a);
@@ -137,12 +272,12 @@ static int launch_grouped(const GroupedArgs &a, hipStream_t st) {
 }
 
 template <int D_DT>
-static int grouped_bias(const GroupedArgs &a, int bias_dtype, hipStream_t st) {
-  if (!a.bias) return launch_grouped<D_DT, BIAS_NONE>(a, st);
+static int grouped_bias(const GroupedArgs &a, int bias_dtype, GroupedKind kind, hipStream_t st) {
+  if (!a.bias) return launch_grouped<D_DT, BIAS_NONE>(a, kind, st);
   switch (bias_dtype) {
-    case AC4K_DTYPE_BF16: return launch_grouped<D_DT, AC4K_DTYPE_BF16>(a, st);
-    case AC4K_DTYPE_FP16: return launch_grouped<D_DT, AC4K_DTYPE_FP16>(a, st);
-    case AC4K_DTYPE_FP32: return launch_grouped<D_DT, AC4K_DTYPE_FP32>(a, st);
+    case AC4K_DTYPE_BF16: return launch_grouped<D_DT, AC4K_DTYPE_BF16>(a, kind, st);
+    case AC4K_DTYPE_FP16: return launch_grouped<D_DT, AC4K_DTYPE_FP16>(a, kind, st);
+    case AC4K_DTYPE_FP32: return launch_grouped<D_DT, AC4K_DTYPE_FP32>(a, kind, st);
   }
   return set_error("bias must be bfloat16, half or float (dtype tag %d)", bias_dtype);
 }
@@ -151,8 +286,10 @@ static int grouped_bias(const GroupedArgs &a, int bias_dtype, hipStream_t st) {
 
 using namespace ac4k;
 
-extern "C" __attribute__((visibility("default"))) int64_t ac4k_linear_grouped_nvfp4_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t E, int has_rows) {
-  return 0;
+extern "C" __attribute__((visibility("default"))) int64_t ac4k_linear_grouped_nvfp4_workspace_bytes(int64_t T, int64_t M, int64_t N, int64_t K, int64_t E,
+                                                                                                   int has_rows) {
+  if (T < 1 || M < 1 || N < 1 || K < 64 || K % 64 != 0 || E < 1 || !has_rows || grouped_kind(T, M, N, K, E, true) == GROUPED_ROWS16) return 0;
+  return K / 64 * align_up(M, 16) * 4;
 }
 
 extern "C" __attribute__((visibility("default"))) int ac4k_linear_grouped_nvfp4(
@@ -171,11 +308,24 @@ extern "C" __attribute__((visibility("default"))) int ac4k_linear_grouped_nvfp4(
   GroupedArgs a{D, static_cast<const uint8_t *>(A), static_cast<const uint32_t *>(A_sf), A_gs, rows, static_cast<const uint8_t *>(B),
                 static_cast<const uint32_t *>(B_sf), B_gs, B_gs_stride, bias, offsets, T, align_up(T, 16), M, N, align_up(N, 16), K, E};
   hipStream_t st = (hipStream_t)stream;
+  const GroupedKind kind = grouped_kind(T, M, N, K, E, rows != nullptr);
+  const int64_t need = ac4k_linear_grouped_nvfp4_workspace_bytes(T, M, N, K, E, rows != nullptr);
+  AC4K_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0), "workspace of %lld bytes needed, on 16 bytes",
+               (long long)need);
+  AC4K_REQUIRE(d_dtype == AC4K_DTYPE_BF16 || d_dtype == AC4K_DTYPE_FP16 || d_dtype == AC4K_DTYPE_FP32, "d must be bfloat16, half or float (dtype tag %d)", d_dtype);
+  AC4K_REQUIRE(!bias || bias_dtype == AC4K_DTYPE_BF16 || bias_dtype == AC4K_DTYPE_FP16 || bias_dtype == AC4K_DTYPE_FP32,
+               "bias must be bfloat16, half or float (dtype tag %d)", bias_dtype);
+  if (need > 0) {
+    hipLaunchKernelGGL(gather_scales_kernel, dim3((unsigned)ceil_div(align_up(M, 16), 256), (unsigned)(K / 64)), dim3(256), 0, st,
+                       static_cast<uint32_t *>(workspace), a.A_sf, rows, M, align_up(M, 16), T, a.Tp);
+    a.A_sf = static_cast<const uint32_t *>(workspace);
+    a.Tp = align_up(M, 16);
+  }
   int rc;
   switch (d_dtype) {
-    case AC4K_DTYPE_BF16: rc = grouped_bias<AC4K_DTYPE_BF16>(a, bias_dtype, st); break;
-    case AC4K_DTYPE_FP16: rc = grouped_bias<AC4K_DTYPE_FP16>(a, bias_dtype, st); break;
-    case AC4K_DTYPE_FP32: rc = grouped_bias<AC4K_DTYPE_FP32>(a, bias_dtype, st); break;
+    case AC4K_DTYPE_BF16: rc = grouped_bias<AC4K_DTYPE_BF16>(a, bias_dtype, kind, st); break;
+    case AC4K_DTYPE_FP16: rc = grouped_bias<AC4K_DTYPE_FP16>(a, bias_dtype, kind, st); break;
+    case AC4K_DTYPE_FP32: rc = grouped_bias<AC4K_DTYPE_FP32>(a, bias_dtype, kind, st); break;
     default: return set_error("d must be bfloat16, half or float (dtype tag %d)", d_dtype);
   }
   if (rc) return rc;

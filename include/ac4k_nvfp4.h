@@ -371,8 +371,8 @@ int ac4k_rope(const ac4k_rope_tensor *tensors, int count, int dtype, int64_t B, 
  * B [E,N,K/2] with B_sf [E,K/64,align_up(N,16),4]; B_gs: one scale (stride 0) or one per expert (stride 1); bias [E,N] or NULL;
  * offsets int32 [E+1] (device), rising.  Rows of D that no range holds stay as they are.  The library never waits for
  * the offsets.  Offsets are clamped to [0, M] and row indexes to [0, T): wrong ones give wrong rows, never an access out of range.
- * K % 64 == 0; A and B on 16 bytes.  `workspace`: ac4k_linear_grouped_nvfp4_workspace_bytes(M, N, K, E, rows != NULL), on 16 bytes. */
-int64_t ac4k_linear_grouped_nvfp4_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t E, int has_rows);
+ * K % 64 == 0; A and B on 16 bytes.  `workspace`: ac4k_linear_grouped_nvfp4_workspace_bytes(T, M, N, K, E, rows != NULL), on 16 bytes (0 where no scales are gathered). */
+int64_t ac4k_linear_grouped_nvfp4_workspace_bytes(int64_t T, int64_t M, int64_t N, int64_t K, int64_t E, int has_rows);
 int ac4k_linear_grouped_nvfp4(void *D, int d_dtype, const void *A, const void *A_sf, const float *A_gs, int64_t T,
                               const int32_t *rows, const void *B, const void *B_sf, const float *B_gs, int64_t B_gs_stride,
                               const void *bias, int bias_dtype, const int32_t *offsets, int64_t M, int64_t N, int64_t K,
