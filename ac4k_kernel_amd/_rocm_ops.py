@@ -461,23 +461,31 @@ _EIGHT_BITS = {torch.float8_e4m3fn: 1, torch.int8: 2}
 
 
 def _check_float(t, name: str) -> int:
+    if isinstance(t, torch.Tensor) and t.is_cuda:
+        tag = _DTYPE_TAG.get(t.dtype)
+        if tag is not None:
+            return tag
     _check(isinstance(t, torch.Tensor), "{} must be a tensor", name)
     _check(t.is_cuda, "{} must be a CUDA tensor", name)
     _check(t.dtype in _DTYPE_TAG, "{} must be bfloat16, half or float", name)
     return _DTYPE_TAG[t.dtype]
 
 
-def _same_device(dev: int, **tensors) -> None:
+def _same_device(*tensors) -> None:
     """Kernels run on the current device and its stream: every operand has to be there."""
-    _check(dev == _current_device(), "operands on device {}, the current device is {}", dev, _current_device())
-    for name, t in tensors.items():
-        _check(t is None or t.get_device() == dev, "{} is on another device than the first operand", name)
+    dev = _current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            _check(False, "operands must be on the current device, {}: got one on {}", dev, t.device)
 
 
 def _rows_view(t, name: str):
     """t [.., K] as rows: (rows, K, elements between rows) of the tensor itself, or None if no single row stride describes it."""
     shape, stride = t.shape, t.stride()
-    _check(t.dim() >= 1 and shape[-1] >= 1, "{} must have a last dim of at least one element", name)
+    if not shape or shape[-1] < 1:
+        _check(False, "{} must have a last dim of at least one element", name)
+    if t.is_contiguous():
+        return t.numel() // shape[-1], shape[-1], shape[-1]
     rows, step = 1, 0
     if shape[-1] > 1 and stride[-1] != 1:
         return None
@@ -505,57 +513,70 @@ def _same_rows(a, b) -> bool:
     return a.data_ptr() == b.data_ptr() and a.stride() == b.stride()
 
 
-def rms_norm(out, sf, global_scale, given_scale: bool, x, weight, residual, residual_out, precision, eps: float) -> None:
-    """out (and sf, global_scale) <- norm of the rows of x, or of x + residual, which residual_out receives."""
+def rms_norm(out, sf, global_scale, given_scale: bool, x, weight, residual, residual_out, precision, eps: float, view=None, fresh=False) -> None:
+    """out (and sf, global_scale) <- norm of the rows of x, or of x + residual, which residual_out receives.  view: _rows_view(x), where the
+    caller has it; fresh: out, sf and residual_out are new dense tensors of the right shapes and overlap nothing."""
     tag = _check_float(x, "x")
-    view = _rows_view(x, "x")
+    view = view or _rows_view(x, "x")
     _check(view is not None, "x must have rows of contiguous elements, evenly apart")
     rows, K, x_step = view
-    _check(precision in _PRECISIONS, "precision must be one of {}", list(_PRECISIONS))
-    _same_device(x.get_device(), weight=weight, residual=residual, residual_out=residual_out, out=out, sf=sf, global_scale=global_scale)
+    number = _PRECISIONS.get(precision)
+    if number is None:
+        _check(False, "precision must be one of {}", list(_PRECISIONS))
+    _same_device(x, weight, residual, residual_out, out, sf, global_scale)
+    weight_ptr, weight_tag = None, tag
     if weight is not None:
-        _check(_check_float(weight, "weight") == tag or weight.dtype == torch.float32, "weight must have the type of x or be float")
-        _check(weight.dim() == 1 and weight.size(0) == K and weight.is_contiguous(), "weight must be contiguous of [{}]", K)
+        weight_tag = _check_float(weight, "weight")
+        _check(weight_tag == tag or weight_tag == 2, "weight must have the type of x or be float")
+        if weight.shape != (K,) or not weight.is_contiguous():
+            _check(False, "weight must be contiguous of [{}]", K)
+        weight_ptr = weight.data_ptr()
     _check((residual is None) == (residual_out is None), "a residual comes with residual_out, and the other way round")
-    steps = [0, 0]
+    residual_ptr = sum_ptr = None
+    residual_step = sum_step = 0
     if residual is not None:
-        for i, (t, name) in enumerate(((residual, "residual"), (residual_out, "residual_out"))):
-            _check(_check_float(t, name) == tag and t.shape == x.shape, "{} must have the type and shape of x", name)
-            v = _rows_view(t, name)
-            _check(v is not None, "{} must have rows of contiguous elements, evenly apart", name)
-            steps[i] = v[2]
-        _check(rows <= 1 or abs(steps[1]) >= K, "residual_out must have rows of its own")
-        for t in (x, residual):
-            _check(_same_rows(t, residual_out) or not _may_overlap(t, residual_out),
-                   "residual_out may be x or residual itself, but not overlap them otherwise")
-    out_step = 0
-    if precision is None:
-        _check(_check_float(out, "out") == tag and out.shape == x.shape, "out must have the type and shape of x")
-        v = _rows_view(out, "out")
-        _check(v is not None and (rows <= 1 or abs(v[2]) >= K), "out must have rows of contiguous elements, evenly apart")
-        out_step = v[2]
-        _check(_same_rows(out, x) or not _may_overlap(out, x), "out may be x itself, but not overlap it otherwise")
-        for t in (residual, residual_out):
-            _check(t is None or not _may_overlap(out, t), "out must not overlap residual or residual_out")
-    else:
-        nvfp4 = precision == "nvfp4"
-        _check_tensor(out, torch.uint8 if nvfp4 else torch.float8_e4m3fn if precision == "fp8e4m3" else torch.int8, "out")
-        _check(list(out.shape) == [rows, _align_up(K, 64) // 2 if nvfp4 else _align_up(K, 16)], "meet invalid out shape")
-        _check_tensor(sf, torch.float8_e4m3fn if nvfp4 else torch.float32, "sf")
-        _check(list(sf.shape) == ([_align_up(K, 64) // 64, _align_up(rows, 16), 4] if nvfp4 else [_align_up(rows, 16)]), "meet invalid sf shape")
-        if nvfp4:
-            _check_tensor(global_scale, torch.float32, "global_scale")
-            _check(global_scale.dim() == 0, "global_scale must be a scalar")
+        _check(_check_float(residual, "residual") == tag and residual.shape == x.shape, "residual must have the type and shape of x")
+        v = _rows_view(residual, "residual")
+        _check(v is not None, "residual must have rows of contiguous elements, evenly apart")
+        residual_ptr, residual_step, sum_ptr, sum_step = residual.data_ptr(), v[2], residual_out.data_ptr(), K
+        if not fresh:
+            _check(_check_float(residual_out, "residual_out") == tag and residual_out.shape == x.shape, "residual_out must have the type and shape of x")
+            v = _rows_view(residual_out, "residual_out")
+            _check(v is not None and (rows <= 1 or v[2] >= K), "residual_out must have rows of contiguous elements, evenly apart")
+            sum_step = v[2]
+            for t in (x, residual):
+                _check(_same_rows(t, residual_out) or not _may_overlap(t, residual_out),
+                       "residual_out may be x or residual itself, but not overlap them otherwise")
+    out_step = K
+    if not fresh:
+        if precision is None:
+            _check(_check_float(out, "out") == tag and out.shape == x.shape, "out must have the type and shape of x")
+            v = _rows_view(out, "out")
+            _check(v is not None and (rows <= 1 or v[2] >= K), "out must have rows of contiguous elements, evenly apart")
+            out_step = v[2]
+            _check(_same_rows(out, x) or not _may_overlap(out, x), "out may be x itself, but not overlap it otherwise")
+            for t in (residual, residual_out):
+                _check(t is None or not _may_overlap(out, t), "out must not overlap residual or residual_out")
+        else:
+            nvfp4 = precision == "nvfp4"
+            _check_tensor(out, torch.uint8 if nvfp4 else torch.float8_e4m3fn if precision == "fp8e4m3" else torch.int8, "out")
+            _check(list(out.shape) == [rows, _align_up(K, 64) // 2 if nvfp4 else _align_up(K, 16)], "meet invalid out shape")
+            _check_tensor(sf, torch.float8_e4m3fn if nvfp4 else torch.float32, "sf")
+            _check(list(sf.shape) == ([_align_up(K, 64) // 64, _align_up(rows, 16), 4] if nvfp4 else [_align_up(rows, 16)]), "meet invalid sf shape")
+    if global_scale is not None:
+        _check_tensor(global_scale, torch.float32, "global_scale")
+        _check(global_scale.dim() == 0, "global_scale must be a scalar")
     if rows == 0:
         return
-    nbytes = _L.ac4k_rms_norm_workspace_bytes(rows, K, tag, _PRECISIONS[precision], int(given_scale))
-    ws = x.new_empty((nbytes,), dtype=torch.uint8) if nbytes > 0 else None
+    ws_ptr, nbytes = None, 0
+    if number == 3 and not given_scale:
+        nbytes = _L.ac4k_rms_norm_workspace_bytes(rows, K, tag, number, 0)
+        if nbytes > 0:
+            ws = x.new_empty((nbytes,), dtype=torch.uint8)
+            ws_ptr = ws.data_ptr()
     _lib.check(_L.ac4k_rms_norm(out.data_ptr(), out_step, None if sf is None else sf.data_ptr(),
                                 None if global_scale is None else global_scale.data_ptr(), int(given_scale), x.data_ptr(), x_step,
-                                None if residual is None else residual.data_ptr(), steps[0],
-                                None if residual is None else residual_out.data_ptr(), steps[1],
-                                None if weight is None else weight.data_ptr(), tag if weight is None else _DTYPE_TAG[weight.dtype],
-                                rows, K, tag, _PRECISIONS[precision], float(eps), None if ws is None else ws.data_ptr(), nbytes,
+                                residual_ptr, residual_step, sum_ptr, sum_step, weight_ptr, weight_tag, rows, K, tag, number, eps, ws_ptr, nbytes,
                                 _stream()))
 
 
@@ -566,7 +587,7 @@ def dequantize(out, q, sf, global_scale=None) -> None:
     nvfp4 = q.dtype == torch.uint8
     _check(nvfp4 or q.dtype in _EIGHT_BITS, "q must be uint8 (nvfp4), float8_e4m3fn or int8")
     _check_tensor(q, q.dtype, "q")
-    _same_device(q.get_device(), out=out, sf=sf, global_scale=global_scale)
+    _same_device(q, out, sf, global_scale)
     lead, R, W = list(q.shape[:-2]), q.size(-2), q.size(-1) * (2 if nvfp4 else 1)
     _check(W % (64 if nvfp4 else 16) == 0, "rows of q must be whole pieces of {} elements", 64 if nvfp4 else 16)
     _check_tensor(sf, torch.float8_e4m3fn if nvfp4 else torch.float32, "sf")
@@ -588,51 +609,83 @@ def dequantize(out, q, sf, global_scale=None) -> None:
                                   gs_step, planes, R, W, out.size(-1), 3 if nvfp4 else _EIGHT_BITS[q.dtype], _stream()))
 
 
-def rope(outs, xs, table, sections, positions, grid, bnhd: bool, interleaved: bool, inverse: bool) -> None:
-    """outs <- xs (one or two tensors) turned by the angles of their tokens' positions."""
-    _check(len(xs) in (1, 2) and len(outs) == len(xs), "rope takes one or two tensors, and as many outputs")
+_ROPE_SECTIONS = {}
+
+
+def _rope_sections(sections, pairs: int):
+    """The C array of a tuple of sections, checked against the table; kept by its values."""
+    got = _ROPE_SECTIONS.get((sections, pairs))
+    if got is None:
+        _check(1 <= len(sections) <= 8 and sum(sections) == pairs and min(sections) >= 0, "sections must be 1 to 8 counts of pairs, {} in all", pairs)
+        if len(_ROPE_SECTIONS) > 64:
+            _ROPE_SECTIONS.clear()
+        got = _ROPE_SECTIONS[sections, pairs] = (_lib._i64 * len(sections))(*sections)
+    return got
+
+
+_RopePair = _lib.RopeTensor * 2
+
+
+def rope(outs, xs, table, sections, positions, grid, bnhd: bool, interleaved: bool, inverse: bool, fresh: bool = False) -> None:
+    """outs <- xs (one or two tensors) turned by the angles of their tokens' positions.  fresh: outs are new dense tensors."""
+    count = len(xs)
+    _check(count in (1, 2) and len(outs) == count, "rope takes one or two tensors, and as many outputs")
     x = xs[0]
     tag = _check_float(x, "x")
     _check(x.dim() == 4, "x must be a 4D tensor")
-    B, D = x.size(0), x.size(3)
-    N = x.size(1 if bnhd else 2)
     _check_tensor(table, torch.float32, "table")
-    _check(table.dim() == 3 and table.size(2) == 2 and table.size(0) >= 1 and table.size(1) >= 1, "table must be [length, pairs, 2]")
-    length, pairs = table.size(0), table.size(1)
-    _check(2 * pairs <= D, "{} pairs do not fit a head of {}", pairs, D)
-    axes = len(sections)
-    _check(1 <= axes <= 8 and sum(sections) == pairs and min(sections) >= 0, "sections must be 1 to 8 counts of pairs, {} in all", pairs)
-    _check((positions is None) != (grid is None), "positions or a grid, one of them")
-    _same_device(x.get_device(), table=table, positions=positions)
-    args = (_lib.RopeTensor * len(xs))()
-    n_dim, h_dim = (1, 2) if bnhd else (2, 1)
+    _check(table.dim() == 3 and table.shape[2] == 2, "table must be [length, pairs, 2]")
+    (B, a, b, D), (length, pairs, _) = x.shape, table.shape
+    N = a if bnhd else b
+    _check(length >= 1 and pairs >= 1, "table must be [length, pairs, 2]")
+    if 2 * pairs > D:
+        _check(False, "{} pairs do not fit a head of {}", pairs, D)
+    section_arg, axes = _rope_sections(sections, pairs), len(sections)
+    _same_device(x, table, positions, *xs[1:], *outs)
+    args = _RopePair()
     empty = B == 0 or N == 0
-    for i, (t, o) in enumerate(zip(xs, outs)):
-        _check(_check_float(t, "x") == tag and _check_float(o, "out") == tag, "all tensors must have one type")
-        _check(t.dim() == 4 and t.size(0) == B and t.size(n_dim) == N and t.size(3) == D, "all tensors must have the same batch, tokens and head dim")
-        _check(o.shape == t.shape, "out must have the shape of x")
-        _same_device(x.get_device(), x=t, out=o)
-        _check(t.stride(3) == 1 and o.stride(3) == 1, "heads must be contiguous")
-        _check(_same_rows(t, o) or not _may_overlap(t, o), "out may be x itself, but not overlap it otherwise")
-        empty = empty or t.size(h_dim) == 0
-        args[i] = _lib.RopeTensor(t.data_ptr(), o.data_ptr(), t.stride(0), t.stride(n_dim), t.stride(h_dim), o.stride(0), o.stride(n_dim),
-                                  o.stride(h_dim), t.size(h_dim))
-    if len(xs) == 2:
+    for i in range(count):
+        t, o = xs[i], outs[i]
+        if t is not x:
+            _check(_check_float(t, "x") == tag, "all tensors must have one type")
+            _check(t.dim() == 4 and t.shape[0] == B and t.shape[1 if bnhd else 2] == N and t.shape[3] == D,
+                   "all tensors must have the same batch, tokens and head dim")
+        t_stride, o_stride = t.stride(), o.stride()
+        if not fresh:
+            _check(_check_float(o, "out") == tag, "all tensors must have one type")
+            _check(o.shape == t.shape, "out must have the shape of x")
+            _check(o_stride[3] == 1, "heads must be contiguous")
+            _check(_same_rows(t, o) or not _may_overlap(t, o), "out may be x itself, but not overlap it otherwise")
+        _check(t_stride[3] == 1, "heads must be contiguous")
+        r = args[i]
+        r.input, r.out = t.data_ptr(), o.data_ptr()
+        if bnhd:
+            r.in_b, r.in_n, r.in_h, _ = t_stride
+            r.out_b, r.out_n, r.out_h, _ = o_stride
+            r.heads = t.shape[2]
+        else:
+            r.in_b, r.in_h, r.in_n, _ = t_stride
+            r.out_b, r.out_h, r.out_n, _ = o_stride
+            r.heads = t.shape[1]
+        empty = empty or r.heads == 0
+    if count == 2 and not fresh:
         _check(not any(_may_overlap(o, t) for o, t in ((outs[0], xs[1]), (outs[1], xs[0]), (outs[0], outs[1])) if o.numel() and t.numel())
                or _interleaved_heads(outs, xs), "the two tensors must not overlap each other")
     pos_ptr, pos_bytes, pos_strides, grid_arg = None, 0, (0, 0, 0), None
     if positions is not None:
-        _check(isinstance(positions, torch.Tensor) and positions.is_cuda and positions.dtype in (torch.int32, torch.int64), "positions must be a CUDA tensor of int32 or int64")
-        _check(list(positions.shape) == [axes, B, N], "positions must be [{}, {}, {}]", axes, B, N)
+        _check(grid is None, "positions or a grid, one of them")
+        _check(positions.is_cuda and positions.dtype in (torch.int32, torch.int64), "positions must be a CUDA tensor of int32 or int64")
+        if positions.shape != (axes, B, N):
+            _check(False, "positions must be [{}, {}, {}]", axes, B, N)
         pos_ptr, pos_bytes, pos_strides = positions.data_ptr(), positions.element_size(), positions.stride()
     else:
-        _check(len(grid) == axes and all(1 <= g for g in grid), "grid must have one size of at least 1 for each axis")
+        _check(grid is not None and len(grid) == axes and min(grid) >= 1, "grid must have one size of at least 1 for each axis")
         _check(max(grid) <= length, "the table has {} positions, the grid {}", length, max(grid))
         grid_arg = (_lib._i64 * axes)(*grid)
     if empty:
         return
-    _lib.check(_L.ac4k_rope(args, len(xs), tag, B, N, D, table.data_ptr(), length, pairs, (_lib._i64 * axes)(*sections), axes, pos_ptr,
-                            pos_bytes, *pos_strides, grid_arg, int(interleaved), int(inverse), _stream()))
+    _lib.check(_L.ac4k_rope(args, count, tag, B, N, D, table.data_ptr(), length, pairs, section_arg, axes, pos_ptr, pos_bytes, *pos_strides,
+                            grid_arg, interleaved, inverse, _stream()))
 
 
 def _interleaved_heads(outs, xs) -> bool:
@@ -680,7 +733,7 @@ def linear_grouped_nvfp4(D, A, A_sf, A_global_scale, B, B_sf, B_global_scale, of
     _check(B.size(2) * 2 == K, "b size(2) must equal a size(1)")
     _check_tensor(B, torch.uint8, "b")
     _check_tensor(B_sf, torch.float8_e4m3fn, "scale_b")
-    _check(list(B_sf.shape) == [E, K // 64, _align_up(N, 16), 4], "scale_b has an invalid shape")
+    _check(B_sf.shape == (E, K // 64, _align_up(N, 16), 4), "scale_b has an invalid shape")
     _check_tensor(B_global_scale, torch.float32, "global_scale_b")
     _check(B_global_scale.dim() == 0 or list(B_global_scale.shape) == [E], "b_global_scale must be a scalar or one per expert")
     _check_tensor(offsets, torch.int32, "offsets")
@@ -695,8 +748,7 @@ def linear_grouped_nvfp4(D, A, A_sf, A_global_scale, B, B_sf, B_global_scale, of
         bias_tag = _check_float(bias, "bias")
         _check(bias.is_contiguous() and list(bias.shape) == [E, N], "bias must be contiguous of [{}, {}]", E, N)
         bias_ptr = bias.data_ptr()
-    _same_device(D.get_device(), a=A, scale_a=A_sf, global_scale_a=A_global_scale, b=B, scale_b=B_sf, global_scale_b=B_global_scale,
-                 offsets=offsets, rows=rows, bias=bias)
+    _same_device(D, A, A_sf, A_global_scale, B, B_sf, B_global_scale, offsets, rows, bias)
     if M == 0 or N == 0 or E == 0:
         return
     _check(T > 0, "rows of an empty a")

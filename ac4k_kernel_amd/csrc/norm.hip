@@ -36,11 +36,41 @@ struct NormArgs {
 
 constexpr float NORM_LEAST = 0x1p-100f;  // a smaller maximum counts as zero
 
-// Sum over the 64 lanes, in every lane: the five steps inside a half by lane exchange, the halves at the end.
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-  for (int m = 1; m < 64; m *= 2) v += __shfl_xor(v, m, 64);
+// Sum over groups of L lanes (16, 32 or 64), in every lane of the group.  (By lane shuffles through LDS, a row's chain of waits was half a microsecond longer.)
+template <int CTRL>
+__device__ __forceinline__ double dpp_f64(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  return __builtin_bit_cast(double, (uint64_t)dpp_u32<CTRL>((uint32_t)(b >> 32)) << 32 | dpp_u32<CTRL>((uint32_t)b));
+}
+template <int L>
+__device__ __forceinline__ double group_sum(double v) {
+  v += dpp_f64<DPP_QUAD_XOR1>(v);
+  v += dpp_f64<DPP_QUAD_XOR2>(v);
+  v += dpp_f64<DPP_ROW_HALF_MIRROR>(v);
+  v += dpp_f64<DPP_ROW_MIRROR>(v);
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  if constexpr (L == 32) {
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_ds_swizzle((int)(b >> 32), 0x401F), lo = (uint32_t)__builtin_amdgcn_ds_swizzle((int)b, 0x401F);  // xor 16
+    v += __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+  }
+  if constexpr (L == 64) {
+    auto row = [&](int lane) {  // the sum of 16 lanes that this lane has
+      return __builtin_bit_cast(double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(b >> 32), lane) << 32 |
+                                            (uint32_t)__builtin_amdgcn_readlane((int)b, lane));
+    };
+    v = (row(0) + row(16)) + (row(32) + row(48));
+  }
   return v;
+}
+
+// 1 / sqrt(x) to 2^-50: the hardware's estimate and a step of Newton's method.  Rounded to fp32 it is the correctly rounded value but for one
+// row in ten million; a division behind a square root took twenty times the instructions.
+__device__ __forceinline__ float norm_factor(double x) {
+  const double e = __builtin_amdgcn_rsq(x);
+  const double half = 0.5 * x * e;
+  const double once = __builtin_fma(e, __builtin_fma(-half, e, 0.5), e);
+  const double r = __builtin_fma(once, __builtin_fma(-0.5 * x * once, once, 0.5), once);
+  return (float)(x > 0.0 && x < __builtin_inf() ? r : e);  // (1 / 0, 1 / inf and NaN)
 }
 
 // A row holds at most one vector that is cut by its end.  It is read and written apart from the others, once a row, so that the code for
@@ -57,27 +87,32 @@ __device__ __forceinline__ void row_vector(Vec8<DT> &v, const void *row, int64_t
   else vec8_zero(v);
 }
 
-// BW waves a workgroup, WPR of them a row, NV vectors of eight elements a lane: K <= 512 * WPR * NV.  A workgroup takes rows_per_block rows,
-// a multiple of BW / WPR.
-template <int DT, int WT, int OUT, int BW, int WPR, int NV>
+// BW waves a workgroup, LPR lanes a row, NV vectors of eight elements a lane: K <= 8 * LPR * NV.  A workgroup takes rows_per_block rows, a
+// multiple of the rows that it has lanes for.
+template <int DT, int WT, int OUT, int BW, int LPR, int NV>
 __global__ __launch_bounds__(64 * BW) void rms_norm_kernel(NormArgs a, int rows_per_block) {
   using T = typename Elem<DT>::T;
-  constexpr int LPR = 64 * WPR, GROUPS = BW / WPR;
+  constexpr int GROUPS = 64 * BW / LPR, WPR = LPR / 64;  // WPR: waves a row, 0 where a wave has several
+  constexpr int IN_WAVE = LPR < 64 ? LPR : 64;
   constexpr bool NVFP4 = OUT == NORM_NVFP4 || OUT == NORM_NVFP4_SECOND || OUT == NORM_NVFP4_ONE;
   constexpr bool SUMS = OUT != NORM_NVFP4_SECOND;  // x is normalized here, not by an earlier launch
   __shared__ double part[WPR > 1 ? BW : 1];
   __shared__ uint32_t part_max[BW];
   __shared__ float lut[NVFP4 ? 128 : 1];
   const int tid = threadIdx.x, sub = tid % LPR, wave = tid >> 6;
-  const int group = __builtin_amdgcn_readfirstlane(tid / LPR);
+  const int group = WPR == 0 ? tid / LPR : __builtin_amdgcn_readfirstlane(tid / LPR);
   float alpha = 0.0f;
-  if constexpr (NVFP4) load_rcp_table(lut);
+  float rcp = 0.0f;  // for the table; it is in LDS behind the next barrier
+  if constexpr (NVFP4) rcp = g_rcp_e4m3.v[tid & 127];
   if constexpr (OUT == NORM_NVFP4) {
+    if (tid < 128) lut[tid] = rcp;
+    __syncthreads();
     const float g = *a.gs;
     alpha = __builtin_fabsf(g) < NORM_LEAST / 4096.0f ? 0.0f : 1.0f / g;
   }
   auto block_max = [&](uint32_t m) {  // of every wave's m (uniform in a wave)
     if ((tid & 63) == 0) part_max[wave] = m;
+    if (NVFP4 && tid < 128) lut[tid] = rcp;
     __syncthreads();
     uint32_t b = part_max[0];
 #pragma unroll
@@ -91,22 +126,24 @@ __global__ __launch_bounds__(64 * BW) void rms_norm_kernel(NormArgs a, int rows_
     alpha = g == 0.0f ? 0.0f : 1.0f / g;
     if (blockIdx.x == 0 && tid == 0) *a.gs = g;
   };
-  if constexpr (OUT == NORM_NVFP4_SECOND) {
-    uint32_t m = 0;
-    for (int i = tid; i < a.maxima_count; i += 64 * BW) m = umax32(m, __float_as_uint(a.maxima[i]));
-    global_scale(block_max(group_umax<64>(m)));
-  }
   const int cut = (int)(a.K & 7);
   const int64_t k_cut = a.K - cut;
   const bool cut_mine = cut != 0 && (int)(k_cut / 8 % LPR) == sub;
-  Vec8<WT> weight_cut;
-  cut_load(weight_cut, a.weight, k_cut, cut_mine && a.weight, cut);
+  // the weights, once for all rows of the workgroup, and under way before the first row's sum is known
+  Vec8<WT> w[NV];
+  const bool weighted = a.weight != nullptr;
+  if (weighted) {
+    Vec8<WT> w_cut;
+    cut_load(w_cut, a.weight, k_cut, cut_mine, cut);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) row_vector(w[j], a.weight, (j * LPR + sub) * 8, a.K, w_cut);
+  }
   uint32_t block_m = 0;
   const int64_t row0 = (int64_t)blockIdx.x * rows_per_block;
   for (int it = 0; it * GROUPS < rows_per_block; ++it) {
     const int64_t row = row0 + it * GROUPS + group;
     const bool valid = row < a.rows;
-    if (WPR == 1 && OUT != NORM_NVFP4_ONE && !valid && !(NVFP4 && row < a.Rp)) break;  // (rows of several waves meet at barriers)
+    if (WPR <= 1 && OUT != NORM_NVFP4_ONE && !(OUT == NORM_NVFP4_SECOND && it == 0) && !valid && !(NVFP4 && row < a.Rp)) break;  // (rows of several waves meet at barriers)
     Vec8<DT> h[NV];
     float r = 0.0f;
     {
@@ -144,7 +181,7 @@ __global__ __launch_bounds__(64 * BW) void rms_norm_kernel(NormArgs a, int rows_
           const double v = vec8_get(h[j], i);
           s = __builtin_fma(v, v, s);
         }
-      s = wave_sum(s);
+      s = group_sum<IN_WAVE>(s);
       if constexpr (WPR > 1) {
         if (it) __syncthreads();  // the parts of the row before have been read
         if ((tid & 63) == 0) part[wave] = s;
@@ -153,20 +190,23 @@ __global__ __launch_bounds__(64 * BW) void rms_norm_kernel(NormArgs a, int rows_
 #pragma unroll
         for (int i = 0; i < WPR; ++i) s += part[group * WPR + i];
       }
-      r = (float)(1.0 / __builtin_sqrt(s / (double)a.K + a.eps));
+      r = norm_factor(s / (double)a.K + a.eps);
     } else {
       r = valid ? a.factors[row] : 0.0f;
+      if (it == 0) {  // (the loads of the first row are under way)
+        uint32_t m = 0;
+        for (int i = tid; i < a.maxima_count; i += 64 * BW) m = umax32(m, __float_as_uint(a.maxima[i]));
+        global_scale(block_max(group_umax<64>(m)));
+      }
     }
     // y of vector j
     auto values = [&](int j, float (&y)[8]) {
       const int k = (j * LPR + sub) * 8;
 #pragma unroll
       for (int i = 0; i < 8; ++i) y[i] = vec8_get(h[j], i) * r;
-      if (a.weight) {
-        Vec8<WT> w;
-        row_vector(w, a.weight, k, a.K, weight_cut);
+      if (weighted) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = y[i] * vec8_get(w, i);
+        for (int i = 0; i < 8; ++i) y[i] = y[i] * vec8_get(w[j], i);
       }
       // behind the row the product 0 * r * 0 is not 0 where r is not finite
       if (k + 8 > a.K) {
@@ -213,7 +253,7 @@ __global__ __launch_bounds__(64 * BW) void rms_norm_kernel(NormArgs a, int rows_
         }
         continue;
       }
-      m = group_umax<64>(valid ? m : 0);
+      m = group_umax<OUT == NORM_NVFP4_ONE ? 64 : IN_WAVE>(valid ? m : 0);
       if constexpr (OUT == NORM_NVFP4_ONE) {  // one workgroup, one pass of its loop
         global_scale(block_max(m));
       } else {
@@ -295,83 +335,103 @@ __global__ __launch_bounds__(64 * BW) void rms_norm_kernel(NormArgs a, int rows_
   }
 }
 
-// Shape of a launch.  Rows of up to 512 * 16 elements (fp32: half) belong to a wave where there are rows enough to fill the GPU, others to four
-// waves or sixteen.
+// Shape of a launch: so many waves a row that a lane holds two or three vectors of it (weights and residual beside them stay under 80 registers,
+// and six to eight waves on a SIMD hide each other's loads and reductions), more only behind sixteen waves.
 struct NormPlan {
-  int bw, wpr, nv, rows_per_block;
+  int bw, lpr, nv, rows_per_block;
 };
-static NormPlan norm_plan(int64_t rows, int64_t K, int dtype, bool nvfp4) {
+static NormPlan norm_plan(int64_t rows, int64_t K, bool nvfp4) {
   const int64_t vecs = ceil_div(K, 512);  // of a wave
-  const int most = dtype == AC4K_DTYPE_FP32 ? 8 : 16;
-  const int wpr = vecs <= 1 || (rows >= 2048 && vecs <= most) ? 1 : vecs <= 32 && (rows >= 512 || vecs <= 4) ? 4 : 16;
-  const int64_t need = ceil_div(vecs, wpr);
-  const int nv = need <= 1 ? 1 : need <= 4 ? 4 : need <= 8 ? 8 : 16;
-  NormPlan p{wpr == 16 ? 16 : 4, wpr, nv, 1};
-  p.rows_per_block = p.bw / p.wpr;
-  // nvfp4: the scales of 16 neighbouring rows are one 64-byte run
-  if (nvfp4 && rows >= 4096) p.rows_per_block = 16;
+  NormPlan p;
+  p.lpr = K <= 128 ? 16 : K <= 256 ? 32 : 64 * (vecs <= 2 ? 1 : vecs <= 4 ? 2 : vecs <= 12 ? 4 : vecs <= 16 ? 8 : 16);
+  const int64_t need = ceil_div(K, 8 * p.lpr);
+  p.nv = need <= 1 && p.lpr <= 64 ? 1 : need <= 2 ? 2 : need <= 3 && p.lpr == 256 ? 3 : need <= 4 ? 4 : 8;
+  p.bw = p.lpr < 256 ? 4 : p.lpr / 64;
+  // A workgroup takes some rows one after the other where there are workgroups enough: they share the weights, and nvfp4 scales of
+  // neighbouring rows leave for one line.  Second launch of nvfp4, 8192 x 4096, rows a workgroup / us: 1 48, 4 27, 8 23, 16 28;
+  // 75600 x 5120 to bf16: 1 279, 2 264, 4 281, 16 310.
+  const int groups = 64 * p.bw / p.lpr;
+  const int64_t sets = ceil_div(rows, groups);
+  int64_t turns = nvfp4 ? (sets >= 8192 ? 8 : sets >= 2048 ? 4 : sets >= 1024 ? 2 : 1) : sets >= 2048 ? 2 : 1;
+  if (turns < sets >> 20) turns = (sets >> 20) + 1;  // 2^32 threads a launch
+  p.rows_per_block = (int)(turns * groups);
   return p;
 }
+
+// vectors of a lane in the kernel that takes a tensor in one workgroup (128 registers)
+constexpr int norm_one_vectors(int dtype) { return dtype == AC4K_DTYPE_FP32 ? 2 : 4; }
 
 template <int DT, int WT, int OUT>
 static int launch_norm(const NormArgs &a, const NormPlan &p, hipStream_t st) {
   const int64_t rows = OUT == NORM_NVFP4 || OUT == NORM_NVFP4_SECOND ? a.Rp : a.rows;
   const int64_t blocks = ceil_div(rows, p.rows_per_block);
   auto go = [&](auto kernel, int bw) { hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(64 * bw), 0, st, a, p.rows_per_block); };
-#define AC4K_NORM(BW, WPR, NV) \
-  if (p.bw == BW && p.wpr == WPR && p.nv == NV) return go(rms_norm_kernel<DT, WT, OUT, BW, WPR, NV>, BW), 0
-  constexpr bool WIDE = DT == AC4K_DTYPE_FP32;
+#define AC4K_NORM(BW, LPR, NV) \
+  if (p.bw == BW && p.lpr == LPR && p.nv == NV) return go(rms_norm_kernel<DT, WT, OUT, BW, LPR, NV>, BW), 0
+  constexpr int NV1 = norm_one_vectors(DT);
   if constexpr (OUT == NORM_NVFP4_ONE) {
-    AC4K_NORM(16, 1, 4);
-    AC4K_NORM(16, 2, 4);
-    AC4K_NORM(16, 4, 4);
-    AC4K_NORM(16, 8, 4);
-    AC4K_NORM(16, 16, 4);
+    AC4K_NORM(8, 512, 2);
+    AC4K_NORM(16, 64, NV1);
+    AC4K_NORM(16, 128, NV1);
+    AC4K_NORM(16, 256, NV1);
+    AC4K_NORM(16, 512, NV1);
+    AC4K_NORM(16, 1024, NV1);
   } else {
-    AC4K_NORM(4, 1, 1);
-    AC4K_NORM(4, 1, 4);
-    AC4K_NORM(4, 1, 8);
-    if constexpr (!WIDE) AC4K_NORM(4, 1, 16);
-    AC4K_NORM(4, 4, 1);
-    AC4K_NORM(4, 4, 4);
-    AC4K_NORM(4, 4, 8);
-    AC4K_NORM(16, 16, 1);
-    AC4K_NORM(16, 16, 4);
-    AC4K_NORM(16, 16, 8);
+    AC4K_NORM(4, 16, 1);
+    AC4K_NORM(4, 32, 1);
+    AC4K_NORM(4, 64, 1);
+    AC4K_NORM(4, 64, 2);
+    AC4K_NORM(4, 128, 2);
+    AC4K_NORM(4, 256, 2);
+    AC4K_NORM(4, 256, 3);
+    AC4K_NORM(8, 512, 2);
+    AC4K_NORM(16, 1024, 2);
+    AC4K_NORM(16, 1024, 4);
+    AC4K_NORM(16, 1024, 8);
   }
 #undef AC4K_NORM
-  return set_error("rms_norm: no kernel for %d waves a row and %d vectors a lane", p.wpr, p.nv);
+  return set_error("rms_norm: no kernel for %d lanes a row and %d vectors a lane", p.lpr, p.nv);
 }
 
-// Tensors of up to 32768 elements in 16 rows at the most: one workgroup holds all of them and finds the global scale by itself.
-static bool norm_one(int64_t rows, int64_t K, NormPlan &p) {
+// Tensors of up to 32768 elements (fp32: half) in 16 rows at the most: one workgroup holds all of them and finds the global scale by itself.
+static bool norm_one(int64_t rows, int64_t K, int dtype, NormPlan &p) {
+  if (rows == 1 && K <= 8192) {
+    p = {8, 512, 2, 1};
+    return true;
+  }
   int wpr = 16;
   while (wpr > 1 && 16 / wpr < rows) wpr /= 2;
-  if (16 / wpr < rows || ceil_div(K, 512 * wpr) > 4) return false;
-  p = {16, wpr, 4, 16 / wpr};
+  if (16 / wpr < rows || ceil_div(K, 512 * wpr) > norm_one_vectors(dtype)) return false;
+  p = {16, 64 * wpr, norm_one_vectors(dtype), 16 / wpr};
   return true;
+}
+// Its first launch: few enough workgroups that each of the second can read the maxima of all
+static NormPlan norm_stats_plan(int64_t rows, int64_t K) {
+  NormPlan p = norm_plan(rows, K, false);
+  const int64_t least = ceil_div(rows, 2048);
+  if (p.rows_per_block < least) p.rows_per_block = (int)align_up(least, 64 * p.bw / p.lpr);
+  return p;
 }
 static int64_t norm_workspace(int64_t rows, int64_t K, int dtype) {
   NormPlan p;
-  if (norm_one(rows, K, p)) return 0;
-  p = norm_plan(rows, K, dtype, true);
-  return 4 * (align_up(rows, 64) + ceil_div(rows, p.rows_per_block));
+  if (norm_one(rows, K, dtype, p)) return 0;
+  return 4 * (align_up(rows, 64) + ceil_div(rows, norm_stats_plan(rows, K).rows_per_block));
 }
 
 template <int DT, int WT>
 static int norm_dtype(NormArgs a, int precision, bool find_scale, float *workspace, int dtype, hipStream_t st) {
   if (precision == AC4K_PRECISION_NVFP4 && find_scale) {
     NormPlan p;
-    if (norm_one(a.rows, a.K, p)) return launch_norm<DT, WT, NORM_NVFP4_ONE>(a, p, st);
-    p = norm_plan(a.rows, a.K, dtype, true);
+    if (norm_one(a.rows, a.K, dtype, p)) return launch_norm<DT, WT, NORM_NVFP4_ONE>(a, p, st);
+    p = norm_stats_plan(a.rows, a.K);
     a.factors = workspace;
     a.maxima = workspace + align_up(a.rows, 64);
     a.maxima_count = (int)ceil_div(a.rows, p.rows_per_block);
     if (int rc = launch_norm<DT, WT, NORM_STATS>(a, p, st)) return rc;
     if (a.residual) a.x = a.sum, a.x_stride = a.sum_stride;
-    return launch_norm<DT, WT, NORM_NVFP4_SECOND>(a, p, st);
+    return launch_norm<DT, WT, NORM_NVFP4_SECOND>(a, norm_plan(a.rows, a.K, true), st);
   }
-  const NormPlan p = norm_plan(a.rows, a.K, dtype, precision == AC4K_PRECISION_NVFP4);
+  const NormPlan p = norm_plan(a.rows, a.K, precision == AC4K_PRECISION_NVFP4);
   switch (precision) {
     case AC4K_PRECISION_NONE: return launch_norm<DT, WT, NORM_PLAIN>(a, p, st);
     case AC4K_PRECISION_FP8: return launch_norm<DT, WT, NORM_FP8>(a, p, st);
@@ -392,57 +452,86 @@ struct DequantArgs {
   int64_t gs_stride;             // 0: one scale for all leading planes
 };
 
-// A lane takes eight elements; a wave 512 columns of four rows, a workgroup 16 rows, whose nvfp4 scales are whole 64-byte runs.
+// A wave takes 512 columns of four rows, a workgroup 16 rows, whose nvfp4 scales are whole 64-byte runs.  A lane takes eight elements of a row,
+// as one vector of 16 bytes of the output or two, so that a wave's stores are whole runs of a kilobyte.
+// 8192 x 4096 nvfp4 to bf16 14.6 us, 5.9 TB/s.
 template <int DT, int PRECISION>
 __global__ __launch_bounds__(256) void dequantize_kernel(DequantArgs a) {
+  using T = typename Elem<DT>::T;
+  constexpr int V = 16 / sizeof(T), PIECES = 8 / V;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t spans = ceil_div(a.W, 512), bands = ceil_div(a.R, 16);
-  const int64_t span = blockIdx.x % spans, rest = blockIdx.x / spans;
-  const int64_t lead = rest / bands, band = rest % bands;
-  const int64_t k = span * 512 + lane * 8;
-  if (k >= a.cols) return;
+  const uint32_t spans = (uint32_t)ceil_div(a.W, 512), bands = (uint32_t)ceil_div(a.R, 16);
+  const uint32_t rest = blockIdx.x / spans, span = blockIdx.x - rest * spans;
+  const uint32_t lead = rest / bands, band = rest - lead * bands;
+  const int64_t k0 = span * 512ll + lane * V;
+  if (k0 >= a.cols) return;
   const float gs = PRECISION == AC4K_PRECISION_NVFP4 ? a.gs[lead * a.gs_stride] : 1.0f;
-  uint2 v[4];
-  float s[4];
+  uint32_t v[4][2];  // eight elements: nibbles in the first word (two pieces: half of it each), bytes in both
+  float s[4][PIECES];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int64_t row = band * 16 + wave * 4 + i;
+    const int64_t row = band * 16ll + wave * 4 + i;
     if (row >= a.R) break;
-    if constexpr (PRECISION == AC4K_PRECISION_NVFP4) {
-      v[i].x = *reinterpret_cast<const uint32_t *>(a.q + (lead * a.R + row) * (a.W / 2) + k / 2);
-      s[i] = e4m3_to_f32(static_cast<const uint8_t *>(a.sf)[((lead * (a.W / 64) + k / 64) * a.Rp + row) * 4 + k % 64 / 16]);
-    } else {
-      const u32x2 w = *reinterpret_cast<const u32x2_elem *>(a.q + (lead * a.R + row) * a.W + k);
-      v[i] = make_uint2(w.x, w.y);
-      s[i] = static_cast<const float *>(a.sf)[lead * a.Rp + row];
+#pragma unroll
+    for (int p = 0; p < PIECES; ++p) {
+      const int64_t k = k0 + p * 64 * V;
+      if (k >= a.cols) break;
+      if constexpr (PRECISION == AC4K_PRECISION_NVFP4) {
+        const uint8_t *q = a.q + (lead * a.R + row) * (a.W / 2) + k / 2;
+        v[i][p] = V == 8 ? *reinterpret_cast<const uint32_t *>(q) : *reinterpret_cast<const uint16_t *>(q);
+        s[i][p] = e4m3_to_f32(static_cast<const uint8_t *>(a.sf)[((lead * (a.W / 64) + k / 64) * a.Rp + row) * 4 + k % 64 / 16]);
+      } else {
+        const uint8_t *q = a.q + (lead * a.R + row) * a.W + k;
+        if constexpr (V == 8) {
+          const u32x2 w = *reinterpret_cast<const u32x2_elem *>(q);
+          v[i][0] = w.x, v[i][1] = w.y;
+        } else {
+          typedef uint32_t u32_byte __attribute__((aligned(1)));
+          v[i][p] = *reinterpret_cast<const u32_byte *>(q);
+        }
+        s[i][p] = static_cast<const float *>(a.sf)[lead * a.Rp + row];
+      }
     }
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int64_t row = band * 16 + wave * 4 + i;
+    const int64_t row = band * 16ll + wave * 4 + i;
     if (row >= a.R) break;
-    float f[8];
-    if constexpr (PRECISION == AC4K_PRECISION_NVFP4) {
-      // e2m1 times the scale of 16 is exact; the product with the global scale is the one rounding in 32 bits
 #pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        const f32x2 d = p == 0   ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(v[i].x, 1.0f, 0)
-                        : p == 1 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(v[i].x, 1.0f, 1)
-                        : p == 2 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(v[i].x, 1.0f, 2)
-                                 : __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(v[i].x, 1.0f, 3);
-        f[2 * p] = d.x * s[i] * gs;
-        f[2 * p + 1] = d.y * s[i] * gs;
+    for (int p = 0; p < PIECES; ++p) {
+      const int64_t k = k0 + p * 64 * V;
+      if (k >= a.cols) break;
+      float f[V];
+#pragma unroll
+      for (int e = 0; e < V; e += 2) {
+        if constexpr (PRECISION == AC4K_PRECISION_NVFP4) {
+          // e2m1 times the scale of 16 is exact; the product with the global scale is the one rounding in 32 bits
+          const f32x2 d = e == 0   ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(v[i][p], 1.0f, 0)
+                          : e == 2 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(v[i][p], 1.0f, 1)
+                          : e == 4 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(v[i][p], 1.0f, 2)
+                                   : __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(v[i][p], 1.0f, 3);
+          f[e] = d.x * s[i][p] * gs;
+          f[e + 1] = d.y * s[i][p] * gs;
+        } else {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t b = v[i][V == 8 ? e / 4 : p] >> (8 * ((e + h) & 3)) & 0xffu;
+            f[e + h] = (PRECISION == AC4K_PRECISION_INT8 ? (float)(int8_t)b : e4m3_to_f32(b)) * s[i][p];
+          }
+        }
       }
-    } else {
+      T *out = static_cast<T *>(a.out) + (lead * a.R + row) * a.cols + k;
+      if (k + V <= a.cols) {
+        u32x4 w;
+        if constexpr (V == 8) w = (u32x4){Elem<DT>::cvt2(f[0], f[1]), Elem<DT>::cvt2(f[2], f[3]), Elem<DT>::cvt2(f[4], f[5]), Elem<DT>::cvt2(f[6], f[7])};
+        else w = (u32x4){__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])};
+        *reinterpret_cast<u32x4_elem *>(out) = w;
+      } else {
 #pragma unroll
-      for (int p = 0; p < 8; ++p) {
-        const uint32_t b = (p < 4 ? v[i].x : v[i].y) >> (8 * (p & 3)) & 0xffu;
-        f[p] = (PRECISION == AC4K_PRECISION_INT8 ? (float)(int8_t)b : e4m3_to_f32(b)) * s[i];
+        for (int e = 0; e < V; ++e)
+          if (k + e < a.cols) out[e] = Elem<DT>::cvt(f[e]);
       }
     }
-    Vec8<DT> o;
-    vec8_set(o, f);
-    vec8_store(static_cast<char *>(a.out) + (lead * a.R + row) * a.cols * (int64_t)sizeof(typename Elem<DT>::T), o, k, a.cols);
   }
 }
 

@@ -6,8 +6,8 @@
 // last pair are copied.  The table holds cosines and sines in fp32, made from angles in 64 bits: a product of a far position and a
 // frequency in 32 bits would be off by more than the rounding of the result.
 //
-// Bound by memory: every element is read and written once.  A thread keeps its place inside the head and goes over the heads of its token,
-// so that it reads the four to eight entries of the table once per token.
+// Bound by memory: every element is read and written once.  A thread keeps its token and its place inside the head and goes over the heads, so
+// that it reads its four to eight entries of the table once.
 #include "elements.h"
 
 namespace ac4k {
@@ -24,105 +24,187 @@ struct RopeArgs {
   const float2 *table;  // [length][pairs]
   const void *positions;
   int64_t pos_axis, pos_b, pos_n;  // strides; positions null: the token's place in a grid
-  int64_t grid[AC4K_ROPE_MAX_AXES];
-  int64_t B, N, length;
+  uint32_t grid[AC4K_ROPE_MAX_AXES];
+  uint32_t N;
+  int64_t length;
   int D, pairs, axes, pos_bytes;
   int end[AC4K_ROPE_MAX_AXES];  // first pair behind each axis
+  uint32_t rot_vecs, vecs;      // vectors of a head: those that hold pairs, and with those that are copied
+  uint32_t vecs_inverse;        // ceil(2^16 / vecs)
+  uint32_t blocks_b;            // workgroups of a batch
+  uint32_t once_log, across;    // 2^once_log tokens a workgroup, `across` heads of each at a time
+  bool heads_first;             // neighbouring threads are on neighbouring heads of a token, otherwise on neighbouring tokens of a head
+  float sign;                   // of the sines
 };
 
-// Position of token n of batch b along an axis; negative: the token stays as it is.
-__device__ __forceinline__ int64_t rope_position(const RopeArgs &a, int64_t b, int64_t n, int axis) {
-  if (a.positions) {
-    const int64_t i = axis * a.pos_axis + b * a.pos_b + n * a.pos_n;
-    return a.pos_bytes == 8 ? static_cast<const int64_t *>(a.positions)[i] : static_cast<const int32_t *>(a.positions)[i];
-  }
-  int64_t at = n;
-  for (int x = a.axes - 1; x > axis; --x) at /= a.grid[x];
-  return axis == 0 ? (at < a.grid[0] ? at : -1) : at % a.grid[axis];
-}
-
-template <int DT, bool INTERLEAVED, bool INVERSE>
+// WHOLE: no vector is cut by the end of the pairs or of the head; four of them are under way at a time then, with no branch between their loads
+// (with the loads of cut vectors in between, every load was waited for by itself).
+template <int DT, bool INTERLEAVED, bool WHOLE>
 __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
   using T = typename Elem<DT>::T;
-  // vectors of a head: those that hold pairs (INTERLEAVED: 4 pairs each; otherwise 8 first elements, their partners `pairs` further on),
-  // then those that are copied
-  const int rot = 2 * a.pairs;
-  const int rot_vecs = INTERLEAVED ? (rot + 7) / 8 : (a.pairs + 7) / 8;
-  const int vecs = rot_vecs + (a.D - rot + 7) / 8;
-  const int across = 256 / vecs;  // heads at a time
-  const int v = threadIdx.x % vecs, head0 = threadIdx.x / vecs;
-  const int64_t n = blockIdx.x % a.N, b = blockIdx.x / a.N;
-  if (head0 >= across) return;
+  constexpr int AHEAD = WHOLE ? 4 : 1;
+  // INTERLEAVED: a vector holds four pairs; otherwise the first elements of eight, their partners `pairs` further on
   constexpr int NP = INTERLEAVED ? 4 : 8;
+  const int rot = 2 * a.pairs;
+  const uint32_t u = threadIdx.x * a.vecs_inverse >> 16, v = threadIdx.x - u * a.vecs;  // (exact: both under 2^8)
+  uint32_t my, head0;
+  if (a.heads_first) {
+    my = 0, head0 = u;
+    if (a.once_log) my = u / a.across, head0 = u - my * a.across;
+  } else {
+    my = u & ((1u << a.once_log) - 1), head0 = u >> a.once_log;
+  }
+  const uint32_t b = blockIdx.x / a.blocks_b, n = ((blockIdx.x - b * a.blocks_b) << a.once_log) + my;
+  if (my >> a.once_log || head0 >= a.across || n >= a.N) return;
+
+  // first element of what the thread moves of a head, and the end of its kind
+  const bool turned = v < a.rot_vecs;
+  const int k0 = turned ? v * 8 : rot + (v - a.rot_vecs) * 8;
+  const int k1 = !turned ? a.D : INTERLEAVED ? rot : a.pairs;
+  const uint32_t first = a.t[0].heads, heads = first + a.t[1].heads;
+  const T *in[2];
+  T *out[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    in[i] = static_cast<const T *>(a.t[i].in) + b * a.t[i].in_b + n * a.t[i].in_n;
+    out[i] = static_cast<T *>(a.t[i].out) + b * a.t[i].out_b + n * a.t[i].out_n;
+  }
+  Vec8<DT> x[AHEAD], y[AHEAD];  // y: the partners, where they are apart
+  auto move_in = [&](Vec8<DT> &to, const T *p) {
+    if constexpr (WHOLE) vec8_load_all(to, p + k0);
+    else vec8_load(to, p, k0, k1);
+  };
+  auto move_out = [&](T *p, const Vec8<DT> &from) {
+    if constexpr (WHOLE) vec8_store_all(p + k0, from);
+    else vec8_store(p, from, k0, k1);
+  };
+  auto load = [&](uint32_t h0) {  // heads past the last one: the last one again
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const uint32_t h = h0 + i * a.across < heads ? h0 + i * a.across : heads - 1;
+      const T *p = h < first ? in[0] + h * a.t[0].in_h : in[1] + (h - first) * a.t[1].in_h;
+      move_in(x[i], p);
+      if constexpr (!INTERLEAVED) move_in(y[i], p + (turned ? a.pairs : 0));
+    }
+  };
+  load(head0);  // under way while positions and angles are looked up
+
   float c[NP], s[NP];
   bool stay = false;
-  for (int x = 0; x < a.axes; ++x) stay |= rope_position(a, b, n, x) < 0;
   const int pair0 = v * NP;
-  if (v < rot_vecs) {
-    int axis = 0;
-    while (axis + 1 < a.axes && pair0 >= a.end[axis]) ++axis;
-    int64_t at = rope_position(a, b, n, axis);
+  int64_t at[NP];
+  int axis_end = 0;  // of the first pair
+  {
+    int64_t pos[AC4K_ROPE_MAX_AXES];
+    if (a.positions) {
+      const int64_t i = b * a.pos_b + n * a.pos_n;
 #pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const int pair = pair0 + i;
-      while (axis + 1 < a.axes && pair >= a.end[axis]) at = rope_position(a, b, n, ++axis);
-      c[i] = 1.0f, s[i] = 0.0f;
-      if (pair < a.pairs && !stay) {
-        // a position that the table does not have has no angle: NaN, and nothing behind the table is read
-        float2 cs = make_float2(__builtin_nanf(""), __builtin_nanf(""));
-        if (at < a.length) cs = a.table[at * a.pairs + pair];
-        c[i] = cs.x, s[i] = INVERSE ? -cs.y : cs.y;
-      }
-    }
-  }
-  const int heads = a.t[0].heads + a.t[1].heads;
-  for (int h = head0; h < heads; h += across) {
-    const bool second = h >= a.t[0].heads;
-    const RopeTensor &t = second ? a.t[1] : a.t[0];
-    const int hh = second ? h - a.t[0].heads : h;
-    const T *in = static_cast<const T *>(t.in) + b * t.in_b + n * t.in_n + hh * t.in_h;
-    T *out = static_cast<T *>(t.out) + b * t.out_b + n * t.out_n + hh * t.out_h;
-    if (v >= rot_vecs) {  // copied
-      Vec8<DT> x;
-      const int k = rot + (v - rot_vecs) * 8;
-      vec8_load(x, in, k, a.D);
-      vec8_store(out, x, k, a.D);
-    } else if constexpr (INTERLEAVED) {
-      Vec8<DT> x;
-      vec8_load(x, in, v * 8, rot);
-      float f[8];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float p = vec8_get(x, 2 * i), q = vec8_get(x, 2 * i + 1);
-        f[2 * i] = stay ? p : p * c[i] - q * s[i];
-        f[2 * i + 1] = stay ? q : q * c[i] + p * s[i];
-      }
-      vec8_set(x, f);
-      vec8_store(out, x, v * 8, rot);
+      for (int axis = 0; axis < AC4K_ROPE_MAX_AXES; ++axis)
+        if (axis < a.axes)
+          pos[axis] = a.pos_bytes == 8 ? static_cast<const int64_t *>(a.positions)[i + axis * a.pos_axis] : static_cast<const int32_t *>(a.positions)[i + axis * a.pos_axis];
     } else {
-      Vec8<DT> x, y;
-      vec8_load(x, in, v * 8, a.pairs);
-      vec8_load(y, in + a.pairs, v * 8, a.pairs);
-      float f[8], g[8];
+      uint32_t place = n;  // by the last axis first
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float p = vec8_get(x, i), q = vec8_get(y, i);
-        f[i] = stay ? p : p * c[i] - q * s[i];
-        g[i] = stay ? q : q * c[i] + p * s[i];
-      }
-      vec8_set(x, f);
-      vec8_set(y, g);
-      vec8_store(out, x, v * 8, a.pairs);
-      vec8_store(out + a.pairs, y, v * 8, a.pairs);
+      for (int axis = AC4K_ROPE_MAX_AXES - 1; axis >= 0; --axis)
+        if (axis < a.axes) {
+          const uint32_t q = place / a.grid[axis];
+          pos[axis] = place - q * a.grid[axis];
+          place = q;
+        }
+      stay = place > 0;  // behind the last place
     }
+#pragma unroll
+    for (int i = 0; i < NP; ++i) at[i] = 0;
+#pragma unroll
+    for (int axis = AC4K_ROPE_MAX_AXES - 1; axis >= 0; --axis)
+      if (axis < a.axes) {
+        stay |= pos[axis] < 0;
+#pragma unroll
+        for (int i = 0; i < NP; ++i)
+          if (pair0 + i < a.end[axis]) at[i] = pos[axis];  // (axes in front overwrite)
+        if (pair0 < a.end[axis]) axis_end = a.end[axis];
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < NP; ++i) c[i] = 1.0f, s[i] = 0.0f;
+  if (turned && !stay) {
+    // a position that the table does not have has no angle: NaN, and nothing behind the table is read
+    if (pair0 + NP <= axis_end && at[0] < a.length) {  // one row of the table
+      const char *row = reinterpret_cast<const char *>(a.table + at[0] * a.pairs + pair0);
+#pragma unroll
+      for (int i = 0; i < NP; i += 2) {
+        const f32x4 cs = *reinterpret_cast<const f32x4_elem *>(row + i * 8);
+        c[i] = cs.x, s[i] = cs.y, c[i + 1] = cs.z, s[i + 1] = cs.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NP; ++i)
+        if (pair0 + i < a.pairs) {
+          float2 cs = make_float2(__builtin_nanf(""), __builtin_nanf(""));
+          if (at[i] < a.length) cs = a.table[at[i] * a.pairs + pair0 + i];
+          c[i] = cs.x, s[i] = cs.y;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NP; ++i) s[i] *= a.sign;
+  }
+  for (uint32_t h0 = head0; h0 < heads;) {
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const uint32_t h = h0 + i * a.across;
+      if (turned && !stay) {
+        float f[8], g[8];
+        if constexpr (INTERLEAVED) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float p = vec8_get(x[i], 2 * j), q = vec8_get(x[i], 2 * j + 1);
+            f[2 * j] = __builtin_fmaf(p, c[j], -(q * s[j]));
+            f[2 * j + 1] = __builtin_fmaf(q, c[j], p * s[j]);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float p = vec8_get(x[i], j), q = vec8_get(y[i], j);
+            f[j] = __builtin_fmaf(p, c[j], -(q * s[j]));
+            g[j] = __builtin_fmaf(q, c[j], p * s[j]);
+          }
+          vec8_set(y[i], g);
+        }
+        vec8_set(x[i], f);
+      }
+      if (h < heads) {
+        T *p = h < first ? out[0] + h * a.t[0].out_h : out[1] + (h - first) * a.t[1].out_h;
+        move_out(p, x[i]);
+        if constexpr (!INTERLEAVED)
+          if (turned) move_out(p + a.pairs, y[i]);
+      }
+    }
+    h0 += AHEAD * a.across;
+    if (h0 < heads) load(h0);
   }
 }
 
 template <int DT>
-static void launch_rope(const RopeArgs &a, bool interleaved, bool inverse, hipStream_t st) {
-  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)(a.B * a.N)), dim3(256), 0, st, a); };
-  if (interleaved) inverse ? go(rope_kernel<DT, true, true>) : go(rope_kernel<DT, true, false>);
-  else inverse ? go(rope_kernel<DT, false, true>) : go(rope_kernel<DT, false, false>);
+static void launch_rope(RopeArgs a, int64_t B, bool interleaved, hipStream_t st) {
+  a.rot_vecs = interleaved ? (2 * a.pairs + 7) / 8 : (a.pairs + 7) / 8;
+  a.vecs = a.rot_vecs + (a.D - 2 * a.pairs + 7) / 8;
+  a.vecs_inverse = (65536 + a.vecs - 1) / a.vecs;
+  const uint32_t across = 256 / a.vecs, heads = a.t[0].heads + a.t[1].heads;
+  // Threads side by side are on the neighbours in memory: heads of a token, or tokens of a head.  A workgroup takes tokens enough that a
+  // thread has four heads to go over (and eight tokens where they are the neighbours), as long as a thousand workgroups remain.  us, one
+  // token at a time / two / four / eight: 8002 x 24 heads of 64, fp32 31 / 27 / 23 / 21; 8192 x 48 of 128, halves 39 / 36 / 34 / 34;
+  // 75600 x 80 of 128 552 / 573 / 589 / 596.
+  a.heads_first = a.t[0].in_h <= a.t[0].in_n;
+  while ((2u << a.once_log) <= across && (1u << a.once_log) < a.N && ((heads << a.once_log) < 4 * across || (!a.heads_first && a.once_log < 3)) &&
+         B * a.N >> (a.once_log + 1) >= 1000)
+    ++a.once_log;
+  a.across = across >> a.once_log;
+  a.blocks_b = (a.N + (1u << a.once_log) - 1) >> a.once_log;
+  const dim3 grid((unsigned)(B * a.blocks_b));
+  const bool whole = (interleaved ? 2 * a.pairs : a.pairs) % 8 == 0 && (a.D - 2 * a.pairs) % 8 == 0;
+  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, a); };
+  if (interleaved) whole ? go(rope_kernel<DT, true, true>) : go(rope_kernel<DT, true, false>);
+  else whole ? go(rope_kernel<DT, false, true>) : go(rope_kernel<DT, false, false>);
 }
 
 }  // namespace ac4k
@@ -152,7 +234,8 @@ extern "C" __attribute__((visibility("default"))) int ac4k_rope(
     if (grid) {
       AC4K_REQUIRE(grid[x] >= 1, "a grid has at least one place along every axis");
       AC4K_REQUIRE(grid[x] <= length, "the table has %lld positions, the grid %lld", (long long)length, (long long)grid[x]);
-      a.grid[x] = grid[x];
+      AC4K_REQUIRE(grid[x] < (1ll << 31), "grid too large");
+      a.grid[x] = (uint32_t)grid[x];
     }
   }
   AC4K_REQUIRE(sum == pairs, "sections of %lld pairs, the table has %lld", (long long)sum, (long long)pairs);
@@ -164,10 +247,10 @@ extern "C" __attribute__((visibility("default"))) int ac4k_rope(
   }
   a.table = reinterpret_cast<const float2 *>(table);
   a.positions = positions, a.pos_axis = pos_axis_stride, a.pos_b = pos_b_stride, a.pos_n = pos_n_stride, a.pos_bytes = positions_bytes;
-  a.B = B, a.N = N, a.length = length, a.D = (int)D, a.pairs = (int)pairs, a.axes = axes;
+  a.N = (uint32_t)N, a.length = length, a.sign = inverse ? -1.0f : 1.0f, a.D = (int)D, a.pairs = (int)pairs, a.axes = axes;
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == AC4K_DTYPE_BF16) launch_rope<AC4K_DTYPE_BF16>(a, interleaved, inverse, st);
-  else if (dtype == AC4K_DTYPE_FP16) launch_rope<AC4K_DTYPE_FP16>(a, interleaved, inverse, st);
-  else launch_rope<AC4K_DTYPE_FP32>(a, interleaved, inverse, st);
+  if (dtype == AC4K_DTYPE_BF16) launch_rope<AC4K_DTYPE_BF16>(a, B, interleaved, st);
+  else if (dtype == AC4K_DTYPE_FP16) launch_rope<AC4K_DTYPE_FP16>(a, B, interleaved, st);
+  else launch_rope<AC4K_DTYPE_FP32>(a, B, interleaved, st);
   return check_launch("ac4k_rope");
 }

@@ -31,13 +31,16 @@ def rms_norm(x, weight=None, eps=1e-6, residual=None, residual_out=None, precisi
     if view is None:
         x = x.contiguous()
         view = _rocm_ops._rows_view(x, "x")
+    fresh = out is None
     if residual is not None:
-        if _rocm_ops._rows_view(residual, "residual") is None:
+        if not residual.is_contiguous() and _rocm_ops._rows_view(residual, "residual") is None:
             if residual_out is residual:
                 raise RuntimeError("residual_out must have rows of contiguous elements, evenly apart")
             residual = residual.contiguous()
         if residual_out is None:
             residual_out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        else:
+            fresh = False
     elif residual_out is not None:
         raise RuntimeError("residual_out without a residual")
     rows, k, _ = view
@@ -59,7 +62,7 @@ def rms_norm(x, weight=None, eps=1e-6, residual=None, residual_out=None, precisi
         sf = torch.empty((align_up(rows, 16),), dtype=torch.float32, device=x.device)
     else:
         raise RuntimeError(f"precision must be None, nvfp4, fp8e4m3 or int8, not {precision}")
-    _rocm_ops.rms_norm(out, sf, global_scale, given, x, weight, residual, residual_out, precision, eps)
+    _rocm_ops.rms_norm(out, sf, global_scale, given, x, weight, residual, residual_out, precision, float(eps), view, fresh)
     got = (out,) if precision is None else (out, sf, global_scale) if precision == "nvfp4" else (out, sf)
     if residual is not None:
         got += (residual_out,)

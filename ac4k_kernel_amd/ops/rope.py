@@ -38,24 +38,32 @@ def rope(x, table, positions=None, grid=None, sections=None, layout="BNHD", inte
         raise RuntimeError(f"Unsupported layout: {layout}")
     single = isinstance(x, torch.Tensor)
     xs = (x,) if single else tuple(x)
-    if not xs or not all(isinstance(t, torch.Tensor) and t.dim() == 4 for t in xs) or not isinstance(table, torch.Tensor) or table.dim() != 3:
+    for t in xs:
+        if not isinstance(t, torch.Tensor) or t.dim() != 4:
+            raise RuntimeError("rope takes one or two 4D tensors")
+    if not xs or not isinstance(table, torch.Tensor) or table.dim() != 3:
         raise RuntimeError("rope takes one or two 4D tensors and a table of [length, pairs, 2]")
-    outs = tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in xs) if out is None else (out,) if single else tuple(out)
-    sections = (table.shape[1],) if sections is None else tuple(int(n) for n in sections)
+    fresh = out is None
+    outs = tuple([torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in xs]) if fresh else (out,) if single else tuple(out)
+    sections = (table.shape[1],) if sections is None else tuple(sections)
     bnhd = layout == "BNHD"
-    batch, tokens = xs[0].shape[0], xs[0].shape[1 if bnhd else 2]
     if positions is None:
-        grid = (tokens,) if grid is None and len(sections) == 1 else grid
+        tokens = xs[0].shape[1 if bnhd else 2]
         if grid is None:
-            raise RuntimeError("several axes need positions or a grid")
-        grid = tuple(int(g) for g in grid) if tokens else (1,) * len(sections)
+            if len(sections) != 1:
+                raise RuntimeError("several axes need positions or a grid")
+            grid = (tokens,)
+        grid = tuple([int(g) for g in grid]) if tokens else (1,) * len(sections)
     elif isinstance(positions, torch.Tensor):
-        if positions.dim() < 3:
+        while positions.dim() < 3:
             positions = positions.unsqueeze(0)
-        if positions.dim() < 3:
-            positions = positions.unsqueeze(0)
-        if positions.dim() == 3 and positions.shape[1] == 1:
-            positions = positions.expand(-1, batch, -1)
-    xs = tuple(t if t.stride(3) == 1 else t.contiguous() for t in xs)
-    _rocm_ops.rope(outs, xs, table, sections, positions, grid, bnhd, interleaved, inverse)
+        if positions.shape[1] == 1 != xs[0].shape[0]:
+            positions = positions.expand(-1, xs[0].shape[0], -1)
+    else:
+        raise RuntimeError("positions must be a CUDA tensor of int32 or int64")
+    for t in xs:
+        if t.stride(3) != 1:
+            xs = tuple([t.contiguous() if t.stride(3) != 1 else t for t in xs])
+            break
+    _rocm_ops.rope(outs, xs, table, sections, positions, grid, bnhd, interleaved, inverse, fresh)
     return outs[0] if single else outs
