@@ -547,6 +547,7 @@ def rms_norm(out, sf, global_scale, given_scale: bool, x, weight, residual, resi
             for t in (x, residual):
                 _check(_same_rows(t, residual_out) or not _may_overlap(t, residual_out),
                        "residual_out may be x or residual itself, but not overlap them otherwise")
+            _check(weight is None or not _may_overlap(weight, residual_out), "residual_out must not overlap weight")
     out_step = K
     if not fresh:
         if precision is None:
@@ -555,8 +556,8 @@ def rms_norm(out, sf, global_scale, given_scale: bool, x, weight, residual, resi
             _check(v is not None and (rows <= 1 or v[2] >= K), "out must have rows of contiguous elements, evenly apart")
             out_step = v[2]
             _check(_same_rows(out, x) or not _may_overlap(out, x), "out may be x itself, but not overlap it otherwise")
-            for t in (residual, residual_out):
-                _check(t is None or not _may_overlap(out, t), "out must not overlap residual or residual_out")
+            for t in (residual, residual_out, weight):
+                _check(t is None or not _may_overlap(out, t), "out must not overlap residual, residual_out or weight")
         else:
             nvfp4 = precision == "nvfp4"
             _check_tensor(out, torch.uint8 if nvfp4 else torch.float8_e4m3fn if precision == "fp8e4m3" else torch.int8, "out")
@@ -642,8 +643,7 @@ def rope(outs, xs, table, sections, positions, grid, bnhd: bool, interleaved: bo
         _check(False, "{} pairs do not fit a head of {}", pairs, D)
     section_arg, axes = _rope_sections(sections, pairs), len(sections)
     _same_device(x, table, positions, *xs[1:], *outs)
-    args = _RopePair()
-    empty = B == 0 or N == 0
+    args, used = _RopePair(), 0
     for i in range(count):
         t, o = xs[i], outs[i]
         if t is not x:
@@ -657,7 +657,10 @@ def rope(outs, xs, table, sections, positions, grid, bnhd: bool, interleaved: bo
             _check(o_stride[3] == 1, "heads must be contiguous")
             _check(_same_rows(t, o) or not _may_overlap(t, o), "out may be x itself, but not overlap it otherwise")
         _check(t_stride[3] == 1, "heads must be contiguous")
-        r = args[i]
+        if t.numel() == 0:
+            continue
+        r = args[used]
+        used += 1
         r.input, r.out = t.data_ptr(), o.data_ptr()
         if bnhd:
             r.in_b, r.in_n, r.in_h, _ = t_stride
@@ -667,7 +670,6 @@ def rope(outs, xs, table, sections, positions, grid, bnhd: bool, interleaved: bo
             r.in_b, r.in_h, r.in_n, _ = t_stride
             r.out_b, r.out_h, r.out_n, _ = o_stride
             r.heads = t.shape[1]
-        empty = empty or r.heads == 0
     if count == 2 and not fresh:
         _check(not any(_may_overlap(o, t) for o, t in ((outs[0], xs[1]), (outs[1], xs[0]), (outs[0], outs[1])) if o.numel() and t.numel())
                or _interleaved_heads(outs, xs), "the two tensors must not overlap each other")
@@ -682,9 +684,9 @@ def rope(outs, xs, table, sections, positions, grid, bnhd: bool, interleaved: bo
         _check(grid is not None and len(grid) == axes and min(grid) >= 1, "grid must have one size of at least 1 for each axis")
         _check(max(grid) <= length, "the table has {} positions, the grid {}", length, max(grid))
         grid_arg = (_lib._i64 * axes)(*grid)
-    if empty:
+    if used == 0:
         return
-    _lib.check(_L.ac4k_rope(args, count, tag, B, N, D, table.data_ptr(), length, pairs, section_arg, axes, pos_ptr, pos_bytes, *pos_strides,
+    _lib.check(_L.ac4k_rope(args, used, tag, B, N, D, table.data_ptr(), length, pairs, section_arg, axes, pos_ptr, pos_bytes, *pos_strides,
                             grid_arg, interleaved, inverse, _stream()))
 
 

@@ -347,7 +347,7 @@ __device__ __forceinline__ void store_tile(const f32x16 (&acc)[MI][NJ], char *ld
 // tile needs because its k-step is much shorter than the memory latency.
 // Where the rows of a tile are.  In one matrix: first = the tile's index times its height.  GROUPED: first is a multiple of four (the scales of four
 // rows are one transfer), and rows in front of `lo` are another group's; with `rows`, row i of the tile's matrix is row rows[i] of a.A,
-// clamped to its a_rows rows, and a.A_sf has a column for each i already.
+// clamped to its a_rows rows; a.A_sf is that of a.A in tiles of 64 rows, and has a column for each i already in larger ones.
 struct TileRows {
   int64_t first, lo;
   const int32_t *rows;
@@ -425,7 +425,34 @@ __device__ __forceinline__ void tile256p(const LinearArgs &a, const SplitK &sk, 
   const uint8_t *baseS;
   int64_t strideS;
   bool firstS;  // this lane's rows belong to the first chunk of a stage
-  {
+  // Gathered rows of a tile of 64: their scales are not neighbours, and come a dword per lane, the two chunks by waves 0 and 1; those of B by the
+  // waves behind them, so that it stays one transfer a wave.
+  constexpr bool OWN_SCALES = GROUPED && MI == 1;
+  bool dword_scales = false;
+  if (OWN_SCALES && tr.rows) {
+    static_assert(!OWN_SCALES || 2 + PL::NSB <= 4, "a scale transfer per wave");
+    const int t = swave < 2 + PL::NSB ? swave : 1 + PL::NSB;
+    dword_scales = t < 2;
+    int64_t row;
+    int c;
+    if (dword_scales) {
+      c = t;
+      int64_t i = m_first + lane;
+      i = tr.rows[i < a.M ? i : a.M - 1];
+      row = i < 0 ? 0 : i < tr.a_rows ? i : tr.a_rows - 1;
+    } else {
+      const int at = (t - 2) * 256 + lane * 4;
+      c = at >= BN ? 1 : 0;
+      const int loc = at < 2 * BN ? at - c * BN : 0;
+      row = tn * BN + loc + 4 <= a.Np ? tn * BN + loc : a.Np - 4;
+    }
+    const int64_t rows = dword_scales ? a.Mp : a.Np;
+    firstS = c == 0;
+    offS = (uint32_t)((c * rows + row) * 4);
+    strideS = (int64_t)uniform_ptr((const void *)(2 * rows * 4));
+    baseS = uniform_ptr(reinterpret_cast<const uint8_t *>(dword_scales ? a.A_sf : a.B_sf) - (EARLY ? rows : 0) * 4 + kt0 * strideS);
+    ldsS = (uint32_t)__builtin_amdgcn_readfirstlane(dword_scales ? PL::OFF_SFA + t * (BM * 4) : PL::OFF_SFB + (t - 2) * 1024);
+  } else {
     const int t = swave < PL::NSA + PL::NSB ? swave : PL::NSA + PL::NSB - 1;
     const bool isB = t >= PL::NSA;
     const int tt = isB ? t - PL::NSA : t, rows_t = isB ? BN : BM;
@@ -468,13 +495,17 @@ __device__ __forceinline__ void tile256p(const LinearArgs &a, const SplitK &sk, 
     p.s = baseS + kt * strideS;
     return p;
   };
+  auto issue_scales = [&](uint32_t stage_lds, const uint8_t *src, uint32_t off) {
+    if (OWN_SCALES && dword_scales) dma4(src, off, stage_lds, ldsS);
+    else dma16(src, off, stage_lds, ldsS);
+  };
   auto issue_piece = [&](uint32_t stage_lds, const Src &p, int q) {
     if (q < NDA) {
       dma16(p.a, offA[q], stage_lds, ldsA[q]);
     } else if (q < NDA + NDB) {
       dma16(p.b, offB[q - NDA], stage_lds, ldsB[q - NDA]);
     } else {
-      dma16(p.s, offS, stage_lds, ldsS);
+      issue_scales(stage_lds, p.s, offS);
     }
   };
   auto issue_stage = [&](uint32_t stage_lds, const Src &p) {
@@ -527,7 +558,7 @@ __device__ __forceinline__ void tile256p(const LinearArgs &a, const SplitK &sk, 
     for (int q = 0; q < NDA; ++q) dma16(p.a, offA[q] + shift, lds_base, ldsA[q]);
 #pragma unroll
     for (int q = 0; q < NDB; ++q) dma16(p.b, offB[q] + shift, lds_base, ldsB[q]);
-    dma16(p.s, offS + (short0 && firstS ? (uint32_t)(strideS / 2) : 0), lds_base, ldsS);
+    issue_scales(lds_base, p.s, offS + (short0 && firstS ? (uint32_t)(strideS / 2) : 0));
   }
   // A range shorter than the ring is fetched as it is and waited for as a whole: its repeats would be most of a short prologue
   // (10650 x 512 x 384 11.4 -> 10.9 us).

@@ -45,7 +45,7 @@ def rope(x, table, positions=None, grid=None, sections=None, layout="BNHD", inte
         raise RuntimeError("rope takes one or two 4D tensors and a table of [length, pairs, 2]")
     fresh = out is None
     outs = tuple([torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in xs]) if fresh else (out,) if single else tuple(out)
-    sections = (table.shape[1],) if sections is None else tuple(sections)
+    sections = (table.shape[1],) if sections is None else (sections,) if isinstance(sections, int) else tuple(sections)
     bnhd = layout == "BNHD"
     if positions is None:
         tokens = xs[0].shape[1 if bnhd else 2]

@@ -97,6 +97,15 @@ def test_rows_of_no_range_stay(sizes, n, k):
         assert (out[:6] == 7).all() and (out[-9:] == 7).all()
 
 
+def test_every_kernel():
+    """The four kernels by the shapes that take them: few rows on a long K, one tile of 64 rows an expert with narrow and wide weights, many rows;
+    K with and without a half stage, gathered rows and rows in order."""
+    for sizes, n, k in (([3, 0, 5], 4096, 2048), ([30] * 8, 2048, 512), ([20] * 40, 512, 320), ([1500, 900, 10, 1300], 1030, 320), ([1500, 900, 1, 1300], 1030, 512)):
+        for gather in (None, 500):
+            p = Problem(sizes, n, k, rows_of=gather, seed=n, bias="bf16", before=3)
+            check(p, p.run())
+
+
 def test_one_expert_is_the_linear():
     """Up to the order of the fp32 sums: two bf16 roundings apart at the most."""
     for m, n, k in ((4, 512, 1024), (300, 640, 512)):

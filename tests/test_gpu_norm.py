@@ -123,7 +123,21 @@ def test_quantized(rows, k, precision, dtype, w32, residual):
         assert torch.equal(got[-1].cpu(), h)
 
 
-@pytest.mark.parametrize("rows,k", [(1, 64), (5, 200), (600, 1040), (4101, 515)])
+# rows shared by a wave (heads of 128 and less), many turns of a workgroup, more rows than first-launch workgroups
+@pytest.mark.parametrize("rows,k", [(9000, 64), (70001, 40), (5000, 128), (300, 250), (20001, 256), (300, 8192), (9001, 1100), (2100, 13000)])
+@pytest.mark.parametrize("precision", [None, "nvfp4", "fp8e4m3", "int8"])
+def test_many_rows(rows, k, precision):
+    x, w, r = data((rows, k), torch.bfloat16, rows), data((k,), torch.bfloat16, 2), data((rows, k), torch.bfloat16, 3)
+    h, exact, y32 = reference(x, w, r)
+    got = ops().rms_norm(x.cuda(), w.cuda(), eps=EPS, residual=r.cuda(), precision=precision)
+    assert torch.equal(got[-1].cpu(), h)
+    if precision is None:
+        check_plain(got[0], exact)
+    else:
+        check_quantized(got, y32, precision)
+
+
+@pytest.mark.parametrize("rows,k", [(1, 64), (5, 200), (600, 1040), (4101, 515), (9000, 64)])
 def test_given_global_scale(rows, k):
     x, w = data((rows, k), torch.bfloat16, 1), data((k,), torch.bfloat16, 2)
     _, _, y32 = reference(x, w)

@@ -158,6 +158,26 @@ def test_gradient_by_differences():
     assert abs(left - right) <= 9216 * 4 * 2.0 ** -22  # elements, times their size and the roundings of four numbers
 
 
+def test_one_tensor_of_a_pair_without_heads():
+    q, k = data((2, 5, 3, 16), torch.bfloat16, 1).cuda(), torch.empty((2, 5, 0, 16), dtype=torch.bfloat16, device="cuda")
+    table = ops().rope_table(8, 10)
+    for pair in ((q, k), (k, q)):
+        got = ops().rope(pair, table, sections=8)
+        for x, y in zip(pair, got):
+            assert y.shape == x.shape and torch.equal(y, ops().rope(x, table))
+
+
+def test_many_tokens():
+    """Workgroups of several tokens in both layouts, and batches whose last workgroup is not full."""
+    for layout, shape in (("BNHD", (3, 3001, 2, 64)), ("BHND", (3, 5, 3001, 64)), ("BNHD", (1, 9001, 3, 40)), ("BHND", (1, 24, 2999, 128))):
+        n = shape[1] if layout == "BNHD" else shape[2]
+        x = data(shape, torch.bfloat16, n)
+        pos = torch.randint(0, 50, (1, shape[0], n), generator=torch.Generator().manual_seed(1))
+        pairs = shape[3] // 2
+        y = ops().rope(x.cuda(), ops().rope_table(pairs, 50), positions=pos.cuda(), layout=layout, interleaved=layout == "BNHD")
+        check(y, exact(x, pos, (pairs,), layout, layout == "BNHD"))
+
+
 def test_empty():
     table = ops().rope_table(8, 10)
     assert ops().rope(torch.empty((0, 4, 2, 16), device="cuda"), table).shape == (0, 4, 2, 16)

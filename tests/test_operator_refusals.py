@@ -173,7 +173,7 @@ def test_norm_operands():
                      ((shifted, w), dict(out=over)), ((shifted, w), dict(residual=x, residual_out=over)),
                      ((x, w), dict(residual=shifted, residual_out=over)), ((x, w), dict(residual=x.clone(), out=(o := torch.empty_like(x)), residual_out=o)),
                      ((x, w), dict(precision="nvfp4", global_scale=torch.zeros(1, device="cuda"))),
-                     ((x, w), dict(residual=x, residual_out=x[:1].expand(4, 64))), ((torch.zeros((2, 65537), device="cuda"),), {})):
+                     ((x, w), dict(residual=x, residual_out=x[:1].expand(4, 64))), ((x[0], w), dict(out=w)), ((x[0], w), dict(residual=x[1], residual_out=w)), ((torch.zeros((2, 65537), device="cuda"),), {})):
         with pytest.raises(RuntimeError):
             ops().rms_norm(*args, **kw)
 
