@@ -523,21 +523,29 @@ def rms_norm(out, sf, global_scale, given_scale: bool, x, weight, residual, resi
     number = _PRECISIONS.get(precision)
     if number is None:
         _check(False, "precision must be one of {}", list(_PRECISIONS))
-    _same_device(x, weight, residual, residual_out, out, sf, global_scale)
+    dev = _current_device()
+    if x.get_device() != dev or not fresh or global_scale is not None:
+        _same_device(x, residual_out, out, sf, global_scale)
     weight_ptr, weight_tag = None, tag
     if weight is not None:
         weight_tag = _check_float(weight, "weight")
-        _check(weight_tag == tag or weight_tag == 2, "weight must have the type of x or be float")
+        if (weight_tag != tag and weight_tag != 2) or weight.get_device() != dev:
+            _check(weight.get_device() == dev, "weight must be on the current device")
+            _check(False, "weight must have the type of x or be float")
         if weight.shape != (K,) or not weight.is_contiguous():
             _check(False, "weight must be contiguous of [{}]", K)
         weight_ptr = weight.data_ptr()
-    _check((residual is None) == (residual_out is None), "a residual comes with residual_out, and the other way round")
+    if (residual is None) != (residual_out is None):
+        _check(False, "a residual comes with residual_out, and the other way round")
     residual_ptr = sum_ptr = None
     residual_step = sum_step = 0
     if residual is not None:
-        _check(_check_float(residual, "residual") == tag and residual.shape == x.shape, "residual must have the type and shape of x")
+        if _check_float(residual, "residual") != tag or residual.shape != x.shape or residual.get_device() != dev:
+            _check(residual.get_device() == dev, "residual must be on the current device")
+            _check(False, "residual must have the type and shape of x")
         v = _rows_view(residual, "residual")
-        _check(v is not None, "residual must have rows of contiguous elements, evenly apart")
+        if v is None:
+            _check(False, "residual must have rows of contiguous elements, evenly apart")
         residual_ptr, residual_step, sum_ptr, sum_step = residual.data_ptr(), v[2], residual_out.data_ptr(), K
         if not fresh:
             _check(_check_float(residual_out, "residual_out") == tag and residual_out.shape == x.shape, "residual_out must have the type and shape of x")
@@ -584,30 +592,40 @@ def rms_norm(out, sf, global_scale, given_scale: bool, x, weight, residual, resi
 def dequantize(out, q, sf, global_scale=None) -> None:
     """out [.., R, cols] <- the values of q, sf (and global_scale, for nvfp4) as `quantize` returns them without swizzle."""
     tag = _check_float(out, "out")
-    _check(isinstance(q, torch.Tensor) and q.dim() >= 2, "q must have at least two dims")
-    nvfp4 = q.dtype == torch.uint8
-    _check(nvfp4 or q.dtype in _EIGHT_BITS, "q must be uint8 (nvfp4), float8_e4m3fn or int8")
+    if not isinstance(q, torch.Tensor) or q.dim() < 2:
+        _check(False, "q must have at least two dims")
+    nvfp4 = q.dtype is torch.uint8
+    number = 3 if nvfp4 else _EIGHT_BITS.get(q.dtype)
+    if number is None:
+        _check(False, "q must be uint8 (nvfp4), float8_e4m3fn or int8")
     _check_tensor(q, q.dtype, "q")
-    _same_device(q, out, sf, global_scale)
-    lead, R, W = list(q.shape[:-2]), q.size(-2), q.size(-1) * (2 if nvfp4 else 1)
-    _check(W % (64 if nvfp4 else 16) == 0, "rows of q must be whole pieces of {} elements", 64 if nvfp4 else 16)
     _check_tensor(sf, torch.float8_e4m3fn if nvfp4 else torch.float32, "sf")
-    _check(list(sf.shape) == lead + ([W // 64, _align_up(R, 16), 4] if nvfp4 else [_align_up(R, 16)]), "meet invalid sf shape")
-    planes = 1
+    _same_device(q, out, sf, global_scale)
+    *lead, R, W = q.shape
+    planes, gs_step, gs_ptr = 1, 0, None
     for n in lead:
         planes *= n
-    gs_step = 0
     if nvfp4:
+        W *= 2
+        if W % 64 != 0 or sf.shape != (*lead, W // 64, (R + 15) // 16 * 16, 4):
+            _check(W % 64 == 0, "rows of q must be whole pieces of 64 elements")
+            _check(False, "meet invalid sf shape")
         _check_tensor(global_scale, torch.float32, "global_scale")
-        _check(global_scale.dim() == 0 or list(global_scale.shape) == lead, "global_scale must be a scalar or have the leading dims of q")
-        gs_step = int(global_scale.dim() > 0)
+        if global_scale.dim() != 0:
+            _check(list(global_scale.shape) == lead, "global_scale must be a scalar or have the leading dims of q")
+            gs_step = 1
+        gs_ptr = global_scale.data_ptr()
     else:
+        if W % 16 != 0 or sf.shape != (*lead, (R + 15) // 16 * 16):
+            _check(W % 16 == 0, "rows of q must be whole pieces of 16 elements")
+            _check(False, "meet invalid sf shape")
         _check(global_scale is None, "only nvfp4 has a global scale")
-    _check(out.is_contiguous() and list(out.shape[:-1]) == lead + [R] and out.size(-1) <= W, "out must be contiguous of [.., {}, up to {}]", R, W)
+    *out_lead, cols = out.shape
+    if not out.is_contiguous() or out_lead != [*lead, R] or cols > W:
+        _check(False, "out must be contiguous of [.., {}, up to {}]", R, W)
     if out.numel() == 0:
         return
-    _lib.check(_L.ac4k_dequantize(out.data_ptr(), tag, q.data_ptr(), sf.data_ptr(), None if global_scale is None else global_scale.data_ptr(),
-                                  gs_step, planes, R, W, out.size(-1), 3 if nvfp4 else _EIGHT_BITS[q.dtype], _stream()))
+    _lib.check(_L.ac4k_dequantize(out.data_ptr(), tag, q.data_ptr(), sf.data_ptr(), gs_ptr, gs_step, planes, R, W, cols, number, _stream()))
 
 
 _ROPE_SECTIONS = {}
@@ -625,59 +643,57 @@ def _rope_sections(sections, pairs: int):
 
 
 _RopePair = _lib.RopeTensor * 2
+_POSITIONS = {torch.int32, torch.int64}
 
 
 def rope(outs, xs, table, sections, positions, grid, bnhd: bool, interleaved: bool, inverse: bool, fresh: bool = False) -> None:
     """outs <- xs (one or two tensors) turned by the angles of their tokens' positions.  fresh: outs are new dense tensors."""
     count = len(xs)
-    _check(count in (1, 2) and len(outs) == count, "rope takes one or two tensors, and as many outputs")
+    if count not in (1, 2) or len(outs) != count:
+        _check(False, "rope takes one or two tensors, and as many outputs")
     x = xs[0]
     tag = _check_float(x, "x")
-    _check(x.dim() == 4, "x must be a 4D tensor")
     _check_tensor(table, torch.float32, "table")
-    _check(table.dim() == 3 and table.shape[2] == 2, "table must be [length, pairs, 2]")
-    (B, a, b, D), (length, pairs, _) = x.shape, table.shape
-    N = a if bnhd else b
-    _check(length >= 1 and pairs >= 1, "table must be [length, pairs, 2]")
-    if 2 * pairs > D:
+    if x.dim() != 4 or table.dim() != 3 or table.shape[2] != 2:
+        _check(x.dim() == 4, "x must be a 4D tensor")
+        _check(False, "table must be [length, pairs, 2]")
+    (B, N, _, D), (length, pairs, _) = x.shape, table.shape
+    if not bnhd:
+        N = x.shape[2]
+    if length < 1 or pairs < 1 or 2 * pairs > D:
+        _check(length >= 1 and pairs >= 1, "table must be [length, pairs, 2]")
         _check(False, "{} pairs do not fit a head of {}", pairs, D)
     section_arg, axes = _rope_sections(sections, pairs), len(sections)
-    _same_device(x, table, positions, *xs[1:], *outs)
+    _same_device(*xs, table, positions)
     args, used = _RopePair(), 0
-    for i in range(count):
-        t, o = xs[i], outs[i]
+    for t, o in zip(xs, outs):
         if t is not x:
             _check(_check_float(t, "x") == tag, "all tensors must have one type")
             _check(t.dim() == 4 and t.shape[0] == B and t.shape[1 if bnhd else 2] == N and t.shape[3] == D,
                    "all tensors must have the same batch, tokens and head dim")
-        t_stride, o_stride = t.stride(), o.stride()
+        t_b, t_n, t_h, t_d = t.stride()
+        o_b, o_n, o_h, o_d = o.stride()
         if not fresh:
+            _same_device(o)
             _check(_check_float(o, "out") == tag, "all tensors must have one type")
             _check(o.shape == t.shape, "out must have the shape of x")
-            _check(o_stride[3] == 1, "heads must be contiguous")
+            _check(o_d == 1, "heads must be contiguous")
             _check(_same_rows(t, o) or not _may_overlap(t, o), "out may be x itself, but not overlap it otherwise")
-        _check(t_stride[3] == 1, "heads must be contiguous")
+        if t_d != 1:
+            _check(False, "heads must be contiguous")
         if t.numel() == 0:
             continue
-        r = args[used]
+        args[used] = ((t.data_ptr(), o.data_ptr(), t_b, t_n, t_h, o_b, o_n, o_h, t.shape[2]) if bnhd else
+                      (t.data_ptr(), o.data_ptr(), t_b, t_h, t_n, o_b, o_h, o_n, t.shape[1]))
         used += 1
-        r.input, r.out = t.data_ptr(), o.data_ptr()
-        if bnhd:
-            r.in_b, r.in_n, r.in_h, _ = t_stride
-            r.out_b, r.out_n, r.out_h, _ = o_stride
-            r.heads = t.shape[2]
-        else:
-            r.in_b, r.in_h, r.in_n, _ = t_stride
-            r.out_b, r.out_h, r.out_n, _ = o_stride
-            r.heads = t.shape[1]
     if count == 2 and not fresh:
         _check(not any(_may_overlap(o, t) for o, t in ((outs[0], xs[1]), (outs[1], xs[0]), (outs[0], outs[1])) if o.numel() and t.numel())
                or _interleaved_heads(outs, xs), "the two tensors must not overlap each other")
     pos_ptr, pos_bytes, pos_strides, grid_arg = None, 0, (0, 0, 0), None
     if positions is not None:
-        _check(grid is None, "positions or a grid, one of them")
-        _check(positions.is_cuda and positions.dtype in (torch.int32, torch.int64), "positions must be a CUDA tensor of int32 or int64")
-        if positions.shape != (axes, B, N):
+        if grid is not None or positions.dtype not in _POSITIONS or positions.shape != (axes, B, N):
+            _check(grid is None, "positions or a grid, one of them")
+            _check(positions.is_cuda and positions.dtype in _POSITIONS, "positions must be a CUDA tensor of int32 or int64")
             _check(False, "positions must be [{}, {}, {}]", axes, B, N)
         pos_ptr, pos_bytes, pos_strides = positions.data_ptr(), positions.element_size(), positions.stride()
     else:

@@ -38,7 +38,7 @@ def rms_norm(x, weight=None, eps=1e-6, residual=None, residual_out=None, precisi
                 raise RuntimeError("residual_out must have rows of contiguous elements, evenly apart")
             residual = residual.contiguous()
         if residual_out is None:
-            residual_out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            residual_out = torch.empty_like(x, memory_format=torch.contiguous_format)
         else:
             fresh = False
     elif residual_out is not None:
@@ -49,17 +49,17 @@ def rms_norm(x, weight=None, eps=1e-6, residual=None, residual_out=None, precisi
         raise RuntimeError("only nvfp4 has a global scale")
     if precision is None:
         if out is None:
-            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            out = torch.empty_like(x, memory_format=torch.contiguous_format)
     elif out is not None:
         raise RuntimeError("out is for unquantized results")
     elif precision == "nvfp4":
-        out = torch.empty((rows, align_up(k, 64) // 2), dtype=torch.uint8, device=x.device)
-        sf = torch.empty((align_up(k, 64) // 64, align_up(rows, 16), 4), dtype=torch.float8_e4m3fn, device=x.device)
+        out = x.new_empty((rows, align_up(k, 64) // 2), dtype=torch.uint8)
+        sf = x.new_empty((align_up(k, 64) // 64, align_up(rows, 16), 4), dtype=torch.float8_e4m3fn)
         if not given:
-            global_scale = torch.empty((), dtype=torch.float32, device=x.device)
+            global_scale = x.new_empty((), dtype=torch.float32)
     elif precision in _OUT_DTYPES:
-        out = torch.empty((rows, align_up(k, 16)), dtype=_OUT_DTYPES[precision], device=x.device)
-        sf = torch.empty((align_up(rows, 16),), dtype=torch.float32, device=x.device)
+        out = x.new_empty((rows, align_up(k, 16)), dtype=_OUT_DTYPES[precision])
+        sf = x.new_empty((align_up(rows, 16),), dtype=torch.float32)
     else:
         raise RuntimeError(f"precision must be None, nvfp4, fp8e4m3 or int8, not {precision}")
     _rocm_ops.rms_norm(out, sf, global_scale, given, x, weight, residual, residual_out, precision, float(eps), view, fresh)
@@ -78,6 +78,6 @@ def dequantize(output, sf, global_scale=None, dtype=torch.bfloat16, cols=None, o
     """
     if out is None:
         width = output.shape[-1] * (2 if output.dtype == torch.uint8 else 1)
-        out = torch.empty((*output.shape[:-1], width if cols is None else cols), dtype=dtype, device=output.device)
+        out = output.new_empty((*output.shape[:-1], width if cols is None else cols), dtype=dtype)
     _rocm_ops.dequantize(out, output, sf, global_scale)
     return out

@@ -44,7 +44,7 @@ def rope(x, table, positions=None, grid=None, sections=None, layout="BNHD", inte
     if not xs or not isinstance(table, torch.Tensor) or table.dim() != 3:
         raise RuntimeError("rope takes one or two 4D tensors and a table of [length, pairs, 2]")
     fresh = out is None
-    outs = tuple([torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in xs]) if fresh else (out,) if single else tuple(out)
+    outs = tuple([torch.empty_like(t, memory_format=torch.contiguous_format) for t in xs]) if fresh else (out,) if single else tuple(out)
     sections = (table.shape[1],) if sections is None else (sections,) if isinstance(sections, int) else tuple(sections)
     bnhd = layout == "BNHD"
     if positions is None:
