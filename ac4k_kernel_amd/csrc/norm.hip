@@ -129,14 +129,16 @@ __global__ __launch_bounds__(64 * BW) void rms_norm_kernel(NormArgs a, int rows_
   const int cut = (int)(a.K & 7);
   const int64_t k_cut = a.K - cut;
   const bool cut_mine = cut != 0 && (int)(k_cut / 8 % LPR) == sub;
-  // the weights, once for all rows of the workgroup, and under way before the first row's sum is known
-  Vec8<WT> w[NV];
+  // the weights, once for all rows of the workgroup, and under way before the first row's sum is known; rows of eight vectors leave no
+  // registers for them, and read them where they are used
+  constexpr bool HELD = NV <= 4;
+  Vec8<WT> w[HELD ? NV : 1];
   const bool weighted = a.weight != nullptr;
-  if (weighted) {
+  if (HELD && weighted) {
     Vec8<WT> w_cut;
     cut_load(w_cut, a.weight, k_cut, cut_mine, cut);
 #pragma unroll
-    for (int j = 0; j < NV; ++j) row_vector(w[j], a.weight, (j * LPR + sub) * 8, a.K, w_cut);
+    for (int j = 0; j < (HELD ? NV : 0); ++j) row_vector(w[j], a.weight, (j * LPR + sub) * 8, a.K, w_cut);
   }
   uint32_t block_m = 0;
   const int64_t row0 = (int64_t)blockIdx.x * rows_per_block;
@@ -156,17 +158,19 @@ __global__ __launch_bounds__(64 * BW) void rms_norm_kernel(NormArgs a, int rows_
     if constexpr (SUMS) {
       if (a.residual && valid) {
         const T *rp = static_cast<const T *>(a.residual) + row * a.residual_stride;
-        Vec8<DT> q[NV], r_cut;
+        Vec8<DT> q[HELD ? NV : 1], r_cut;
         cut_load(r_cut, rp, k_cut, cut_mine, cut);
 #pragma unroll
-        for (int j = 0; j < NV; ++j) row_vector(q[j], rp, (j * LPR + sub) * 8, a.K, r_cut);
+        for (int j = 0; j < (HELD ? NV : 0); ++j) row_vector(q[j], rp, (j * LPR + sub) * 8, a.K, r_cut);
         T *sp = static_cast<T *>(a.sum) + row * a.sum_stride;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
           const int k = (j * LPR + sub) * 8;
+          Vec8<DT> &v = q[HELD ? j : 0];
+          if constexpr (!HELD) row_vector(v, rp, k, a.K, r_cut);
           float f[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) f[i] = vec8_get(h[j], i) + vec8_get(q[j], i);
+          for (int i = 0; i < 8; ++i) f[i] = vec8_get(h[j], i) + vec8_get(v, i);
           vec8_set(h[j], f);
           if (k + 8 <= a.K) vec8_store_all(sp + k, h[j]);
           else if (k < a.K) r_cut = h[j];
@@ -205,8 +209,10 @@ __global__ __launch_bounds__(64 * BW) void rms_norm_kernel(NormArgs a, int rows_
 #pragma unroll
       for (int i = 0; i < 8; ++i) y[i] = vec8_get(h[j], i) * r;
       if (weighted) {
+        Vec8<WT> &v = w[HELD ? j : 0];
+        if constexpr (!HELD) vec8_load(v, a.weight, k, a.K);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = y[i] * vec8_get(w[j], i);
+        for (int i = 0; i < 8; ++i) y[i] = y[i] * vec8_get(v, i);
       }
       // behind the row the product 0 * r * 0 is not 0 where r is not finite
       if (k + 8 > a.K) {
@@ -239,12 +245,22 @@ __global__ __launch_bounds__(64 * BW) void rms_norm_kernel(NormArgs a, int rows_
       }
     } else if constexpr (OUT == NORM_FP8 || OUT == NORM_INT8 || OUT == NORM_STATS || OUT == NORM_NVFP4_ONE) {
       uint32_t m = 0;
+      constexpr bool KEEP = (OUT == NORM_FP8 || OUT == NORM_INT8) && NV <= 4;  // y stays in registers for the conversion
+      float kept[KEEP ? NV : 1][8];
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        if ((j * LPR + sub) * 8 >= a.K) continue;
-        float y[8];
-        values(j, y);
-        m = umax32(m, max8(y));
+        if constexpr (KEEP) {
+          float y[8] = {};
+          if ((j * LPR + sub) * 8 < a.K) values(j, y);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) kept[j][i] = y[i];
+          m = umax32(m, max8(y));
+        } else {
+          if ((j * LPR + sub) * 8 >= a.K) continue;
+          float y[8];
+          values(j, y);
+          m = umax32(m, max8(y));
+        }
       }
       if constexpr (OUT == NORM_STATS) {
         if (valid) {
@@ -275,20 +291,31 @@ __global__ __launch_bounds__(64 * BW) void rms_norm_kernel(NormArgs a, int rows_
           const int k = (j * LPR + sub) * 8;
           if (k >= a.Kp) continue;
           float y[8];
-          values(j, y);
+          if constexpr (KEEP) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = kept[j][i];
+          } else {
+            values(j, y);
+          }
+          // |y * factor| is at most `most` and a rounding, which rounds back to it: nothing to clamp
           uint32_t lo, hi;
           if constexpr (OUT == NORM_FP8) {
-            lo = f32x4_to_e4m3x4(y[0] * factor, y[1] * factor, y[2] * factor, y[3] * factor);
-            hi = f32x4_to_e4m3x4(y[4] * factor, y[5] * factor, y[6] * factor, y[7] * factor);
+            lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[0] * factor, y[1] * factor, 0, false);
+            lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[2] * factor, y[3] * factor, lo, true);
+            hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[4] * factor, y[5] * factor, 0, false);
+            hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[6] * factor, y[7] * factor, hi, true);
             if (factor != factor) lo = hi = 0x7f7f7f7fu;
           } else {
-            auto s8 = [&](float v) {
-              int q = (int)__builtin_rintf(v * factor);  // saturates, NaN gives 0
-              q = q < -127 ? -127 : q > 127 ? 127 : q;
-              return (uint32_t)q & 0xffu;
+            // added to 1.5 * 2^23, a value is rounded to the nearest whole number (ties to even), whose low byte is that of the sum
+            uint32_t b[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) b[i] = __float_as_uint(y[i] * factor + 12582912.0f);
+            auto bytes4 = [](uint32_t p, uint32_t q, uint32_t r, uint32_t t) {
+              return __builtin_amdgcn_perm(__builtin_amdgcn_perm(t, r, 0x0c0c0400u), __builtin_amdgcn_perm(q, p, 0x0c0c0400u), 0x05040100u);
             };
-            lo = s8(y[0]) | s8(y[1]) << 8 | s8(y[2]) << 16 | s8(y[3]) << 24;
-            hi = s8(y[4]) | s8(y[5]) << 8 | s8(y[6]) << 16 | s8(y[7]) << 24;
+            lo = bytes4(b[0], b[1], b[2], b[3]);
+            hi = bytes4(b[4], b[5], b[6], b[7]);
+            if (factor != factor) lo = hi = 0;
           }
           st_elem_u2(op + k, make_uint2(lo, hi));
         }
