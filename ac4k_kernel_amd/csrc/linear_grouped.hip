@@ -219,14 +219,15 @@ enum GroupedKind { GROUPED_ROWS16, GROUPED_64_128, GROUPED_64_256, GROUPED_256_2
 
 // (the tile kernel's 32-bit lane offsets: whole of x where rows are gathered, the rows of a tile and of a band otherwise)
 static bool grouped_tiles_fit(int64_t T, int64_t N, int64_t K, bool gather) {
-  return K >= P_BK && N >= 128 && (K >> 1) * 260 < (1ll << 31) && (!gather || T * (K >> 1) < (1ll << 32) - 64) && N < (1ll << 27);
+  return K >= P_BK && (K >> 1) * 260 < (1ll << 31) && (!gather || T * (K >> 1) < (1ll << 32) - 64) && N < (1ll << 27);
 }
 // Which kernel, by the time that each is expected to take (us), fitted to 100 shapes of 8 to 128 experts, N of 1003 to 14336, K of 2048 to 14336 and 1 to
 // 2048 rows an expert.  What is known on the host are the counts; the groups are taken for those of rows dealt out evenly at random.  A tile of a
 // shape takes so long for each 4096 of K, and so long besides, with its CU full of them; tiles go to the CUs in whole rounds while these
 // are few.  64 x 256 and 64 x 128 tiles are two to a CU: memory latency and the exchange at the end of one lie under the other's work.
 // Measured, us (256 x 256 / 64 x 256 / 64 x 128 / 16 rows):  8 experts of 14336 x 4096, 2 rows each 162 / 57 / 66 / 80, 128 157 / 137 / 147 / 570,
-// 2048 1291 / 1498 / 1795; 8 of 4096 x 14336, 8 rows 236 / 92 / 69 / 73; 16 of 4096 x 4096, 512 rows 237 / 235 / 274; 128 x 128 tiles, one or two to a CU,
+// 2048 1291 / 1498 / 1795; 8 of 4096 x 14336, 8 rows 236 / 92 / 69 / 73; 16 of 4096 x 4096, 512 rows 237 / 235 / 274; 8 of 64 x 4096, 16 rows 69 / 33 / 23 / 12,
+// 512 69 / 35 / 24; 128 x 128 tiles, one or two to a CU,
 // were nowhere more than 6 % ahead of the best of these.
 static GroupedKind grouped_kind(int64_t T, int64_t M, int64_t N, int64_t K, int64_t E, bool gather) {
   if (!grouped_tiles_fit(T, N, K, gather)) return GROUPED_ROWS16;
@@ -243,7 +244,9 @@ static GroupedKind grouped_kind(int64_t T, int64_t M, int64_t N, int64_t K, int6
   GroupedKind kind = t256 < t64 ? GROUPED_256_256 : GROUPED_64_256;
   double best = t256 < t64 ? t256 : t64;
   if (t128 < best) kind = GROUPED_64_128, best = t128;
-  if ((double)M <= 16 * groups && 8 + groups * (double)N * (double)K * 0.5625 / 3.5e6 < best) kind = GROUPED_ROWS16;  // bytes of the weights
+  // 16 weight rows a workgroup: the weights' bytes, and what a second set of 16 activation rows adds
+  const double read = groups * (double)N * (double)K * 0.5625 / 3.5e6;
+  if ((double)M <= 32 * groups && 8 + read * ((double)M <= 16 * groups ? 1.0 : 2.3) < best) kind = GROUPED_ROWS16;
   return kind;
 }
 

@@ -39,8 +39,9 @@ struct RopeArgs {
   float sign;                   // of the sines
 };
 
-// WHOLE: no vector is cut by the end of the pairs or of the head; four of them are under way at a time then, with no branch between their loads
-// (with the loads of cut vectors in between, every load was waited for by itself).
+// WHOLE: no vector is cut by the end of the pairs or of the head, or the last one is moved back to end there, and two threads write the same
+// values to what lies in both (not in place, where one could read what the other has turned).  Four vectors are under way at a time then, with
+// no branch between their loads (with the loads of cut vectors in between, every load was waited for by itself: 20000 x 48 heads of 40, halves, 54 us, now 30).
 template <int DT, bool INTERLEAVED, bool WHOLE>
 __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
   using T = typename Elem<DT>::T;
@@ -61,8 +62,9 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
 
   // first element of what the thread moves of a head, and the end of its kind
   const bool turned = v < a.rot_vecs;
-  const int k0 = turned ? v * 8 : rot + (v - a.rot_vecs) * 8;
   const int k1 = !turned ? a.D : INTERLEAVED ? rot : a.pairs;
+  int k0 = turned ? v * 8 : rot + (v - a.rot_vecs) * 8;
+  if (WHOLE && k0 > k1 - 8) k0 = k1 - 8;
   const uint32_t first = a.t[0].heads, heads = first + a.t[1].heads;
   const T *in[2];
   T *out[2];
@@ -93,7 +95,7 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
 
   float c[NP], s[NP];
   bool stay = false;
-  const int pair0 = v * NP;
+  const int pair0 = INTERLEAVED ? k0 / 2 : k0;
   int64_t at[NP];
   int axis_end = 0;  // of the first pair
   {
@@ -203,7 +205,9 @@ static void launch_rope(RopeArgs a, int64_t B, bool interleaved, hipStream_t st)
   a.across = across >> a.once_log;
   a.blocks_b = (a.N + (1u << a.once_log) - 1) >> a.once_log;
   const dim3 grid((unsigned)(B * a.blocks_b));
-  const bool whole = (interleaved ? 2 * a.pairs : a.pairs) % 8 == 0 && (a.D - 2 * a.pairs) % 8 == 0;
+  const bool apart = a.t[0].in != a.t[0].out && (a.t[1].heads == 0 || a.t[1].in != a.t[1].out);  // (they do not overlap otherwise)
+  auto fits = [&](int n) { return n % 8 == 0 || (n >= 8 && apart); };
+  const bool whole = fits(interleaved ? 2 * a.pairs : a.pairs) && fits(a.D - 2 * a.pairs);
   auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, a); };
   if (interleaved) whole ? go(rope_kernel<DT, true, true>) : go(rope_kernel<DT, true, false>);
   else whole ? go(rope_kernel<DT, false, true>) : go(rope_kernel<DT, false, false>);

@@ -106,6 +106,18 @@ def test_every_kernel():
             check(p, p.run())
 
 
+@pytest.mark.parametrize("n", [1, 15, 16, 33, 64, 100, 127])
+def test_narrow_weights_and_many_rows(n):
+    """Fewer weight rows than a tile has, down to one: what lies behind the last one is neither read nor written."""
+    for k in (128, 320):
+        p = Problem([700, 0, 300, 65], n, k, rows_of=400, seed=n, bias="fp32", behind=2)
+        buf = torch.full((p.m * n + 4096,), 7.0, dtype=torch.float32, device="cuda")
+        out = buf[2048:2048 + p.m * n].reshape(p.m, n)
+        p.run(out=out)
+        check(p, out)
+        assert (buf[:2048] == 7).all() and (out[-2:] == 7).all() and (buf[2048 + p.m * n:] == 7).all()
+
+
 def test_one_expert_is_the_linear():
     """Up to the order of the fp32 sums: two bf16 roundings apart at the most."""
     for m, n, k in ((4, 512, 1024), (300, 640, 512)):

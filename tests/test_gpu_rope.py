@@ -146,6 +146,22 @@ def test_views_in_place_and_packed_projection():
     check(ops().rope(wide, ops().rope_table(12, 100), positions=pos.cuda()), exact(odd[..., ::2], pos, (12,), "BNHD", True))
 
 
+@pytest.mark.parametrize("d,pairs", [(40, 20), (36, 18), (50, 20), (96, 44), (26, 9), (64, 30), (130, 60), (13, 5)])
+def test_cut_vectors_in_place(d, pairs):
+    """Widths that are no multiple of a vector: in place the same bits as into another tensor, one tensor and two."""
+    table = ops().rope_table(pairs, 50)
+    pos = torch.randint(0, 50, (1, 2, 33), generator=torch.Generator().manual_seed(1))
+    for interleaved in (True, False):
+        q, k = data((2, 33, 7, d), torch.bfloat16, d), data((2, 33, 3, d), torch.bfloat16, d + 1)
+        fresh = ops().rope((q.cuda(), k.cuda()), table, positions=pos.cuda(), interleaved=interleaved)
+        qc, kc = q.cuda(), k.cuda()
+        ops().rope((qc, kc), table, positions=pos.cuda(), interleaved=interleaved, out=(qc, kc))
+        alone = q.cuda()
+        ops().rope(alone, table, positions=pos.cuda(), interleaved=interleaved, out=alone)
+        check(fresh[0], exact(q, pos, (pairs,), "BNHD", interleaved))
+        assert torch.equal(qc, fresh[0]) and torch.equal(kc, fresh[1]) and torch.equal(alone, fresh[0])
+
+
 def test_gradient_by_differences():
     """<rope(x + d) - rope(x), g> = <d, inverse(g)> for a linear map, in fp32."""
     sections = (22, 21, 21)
