@@ -509,6 +509,16 @@ def _may_overlap(a, b) -> bool:
     return a0 < b1 and b0 < a1
 
 
+def _places_of_their_own(t) -> bool:
+    """Whether no two elements of t share memory, as far as strides in rising order say."""
+    reach = 1
+    for s, n in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
+        if s < reach:
+            return False
+        reach = s * n
+    return True
+
+
 def _same_rows(a, b) -> bool:
     return a.data_ptr() == b.data_ptr() and a.stride() == b.stride()
 
@@ -677,7 +687,7 @@ def rope(outs, xs, table, sections, positions, grid, bnhd: bool, interleaved: bo
             _same_device(o)
             _check(_check_float(o, "out") == tag, "all tensors must have one type")
             _check(o.shape == t.shape, "out must have the shape of x")
-            _check(o_d == 1, "heads must be contiguous")
+            _check(o_d == 1 and _places_of_their_own(o), "heads of out must be contiguous, and apart from each other")
             _check(_same_rows(t, o) or not _may_overlap(t, o), "out may be x itself, but not overlap it otherwise")
         if t_d != 1:
             _check(False, "heads must be contiguous")

@@ -250,28 +250,36 @@ static GroupedKind grouped_kind(int64_t T, int64_t M, int64_t N, int64_t K, int6
   return kind;
 }
 
+// Workgroups of a tile launch: rows in tiles, and at most one tile more for each group that has rows
+static int64_t grouped_tiles(int64_t M, int64_t N, int64_t E, GroupedKind kind) {
+  const int bm = kind == GROUPED_256_256 ? 256 : 64, bn = kind == GROUPED_64_128 ? 128 : 256;
+  const int64_t groups = E < M ? E : M;
+  return (M + groups * (bm + 2)) / bm * ceil_div(N, bn);
+}
+
 template <int D_DT, int BIAS_DT, int MI, int NJ, int KW, int PS, int PER_CU>
-static int launch_grouped_tile(const GroupedArgs &a, hipStream_t st) {
-  constexpr int BM = 64 * MI;
+static int launch_grouped_tile(GroupedArgs a, GroupedKind kind, uint32_t *scales, hipStream_t st) {
   const bool early = a.K % P_BK != 0;
   auto *kern = early ? linear_grouped_tile_kernel<D_DT, BIAS_DT, MI, NJ, PS, KW, true, PER_CU> : linear_grouped_tile_kernel<D_DT, BIAS_DT, MI, NJ, PS, KW, false, PER_CU>;
-  using PL = PLayout<BM, 64 * NJ, PS>;
+  using PL = PLayout<64 * MI, 64 * NJ, PS>;
   static std::atomic<uint32_t> lds_ok[2];
   if (int rc = allow_dynamic_lds(kern, lds_ok[early], PL::LDS_BYTES)) return rc;
-  // rows in tiles, and at most one tile more for each group that has rows
-  const int64_t groups = a.E < a.M ? a.E : a.M;
-  const int64_t tiles = (a.M + groups * (BM + 2)) / BM * ceil_div(a.N, 64 * NJ);
-  AC4K_REQUIRE(tiles < (1ll << 24), "problem too large");  // 2^32 threads a launch
-  hipLaunchKernelGGL(kern, dim3((unsigned)tiles), dim3(256), PL::LDS_BYTES, st, a);
+  if (MI > 1 && a.rows) {
+    const int64_t Mp = align_up(a.M, 16);
+    hipLaunchKernelGGL(gather_scales_kernel, dim3((unsigned)ceil_div(Mp, 256), (unsigned)(a.K / 64)), dim3(256), 0, st, scales, a.A_sf, a.rows, a.M, Mp, a.T, a.Tp);
+    a.A_sf = scales;
+    a.Tp = Mp;
+  }
+  hipLaunchKernelGGL(kern, dim3((unsigned)grouped_tiles(a.M, a.N, a.E, kind)), dim3(256), PL::LDS_BYTES, st, a);
   return 0;
 }
 
 template <int D_DT, int BIAS_DT>
-static int launch_grouped(const GroupedArgs &a, GroupedKind kind, hipStream_t st) {
+static int launch_grouped(const GroupedArgs &a, GroupedKind kind, uint32_t *scales, hipStream_t st) {
   switch (kind) {
-    case GROUPED_256_256: return launch_grouped_tile<D_DT, BIAS_DT, 4, 4, 1, 3, 1>(a, st);
-    case GROUPED_64_256: return launch_grouped_tile<D_DT, BIAS_DT, 1, 4, 2, 3, 2>(a, st);
-    case GROUPED_64_128: return launch_grouped_tile<D_DT, BIAS_DT, 1, 2, 2, 5, 2>(a, st);
+    case GROUPED_256_256: return launch_grouped_tile<D_DT, BIAS_DT, 4, 4, 1, 3, 1>(a, kind, scales, st);
+    case GROUPED_64_256: return launch_grouped_tile<D_DT, BIAS_DT, 1, 4, 2, 3, 2>(a, kind, scales, st);
+    case GROUPED_64_128: return launch_grouped_tile<D_DT, BIAS_DT, 1, 2, 2, 5, 2>(a, kind, scales, st);
     case GROUPED_ROWS16: break;
   }
   const dim3 grid((unsigned)ceil_div(a.N, R16_ROWS), (unsigned)a.E);
@@ -281,12 +289,12 @@ static int launch_grouped(const GroupedArgs &a, GroupedKind kind, hipStream_t st
 }
 
 template <int D_DT>
-static int grouped_bias(const GroupedArgs &a, int bias_dtype, GroupedKind kind, hipStream_t st) {
-  if (!a.bias) return launch_grouped<D_DT, BIAS_NONE>(a, kind, st);
+static int grouped_bias(const GroupedArgs &a, int bias_dtype, GroupedKind kind, uint32_t *scales, hipStream_t st) {
+  if (!a.bias) return launch_grouped<D_DT, BIAS_NONE>(a, kind, scales, st);
   switch (bias_dtype) {
-    case AC4K_DTYPE_BF16: return launch_grouped<D_DT, AC4K_DTYPE_BF16>(a, kind, st);
-    case AC4K_DTYPE_FP16: return launch_grouped<D_DT, AC4K_DTYPE_FP16>(a, kind, st);
-    case AC4K_DTYPE_FP32: return launch_grouped<D_DT, AC4K_DTYPE_FP32>(a, kind, st);
+    case AC4K_DTYPE_BF16: return launch_grouped<D_DT, AC4K_DTYPE_BF16>(a, kind, scales, st);
+    case AC4K_DTYPE_FP16: return launch_grouped<D_DT, AC4K_DTYPE_FP16>(a, kind, scales, st);
+    case AC4K_DTYPE_FP32: return launch_grouped<D_DT, AC4K_DTYPE_FP32>(a, kind, scales, st);
   }
   return set_error("bias must be bfloat16, half or float (dtype tag %d)", bias_dtype);
 }
@@ -324,17 +332,12 @@ extern "C" __attribute__((visibility("default"))) int ac4k_linear_grouped_nvfp4(
   AC4K_REQUIRE(d_dtype == AC4K_DTYPE_BF16 || d_dtype == AC4K_DTYPE_FP16 || d_dtype == AC4K_DTYPE_FP32, "d must be bfloat16, half or float (dtype tag %d)", d_dtype);
   AC4K_REQUIRE(!bias || bias_dtype == AC4K_DTYPE_BF16 || bias_dtype == AC4K_DTYPE_FP16 || bias_dtype == AC4K_DTYPE_FP32,
                "bias must be bfloat16, half or float (dtype tag %d)", bias_dtype);
-  if (need > 0) {
-    hipLaunchKernelGGL(gather_scales_kernel, dim3((unsigned)ceil_div(align_up(M, 16), 256), (unsigned)(K / 64)), dim3(256), 0, st,
-                       static_cast<uint32_t *>(workspace), a.A_sf, rows, M, align_up(M, 16), T, a.Tp);
-    a.A_sf = static_cast<const uint32_t *>(workspace);
-    a.Tp = align_up(M, 16);
-  }
+  AC4K_REQUIRE(kind == GROUPED_ROWS16 || grouped_tiles(M, N, E, kind) < (1ll << 24), "problem too large");  // 2^32 threads a launch
   int rc;
   switch (d_dtype) {
-    case AC4K_DTYPE_BF16: rc = grouped_bias<AC4K_DTYPE_BF16>(a, bias_dtype, kind, st); break;
-    case AC4K_DTYPE_FP16: rc = grouped_bias<AC4K_DTYPE_FP16>(a, bias_dtype, kind, st); break;
-    case AC4K_DTYPE_FP32: rc = grouped_bias<AC4K_DTYPE_FP32>(a, bias_dtype, kind, st); break;
+    case AC4K_DTYPE_BF16: rc = grouped_bias<AC4K_DTYPE_BF16>(a, bias_dtype, kind, static_cast<uint32_t *>(workspace), st); break;
+    case AC4K_DTYPE_FP16: rc = grouped_bias<AC4K_DTYPE_FP16>(a, bias_dtype, kind, static_cast<uint32_t *>(workspace), st); break;
+    case AC4K_DTYPE_FP32: rc = grouped_bias<AC4K_DTYPE_FP32>(a, bias_dtype, kind, static_cast<uint32_t *>(workspace), st); break;
     default: return set_error("d must be bfloat16, half or float (dtype tag %d)", d_dtype);
   }
   if (rc) return rc;

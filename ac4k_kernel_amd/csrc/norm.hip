@@ -35,7 +35,7 @@ struct NormArgs {
   float *maxima;          // max|y| of each workgroup, likewise
   int64_t rows, K, Kp, Rp;
   int64_t x_stride, residual_stride, sum_stride, out_stride;  // elements between rows
-  double eps;
+  double eps, inverse_K;
   int maxima_count;
 };
 
@@ -113,7 +113,7 @@ __global__ __launch_bounds__(64 * BW) void rms_norm_kernel(NormArgs a, int rows_
     if (tid < 128) lut[tid] = rcp;
     __syncthreads();
     const float g = *a.gs;
-    alpha = __builtin_fabsf(g) < NORM_LEAST / 4096.0f ? 0.0f : 1.0f / g;
+    alpha = g < NORM_LEAST / 4096.0f ? 0.0f : 1.0f / g;  // (a negative scale, too: codes of the table below are those of positive ones)
   }
   auto block_max = [&](uint32_t m) {  // of every wave's m (uniform in a wave)
     if ((tid & 63) == 0) part_max[wave] = m;
@@ -199,7 +199,7 @@ __global__ __launch_bounds__(64 * BW) void rms_norm_kernel(NormArgs a, int rows_
 #pragma unroll
         for (int i = 0; i < WPR; ++i) s += part[group * WPR + i];
       }
-      r = norm_factor(s / (double)a.K + a.eps);
+      r = norm_factor(s * a.inverse_K + a.eps);
     } else {
       r = valid ? a.factors[row] : 0.0f;
       if (it == 0) {  // (the loads of the first row are under way)
@@ -613,6 +613,7 @@ extern "C" __attribute__((visibility("default"))) int ac4k_rms_norm(
   a.Kp = precision == AC4K_PRECISION_NVFP4 ? align_up(K, 64) : align_up(K, 16);
   a.x_stride = x_stride, a.residual_stride = residual_stride, a.sum_stride = sum_stride, a.out_stride = out_stride;
   a.eps = eps;
+  a.inverse_K = 1.0 / (double)K;
   hipStream_t st = (hipStream_t)stream;
   int rc;
   auto go = [&](auto kernels) { rc = kernels(a, precision, find, static_cast<float *>(workspace), dtype, st); };

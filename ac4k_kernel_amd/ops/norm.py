@@ -20,7 +20,7 @@ def rms_norm(x, weight=None, eps=1e-6, residual=None, residual_out=None, precisi
     leading dims in order:
       "nvfp4"           (output [rows, align_up(K,64)/2] u8, sf [align_up(K,64)/64, align_up(rows,16), 4] e4m3, global_scale)
       "fp8e4m3"/"int8"  (output [rows, align_up(K,16)], sf [align_up(rows,16)] fp32)
-    A 0-dim fp32 global_scale that is passed in is used as it is and saves finding the maximum over all rows.
+    A positive 0-dim fp32 global_scale that is passed in is used as it is and saves finding the maximum over all rows.
     Rows whose largest |y| is under 2^-100 (nvfp4: tensors) give zero codes and zero scales.
     With a residual, h is returned behind the rest; residual_out says where to (default a new tensor; x or residual themselves
     are allowed).
@@ -79,5 +79,7 @@ def dequantize(output, sf, global_scale=None, dtype=torch.bfloat16, cols=None, o
     if out is None:
         width = output.shape[-1] * (2 if output.dtype == torch.uint8 else 1)
         out = output.new_empty((*output.shape[:-1], width if cols is None else cols), dtype=dtype)
+    elif _rocm_ops._may_overlap(out, output) or _rocm_ops._may_overlap(out, sf):
+        raise RuntimeError("out must not overlap the quantized operands")
     _rocm_ops.dequantize(out, output, sf, global_scale)
     return out

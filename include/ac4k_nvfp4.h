@@ -328,7 +328,7 @@ enum { AC4K_PRECISION_NONE = 0, AC4K_PRECISION_FP8 = 1, AC4K_PRECISION_INT8 = 2,
  *   NVFP4: out [rows, align_up(K,64)/2], sf [align_up(K,64)/64, align_up(rows,16), 4]; *global_scale is read where given_scale != 0, otherwise
  *   written: max|y| / 2688 over all rows.
  * Every byte of out and sf is written, zeros in the padding.  A row (nvfp4: a tensor) whose max|y| is under 2^-100 gives zero codes and
- * scales, and so does a given scale under 2^-112.  K <= AC4K_NORM_MAX_COLS.  `workspace`: ac4k_rms_norm_workspace_bytes, on 4 bytes, contents irrelevant, NULL when that is 0
+ * scales, and so does a given scale under 2^-112 or a negative one.  K <= AC4K_NORM_MAX_COLS.  `workspace`: ac4k_rms_norm_workspace_bytes, on 4 bytes, contents irrelevant, NULL when that is 0
  * (it is for everything but nvfp4 whose scale is to be found). */
 int64_t ac4k_rms_norm_workspace_bytes(int64_t rows, int64_t K, int dtype, int precision, int given_scale);
 int ac4k_rms_norm(void *out, int64_t out_stride, void *sf, float *global_scale, int given_scale, const void *x, int64_t x_stride,

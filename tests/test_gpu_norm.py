@@ -148,6 +148,15 @@ def test_given_global_scale(rows, k):
         assert got[2].item() == g.item()
 
 
+def test_a_scale_that_is_no_scale():
+    """Negative: zero codes and scales; NaN: NaN everywhere."""
+    x = data((5, 200), torch.bfloat16, 1).cuda()
+    q, sf, _ = ops().rms_norm(x, precision="nvfp4", global_scale=torch.tensor(-0.01, device="cuda"))
+    assert (sf.float() == 0).all() and ((q & 0x77) == 0).all()
+    q = ops().rms_norm(x, precision="nvfp4", global_scale=torch.tensor(math.nan, device="cuda"))
+    assert torch.isnan(ops().dequantize(*q)).all()
+
+
 def test_found_scale_given_back_gives_the_same():
     x, w = data((300, 1000), torch.bfloat16, 1).cuda(), data((1000,), torch.bfloat16, 2).cuda()
     a = ops().rms_norm(x, w, precision="nvfp4")

@@ -182,7 +182,8 @@ def test_norm_operands():
 def test_dequantize_operands():
     q, sf, gs = ops().quantize(torch.ones((4, 64), dtype=torch.bfloat16, device="cuda"), 0, 1)
     for args, kw in (((q, sf), {}), ((q, sf[:, :8], gs), {}), ((q[:3], sf.float(), gs), {}), ((q, sf, gs.reshape(1)), {}), ((q, sf, gs), dict(cols=65)),
-                     ((q, sf, gs), dict(dtype=torch.int8)), ((q.int(), sf, gs), {}), ((q[:, :31], sf, gs), {})):
+                     ((q, sf, gs), dict(dtype=torch.int8)), ((q.int(), sf, gs), {}), ((q[:, :31], sf, gs), {}),
+                     ((q, sf, gs), dict(out=q.view(torch.bfloat16)))):
         with pytest.raises(RuntimeError):
             ops().dequantize(*args, **kw)
 
@@ -197,7 +198,7 @@ def test_rope_operands():
                      ((x, t), dict(positions=pos, grid=(4,))), ((x, t), dict(grid=(9,))), ((x, t), dict(grid=(2, 2))), ((x, t), dict(sections=(31,))),
                      ((x, t.half()), {}), ((x[..., :62], t), {}), (((x, x.half()), t), {}), (((x, x[:, :3]), t), {}), (((x, x, x), t), {}),
                      ((x, t), dict(out=x[:1])), ((a, t), dict(out=b)), (((a, a), t), dict(out=(a, a))), (((a, x), t), dict(out=(x, a))),
-                     ((x, t), dict(positions=pos.cpu()))):
+                     ((x, t), dict(positions=pos.cpu())), ((x[:, :, :1].expand(2, 4, 3, 64), t), dict(out=x[:, :, :1].expand(2, 4, 3, 64)))):
         with pytest.raises(RuntimeError):
             ops().rope(*args, **kw)
 
