@@ -599,18 +599,21 @@ def rms_norm(out, sf, global_scale, given_scale: bool, x, weight, residual, resi
                                 _stream()))
 
 
-def dequantize(out, q, sf, global_scale=None) -> None:
-    """out [.., R, cols] <- the values of q, sf (and global_scale, for nvfp4) as `quantize` returns them without swizzle."""
-    tag = _check_float(out, "out")
+def dequantize(out, q, sf, global_scale=None, dtype=None, cols=None):
+    """out [.., R, cols] (None: a new tensor of dtype) <- the values of q, sf (and global_scale, for nvfp4) as `quantize` returns them
+    without swizzle; returns out."""
     if not isinstance(q, torch.Tensor) or q.dim() < 2:
         _check(False, "q must have at least two dims")
-    nvfp4 = q.dtype is torch.uint8
-    number = 3 if nvfp4 else _EIGHT_BITS.get(q.dtype)
+    kind = q.dtype
+    nvfp4 = kind is torch.uint8
+    number = 3 if nvfp4 else _EIGHT_BITS.get(kind)
     if number is None:
         _check(False, "q must be uint8 (nvfp4), float8_e4m3fn or int8")
-    _check_tensor(q, q.dtype, "q")
+    _check_tensor(q, kind, "q")
     _check_tensor(sf, torch.float8_e4m3fn if nvfp4 else torch.float32, "sf")
-    _same_device(q, out, sf, global_scale)
+    dev = _current_device()
+    if q.get_device() != dev or sf.get_device() != dev:
+        _same_device(q, sf)
     *lead, R, W = q.shape
     planes, gs_step, gs_ptr = 1, 0, None
     for n in lead:
@@ -621,6 +624,8 @@ def dequantize(out, q, sf, global_scale=None) -> None:
             _check(W % 64 == 0, "rows of q must be whole pieces of 64 elements")
             _check(False, "meet invalid sf shape")
         _check_tensor(global_scale, torch.float32, "global_scale")
+        if global_scale.get_device() != dev:
+            _same_device(global_scale)
         if global_scale.dim() != 0:
             _check(list(global_scale.shape) == lead, "global_scale must be a scalar or have the leading dims of q")
             gs_step = 1
@@ -629,13 +634,24 @@ def dequantize(out, q, sf, global_scale=None) -> None:
         if W % 16 != 0 or sf.shape != (*lead, (R + 15) // 16 * 16):
             _check(W % 16 == 0, "rows of q must be whole pieces of 16 elements")
             _check(False, "meet invalid sf shape")
-        _check(global_scale is None, "only nvfp4 has a global scale")
-    *out_lead, cols = out.shape
-    if not out.is_contiguous() or out_lead != [*lead, R] or cols > W:
-        _check(False, "out must be contiguous of [.., {}, up to {}]", R, W)
-    if out.numel() == 0:
-        return
-    _lib.check(_L.ac4k_dequantize(out.data_ptr(), tag, q.data_ptr(), sf.data_ptr(), gs_ptr, gs_step, planes, R, W, cols, number, _stream()))
+        if global_scale is not None:
+            _check(False, "only nvfp4 has a global scale")
+    if out is None:
+        cols = W if cols is None else cols
+        tag = _DTYPE_TAG.get(dtype)
+        if tag is None or not 0 <= cols <= W:
+            _check(tag is not None, "out must be bfloat16, half or float")
+            _check(False, "out must be contiguous of [.., {}, up to {}]", R, W)
+        out = q.new_empty((*lead, R, cols), dtype=dtype)
+    else:
+        tag = _check_float(out, "out")
+        _same_device(out)
+        *out_lead, cols = out.shape
+        _check(out.is_contiguous() and out_lead == [*lead, R] and cols <= W, "out must be contiguous of [.., {}, up to {}]", R, W)
+        _check(not _may_overlap(out, q) and not _may_overlap(out, sf), "out must not overlap the quantized operands")
+    if planes and R and cols:
+        _lib.check(_L.ac4k_dequantize(out.data_ptr(), tag, q.data_ptr(), sf.data_ptr(), gs_ptr, gs_step, planes, R, W, cols, number, _stream()))
+    return out
 
 
 _ROPE_SECTIONS = {}
@@ -656,52 +672,61 @@ _RopePair = _lib.RopeTensor * 2
 _POSITIONS = {torch.int32, torch.int64}
 
 
-def rope(outs, xs, table, sections, positions, grid, bnhd: bool, interleaved: bool, inverse: bool, fresh: bool = False) -> None:
-    """outs <- xs (one or two tensors) turned by the angles of their tokens' positions.  fresh: outs are new dense tensors."""
+def rope(outs, xs, table, sections, positions, grid, bnhd: bool, interleaved: bool, inverse: bool):
+    """outs (None: new dense tensors) <- xs, one or two tensors, turned by the angles of their tokens' positions; returns outs."""
     count = len(xs)
-    if count not in (1, 2) or len(outs) != count:
+    if count > 2 or count < 1 or (outs is not None and len(outs) != count):
         _check(False, "rope takes one or two tensors, and as many outputs")
     x = xs[0]
     tag = _check_float(x, "x")
+    dev = _current_device()
     _check_tensor(table, torch.float32, "table")
-    if x.dim() != 4 or table.dim() != 3 or table.shape[2] != 2:
-        _check(x.dim() == 4, "x must be a 4D tensor")
-        _check(False, "table must be [length, pairs, 2]")
-    (B, N, _, D), (length, pairs, _) = x.shape, table.shape
+    if x.dim() != 4 or table.dim() != 3:
+        _check(False, "x must be a 4D tensor, table [length, pairs, 2]")
+    B, N, N2, D = x.shape
+    length, pairs, two = table.shape
     if not bnhd:
-        N = x.shape[2]
-    if length < 1 or pairs < 1 or 2 * pairs > D:
-        _check(length >= 1 and pairs >= 1, "table must be [length, pairs, 2]")
+        N = N2
+    if two != 2 or length < 1 or pairs < 1 or 2 * pairs > D:
+        _check(two == 2 and length >= 1 and pairs >= 1, "table must be [length, pairs, 2]")
         _check(False, "{} pairs do not fit a head of {}", pairs, D)
     section_arg, axes = _rope_sections(sections, pairs), len(sections)
-    _same_device(*xs, table, positions)
+    if x.get_device() != dev or table.get_device() != dev:
+        _same_device(x, table)
     args, used = _RopePair(), 0
-    for t, o in zip(xs, outs):
-        if t is not x:
-            _check(_check_float(t, "x") == tag, "all tensors must have one type")
-            _check(t.dim() == 4 and t.shape[0] == B and t.shape[1 if bnhd else 2] == N and t.shape[3] == D,
-                   "all tensors must have the same batch, tokens and head dim")
+    made = []
+    for i, t in enumerate(xs):
+        if i:
+            if t.get_device() != dev or t.dtype is not x.dtype or t.dim() != 4 or t.shape[0] != B or t.shape[1 if bnhd else 2] != N or t.shape[3] != D:
+                _same_device(t)
+                _check(_check_float(t, "x") == tag, "all tensors must have one type")
+                _check(False, "all tensors must have the same batch, tokens and head dim")
         t_b, t_n, t_h, t_d = t.stride()
-        o_b, o_n, o_h, o_d = o.stride()
-        if not fresh:
+        if t_d != 1:
+            _check(False, "heads must be contiguous")
+        if outs is None:
+            o = torch.empty_like(t, memory_format=torch.contiguous_format)
+            made.append(o)
+        else:
+            o = outs[i]
             _same_device(o)
             _check(_check_float(o, "out") == tag, "all tensors must have one type")
             _check(o.shape == t.shape, "out must have the shape of x")
-            _check(o_d == 1 and _places_of_their_own(o), "heads of out must be contiguous, and apart from each other")
+            _check(o.stride(3) == 1 and _places_of_their_own(o), "heads of out must be contiguous, and apart from each other")
             _check(_same_rows(t, o) or not _may_overlap(t, o), "out may be x itself, but not overlap it otherwise")
-        if t_d != 1:
-            _check(False, "heads must be contiguous")
         if t.numel() == 0:
             continue
+        o_b, o_n, o_h, _ = o.stride()
         args[used] = ((t.data_ptr(), o.data_ptr(), t_b, t_n, t_h, o_b, o_n, o_h, t.shape[2]) if bnhd else
                       (t.data_ptr(), o.data_ptr(), t_b, t_h, t_n, o_b, o_h, o_n, t.shape[1]))
         used += 1
-    if count == 2 and not fresh:
+    if count == 2 and outs is not None:
         _check(not any(_may_overlap(o, t) for o, t in ((outs[0], xs[1]), (outs[1], xs[0]), (outs[0], outs[1])) if o.numel() and t.numel())
                or _interleaved_heads(outs, xs), "the two tensors must not overlap each other")
     pos_ptr, pos_bytes, pos_strides, grid_arg = None, 0, (0, 0, 0), None
     if positions is not None:
-        if grid is not None or positions.dtype not in _POSITIONS or positions.shape != (axes, B, N):
+        if grid is not None or positions.dtype not in _POSITIONS or positions.shape != (axes, B, N) or positions.get_device() != dev:
+            _same_device(positions)
             _check(grid is None, "positions or a grid, one of them")
             _check(positions.is_cuda and positions.dtype in _POSITIONS, "positions must be a CUDA tensor of int32 or int64")
             _check(False, "positions must be [{}, {}, {}]", axes, B, N)
@@ -710,10 +735,10 @@ def rope(outs, xs, table, sections, positions, grid, bnhd: bool, interleaved: bo
         _check(grid is not None and len(grid) == axes and min(grid) >= 1, "grid must have one size of at least 1 for each axis")
         _check(max(grid) <= length, "the table has {} positions, the grid {}", length, max(grid))
         grid_arg = (_lib._i64 * axes)(*grid)
-    if used == 0:
-        return
-    _lib.check(_L.ac4k_rope(args, used, tag, B, N, D, table.data_ptr(), length, pairs, section_arg, axes, pos_ptr, pos_bytes, *pos_strides,
-                            grid_arg, interleaved, inverse, _stream()))
+    if used:
+        _lib.check(_L.ac4k_rope(args, used, tag, B, N, D, table.data_ptr(), length, pairs, section_arg, axes, pos_ptr, pos_bytes, *pos_strides,
+                                grid_arg, interleaved, inverse, _stream()))
+    return outs or tuple(made)
 
 
 def _interleaved_heads(outs, xs) -> bool:

@@ -144,13 +144,13 @@ template <int BM>
 __device__ __forceinline__ int group_tiles(const Group &g) {
   return g.count == 0 ? 0 : ((g.first & 3) + g.count + BM - 1) / BM;
 }
-__device__ __forceinline__ int wave_prefix(int v) {  // inclusive
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const int o = __shfl_up(v, d, 64);
-    v += lane >= d ? o : 0;
-  }
+__device__ __forceinline__ int wave_prefix(int v) {  // inclusive: inside rows of 16 lanes, then the last lane of a row to those behind it
+  v += (int)dpp_u32<DPP_ROW_SHR(1)>((uint32_t)v);
+  v += (int)dpp_u32<DPP_ROW_SHR(2)>((uint32_t)v);
+  v += (int)dpp_u32<DPP_ROW_SHR(4)>((uint32_t)v);
+  v += (int)dpp_u32<DPP_ROW_SHR(8)>((uint32_t)v);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15 to rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31 to rows 2 and 3
   return v;
 }
 

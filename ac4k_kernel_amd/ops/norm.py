@@ -76,10 +76,4 @@ def dequantize(output, sf, global_scale=None, dtype=torch.bfloat16, cols=None, o
     one per leading plane.  Returns [.., R, cols] of dtype (bf16, fp16 or fp32), cols up to the padded width W, the
     default.  Each value is the product in fp32, rounded to dtype once.
     """
-    if out is None:
-        width = output.shape[-1] * (2 if output.dtype == torch.uint8 else 1)
-        out = output.new_empty((*output.shape[:-1], width if cols is None else cols), dtype=dtype)
-    elif _rocm_ops._may_overlap(out, output) or _rocm_ops._may_overlap(out, sf):
-        raise RuntimeError("out must not overlap the quantized operands")
-    _rocm_ops.dequantize(out, output, sf, global_scale)
-    return out
+    return _rocm_ops.dequantize(out, output, sf, global_scale, dtype, cols)

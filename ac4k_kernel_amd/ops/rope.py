@@ -41,10 +41,11 @@ def rope(x, table, positions=None, grid=None, sections=None, layout="BNHD", inte
     for t in xs:
         if not isinstance(t, torch.Tensor) or t.dim() != 4:
             raise RuntimeError("rope takes one or two 4D tensors")
+        if t.stride(3) != 1:
+            xs = tuple([u.contiguous() if u.stride(3) != 1 else u for u in xs])
     if not xs or not isinstance(table, torch.Tensor) or table.dim() != 3:
         raise RuntimeError("rope takes one or two 4D tensors and a table of [length, pairs, 2]")
-    fresh = out is None
-    outs = tuple([torch.empty_like(t, memory_format=torch.contiguous_format) for t in xs]) if fresh else (out,) if single else tuple(out)
+    outs = None if out is None else (out,) if single else tuple(out)
     sections = (table.shape[1],) if sections is None else (sections,) if isinstance(sections, int) else tuple(sections)
     bnhd = layout == "BNHD"
     if positions is None:
@@ -61,9 +62,5 @@ def rope(x, table, positions=None, grid=None, sections=None, layout="BNHD", inte
             positions = positions.expand(-1, xs[0].shape[0], -1)
     else:
         raise RuntimeError("positions must be a CUDA tensor of int32 or int64")
-    for t in xs:
-        if t.stride(3) != 1:
-            xs = tuple([t.contiguous() if t.stride(3) != 1 else t for t in xs])
-            break
-    _rocm_ops.rope(outs, xs, table, sections, positions, grid, bnhd, interleaved, inverse, fresh)
+    outs = _rocm_ops.rope(outs, xs, table, sections, positions, grid, bnhd, interleaved, inverse)
     return outs[0] if single else outs
