@@ -127,7 +127,7 @@ __global__ __launch_bounds__(64 * BW) void rms_norm_kernel(NormArgs a, int rows_
   auto global_scale = [&](uint32_t bits) {
     float m = __uint_as_float(bits);
     if (m < NORM_LEAST) m = 0.0f;
-    const float g = m / 2688.0f;
+    const float g = m * (1.0f / 2688.0f);
     alpha = g == 0.0f ? 0.0f : 1.0f / g;
     if (blockIdx.x == 0 && tid == 0) *a.gs = g;
   };
@@ -288,8 +288,8 @@ __global__ __launch_bounds__(64 * BW) void rms_norm_kernel(NormArgs a, int rows_
         float amax = __uint_as_float(m);
         if (amax < NORM_LEAST) amax = 0.0f;
         const float most = OUT == NORM_FP8 ? 448.0f : 127.0f;
-        if (sub == 0) static_cast<float *>(a.sf)[row] = amax / most;
-        const float factor = amax == 0.0f ? 0.0f : most / amax;
+        if (sub == 0) static_cast<float *>(a.sf)[row] = amax * (1.0f / most);
+        const float factor = amax == 0.0f ? 0.0f : 1.0f / amax * most;  // one division a row; with the scale's product two roundings each
         uint8_t *op = static_cast<uint8_t *>(a.out) + row * a.Kp;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
@@ -302,7 +302,7 @@ __global__ __launch_bounds__(64 * BW) void rms_norm_kernel(NormArgs a, int rows_
           } else {
             values(j, y);
           }
-          // |y * factor| is at most `most` and a rounding, which rounds back to it: nothing to clamp
+          // |y * factor| is at most `most` and three roundings, which the conversion rounds back to it: nothing to clamp
           uint32_t lo, hi;
           if constexpr (OUT == NORM_FP8) {
             lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[0] * factor, y[1] * factor, 0, false);

@@ -54,7 +54,7 @@ def quantized(y, precision, gs=None):
         m = blk.abs().amax(-1)
         if gs is None:
             amax = m.amax()
-            gs = (torch.where(amax < 2.0 ** -100, 0.0, amax) / torch.tensor(2688.0)).float()
+            gs = torch.where(amax < 2.0 ** -100, 0.0, amax) * (torch.tensor(1.0) / torch.tensor(2688.0))
         alpha = torch.where(gs.abs() < 2.0 ** -112, 0.0, 1.0 / gs)
         bits = T.f32_to_e4m3_bits(alpha * (m * T.ONE_SIXTH_F32))
         s = T.e4m3_bits_to_f32(bits)
@@ -66,10 +66,10 @@ def quantized(y, precision, gs=None):
     most = 448.0 if precision == "fp8e4m3" else 127.0
     m = y.abs().amax(-1)
     m = torch.where(m < 2.0 ** -100, 0.0, m)
-    factor = torch.where(m == 0, 0.0, torch.tensor(most) / m)
+    factor = torch.where(m == 0, 0.0, (torch.tensor(1.0) / m) * most)
     q = torch.nn.functional.pad(y * factor[:, None], (0, -k % 16))
     q = T.f32_to_e4m3_bits(q) if precision == "fp8e4m3" else T.f32_to_s8_sat(q)
-    return q, torch.nn.functional.pad(m / most, (0, rp - rows)), None
+    return q, torch.nn.functional.pad(m * (torch.tensor(1.0) / torch.tensor(most)), (0, rp - rows)), None
 
 
 def same(a, b):
