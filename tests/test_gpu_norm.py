@@ -252,6 +252,21 @@ def test_large_values_do_not_overflow():
     check_plain(ops().rms_norm(x.cuda(), eps=0.0), reference(x, None, eps=0.0)[1])
 
 
+@pytest.mark.parametrize("precision", ["nvfp4", "fp8e4m3", "int8"])
+@pytest.mark.parametrize("rows,k", [(3, 64), (40, 300), (5000, 64)])
+def test_largest_rows_quantized(rows, k, precision):
+    """Maxima near the largest number of the type, whose reciprocal is a subnormal one: the codes still reach the end of their range."""
+    x, w = data((rows, k), torch.float32, 1), torch.full((k,), 1e37)
+    x[1] = 0
+    x[1, 5] = -1.0  # all of a row in one place: sqrt(k) times the weight, 1.7e38 at k = 300
+    _, _, y32 = reference(x, w)
+    assert y32.abs().max() > 2.0 ** 125 and torch.isfinite(y32).all()
+    got = ops().rms_norm(x.cuda(), w.cuda(), eps=EPS, precision=precision)
+    check_quantized(got, y32, precision)
+    top = got[0][1].view(torch.uint8).cpu()
+    assert (top != 0).any() and torch.isfinite(got[1].float()).all()
+
+
 def test_empty():
     x, w = torch.empty((0, 64), dtype=torch.bfloat16, device="cuda"), torch.ones(64, dtype=torch.bfloat16, device="cuda")
     assert ops().rms_norm(x, w).shape == (0, 64)
