@@ -215,7 +215,9 @@ __global__ __launch_bounds__(256) void gather_scales_kernel(uint32_t *out, const
   out[chunk * Mp + i] = i < M ? sf[chunk * Tp + row] : 0u;
 }
 
-enum GroupedKind { GROUPED_ROWS16, GROUPED_64_128, GROUPED_64_256, GROUPED_256_256 };
+enum GroupedKind { GROUPED_NONE = 0, GROUPED_ROWS16 = 1, GROUPED_64_128 = 2, GROUPED_64_256 = 3, GROUPED_256_256 = 4 };
+// which kernel the last call of this host thread launched (introspection for tests)
+static thread_local int g_last_grouped_kernel = GROUPED_NONE;
 
 // (the tile kernel's 32-bit lane offsets: whole of x where rows are gathered, the rows of a tile and of a band otherwise)
 static bool grouped_tiles_fit(int64_t T, int64_t N, int64_t K, bool gather) {
@@ -280,7 +282,7 @@ static int launch_grouped(const GroupedArgs &a, GroupedKind kind, uint32_t *scal
     case GROUPED_256_256: return launch_grouped_tile<D_DT, BIAS_DT, 4, 4, 1, 3, 1>(a, kind, scales, st);
     case GROUPED_64_256: return launch_grouped_tile<D_DT, BIAS_DT, 1, 4, 2, 3, 2>(a, kind, scales, st);
     case GROUPED_64_128: return launch_grouped_tile<D_DT, BIAS_DT, 1, 2, 2, 5, 2>(a, kind, scales, st);
-    case GROUPED_ROWS16: break;
+    default: break;  // GROUPED_ROWS16
   }
   const dim3 grid((unsigned)ceil_div(a.N, R16_ROWS), (unsigned)a.E);
   if (a.M <= 16 * a.E) hipLaunchKernelGGL((linear_grouped_rows16_kernel<D_DT, BIAS_DT, 1>), grid, dim3(64 * R16_WAVES), 0, st, a);
@@ -341,5 +343,8 @@ extern "C" __attribute__((visibility("default"))) int ac4k_linear_grouped_nvfp4(
     default: return set_error("d must be bfloat16, half or float (dtype tag %d)", d_dtype);
   }
   if (rc) return rc;
+  g_last_grouped_kernel = kind;
   return check_launch("ac4k_linear_grouped_nvfp4");
 }
+
+extern "C" __attribute__((visibility("default"))) int ac4k_debug_last_grouped_kernel(void) { return ac4k::g_last_grouped_kernel; }

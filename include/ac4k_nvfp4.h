@@ -379,6 +379,10 @@ int ac4k_linear_grouped_nvfp4(void *D, int d_dtype, const void *A, const void *A
                               const void *bias, int bias_dtype, const int32_t *offsets, int64_t M, int64_t N, int64_t K,
                               int64_t E, void *workspace, int64_t workspace_bytes, ac4k_stream_t stream);
 
+/* Introspection for tests (no counterpart in the reference): which kernel the calling host thread's last ac4k_linear_grouped_nvfp4 launched: 0 none yet, 1 sixteen
+ * weight rows a workgroup, 2 tiles of 64 x 128, 3 of 64 x 256, 4 of 256 x 256 (behind the launch that gathers scales, where there are `rows`). */
+int ac4k_debug_last_grouped_kernel(void);
+
 #ifdef __cplusplus
 }
 #endif
