@@ -67,11 +67,11 @@ SIGNATURES = {
     "ac4k_dequantize": (_int, [_vp, _int, _vp, _vp, _vp] + [_i64] * 5 + [_int, _vp]),
     "ac4k_rope": (_int, [ctypes.POINTER(RopeTensor), _int, _int, _i64, _i64, _i64, _vp, _i64, _i64, ctypes.POINTER(_i64), _int,
                          _vp, _int, _i64, _i64, _i64, ctypes.POINTER(_i64), _int, _int, _vp]),
-    "ac4k_debug_last_grouped_kernel": (_int, []),
     "ac4k_linear_grouped_nvfp4_workspace_bytes": (_i64, [_i64] * 5 + [_int]),
-    "ac4k_linear_grouped_nvfp4": (_int, [_vp, _int, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _int, _vp] + [_i64] * 4
-                                  + [_vp, _i64, _vp]),
+    "ac4k_debug_last_grouped_kernel": (_int, []),
 }
+for _name in ("ac4k_linear_grouped_nvfp4", "ac4k_linear_grouped_nvfp4_whole"):
+    SIGNATURES[_name] = (_int, [_vp, _int, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _int, _vp] + [_i64] * 4 + [_vp, _i64, _vp])
 
 _lib = None
 

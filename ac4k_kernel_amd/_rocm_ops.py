@@ -773,8 +773,9 @@ def _interleaved_heads(outs, xs) -> bool:
     return True
 
 
-def linear_grouped_nvfp4(D, A, A_sf, A_global_scale, B, B_sf, B_global_scale, offsets, rows=None, bias=None) -> None:
-    """D[i] = linear of row rows[i] (row i without rows) of A on the weight of the expert whose range of offsets holds i."""
+def linear_grouped_nvfp4(D, A, A_sf, A_global_scale, B, B_sf, B_global_scale, offsets, rows=None, bias=None, whole=False) -> None:
+    """D[i] = linear of row rows[i] (row i without rows) of A on the weight of the expert whose range of offsets holds i; rows that no range holds stay
+    as they are, or become zero (whole)."""
     M, N, tag = _check_output(D)
     _check(isinstance(A, torch.Tensor) and A.dim() == 2, "a must be a 2d matrix")
     T = A.size(0)
@@ -803,11 +804,13 @@ def linear_grouped_nvfp4(D, A, A_sf, A_global_scale, B, B_sf, B_global_scale, of
         bias_ptr = bias.data_ptr()
     _same_device(D, A, A_sf, A_global_scale, B, B_sf, B_global_scale, offsets, rows, bias)
     if M == 0 or N == 0 or E == 0:
+        if whole:
+            D.zero_()
         return
     _check(T > 0, "rows of an empty a")
     nbytes = _L.ac4k_linear_grouped_nvfp4_workspace_bytes(T, M, N, K, E, int(rows is not None))
     ws = D.new_empty((nbytes,), dtype=torch.uint8) if nbytes > 0 else None
-    _lib.check(_L.ac4k_linear_grouped_nvfp4(D.data_ptr(), tag, A.data_ptr(), A_sf.data_ptr(), A_global_scale.data_ptr(), T,
-                                            None if rows is None else rows.data_ptr(), B.data_ptr(), B_sf.data_ptr(),
-                                            B_global_scale.data_ptr(), int(B_global_scale.dim() > 0), bias_ptr, bias_tag,
-                                            offsets.data_ptr(), M, N, K, E, None if ws is None else ws.data_ptr(), nbytes, _stream()))
+    call = _L.ac4k_linear_grouped_nvfp4_whole if whole else _L.ac4k_linear_grouped_nvfp4
+    _lib.check(call(D.data_ptr(), tag, A.data_ptr(), A_sf.data_ptr(), A_global_scale.data_ptr(), T, None if rows is None else rows.data_ptr(),
+                    B.data_ptr(), B_sf.data_ptr(), B_global_scale.data_ptr(), int(B_global_scale.dim() > 0), bias_ptr, bias_tag, offsets.data_ptr(),
+                    M, N, K, E, None if ws is None else ws.data_ptr(), nbytes, _stream()))

@@ -5,7 +5,8 @@
 //
 // The sizes of the groups are on the GPU and nothing waits for them: launches are made for the largest number of tiles that the row and
 // expert counts allow, and workgroups without a tile end at once.  Offsets are taken as clamped to [0, rows] and rising, row indexes as
-// clamped to x: a wrong table gives wrong rows, not an access outside of the operands.  Output rows that no group holds stay as they are.
+// clamped to x: a wrong table gives wrong rows, not an access outside of the operands.  Output rows that no group holds stay as they are, or
+// become zero where the caller's output is new memory.
 //
 // Few rows an expert are bound by the weights' bytes, many by the matrix cores.  128 rows on 64 experts of 2048 x 4096 61-65 us (55 of bytes at the rate of a
 // copy; 440 tiles on 256 CUs leave some a tile less), 16384 rows on 8 experts of 14336 x 4096 1396-1450 us, 1.33-1.38 PFLOP/s, matrix cores busy for 82 % of the
@@ -30,6 +31,7 @@ struct GroupedArgs {
   const void *bias;        // [E, N]
   const int32_t *offsets;  // [E + 1]
   int64_t T, Tp, M, N, Np, K, E;
+  bool whole;              // rows of D in front of the first range and behind the last one become zero
 };
 
 struct Group {
@@ -40,6 +42,29 @@ __device__ __forceinline__ Group group_of(const int32_t *offsets, int64_t e, int
   const int first = lo < 0 ? 0 : lo > (int)M ? (int)M : lo;
   const int end = hi > (int)M ? (int)M : hi;
   return {first, end > first ? end - first : 0};
+}
+
+// The rows of D that no range holds, in front of `first` and from `last` on, by all workgroups of the launch in equal shares, before their own work.  (A clearing launch in front would write all of D a second time: half a gigabyte of the 1.4 ms of 16384 x 14336.)
+template <int D_DT>
+__device__ __forceinline__ void zero_other_rows(const GroupedArgs &a, int64_t first, int64_t last) {
+  using T = typename Elem<D_DT>::T;
+  constexpr int V = 16 / sizeof(T);
+  if (last < first) last = first;
+  if (first == 0 && last == a.M) return;
+  const int64_t at = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * blockDim.x + threadIdx.x, step = (int64_t)gridDim.x * gridDim.y * blockDim.x;
+  auto zero = [&](int64_t row, int64_t rows) {
+    T *p = static_cast<T *>(a.D) + row * a.N;
+    const int64_t n = rows * a.N;
+    for (int64_t i = at * V; i < n; i += step * V) {
+      if (i + V <= n) {
+        *reinterpret_cast<u32x4_elem *>(p + i) = (u32x4){0, 0, 0, 0};
+      } else {
+        for (int64_t k = i; k < n; ++k) p[k] = T(0);
+      }
+    }
+  };
+  zero(0, first);
+  zero(last, a.M - last);
 }
 
 // ===========================================================================
@@ -54,6 +79,10 @@ template <int D_DT, int BIAS_DT, int MT>
 __global__ __launch_bounds__(64 * R16_WAVES, 2) void linear_grouped_rows16_kernel(GroupedArgs a) {
   __shared__ float4 part[R16_WAVES][MT][64];
   const Group grp = group_of(a.offsets, blockIdx.y, a.M);
+  if (a.whole) {
+    const Group end = group_of(a.offsets, a.E - 1, a.M);
+    zero_other_rows<D_DT>(a, group_of(a.offsets, 0, a.M).first, end.first + end.count);
+  }
   if (grp.count == 0) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
   const int64_t e = blockIdx.y, n0 = (int64_t)blockIdx.x * R16_ROWS, kb = a.K >> 1;
@@ -156,6 +185,7 @@ __device__ __forceinline__ int wave_prefix(int v) {  // inclusive: inside rows o
 
 struct GroupTile {
   int e, first, count, tile, tn;  // tile: index inside the group; e < 0: none
+  int rows_first, rows_last;      // of all groups: first row of the first one, end of the last one
 };
 template <int BM, int BN>
 __device__ __forceinline__ GroupTile tile_of_groups(const GroupedArgs &a) {
@@ -163,16 +193,18 @@ __device__ __forceinline__ GroupTile tile_of_groups(const GroupedArgs &a) {
   const uint32_t tiles_n = (uint32_t)ceil_div(a.N, BN);
   int64_t sum = 0;
   Group grp{0, 0};
-  int incl = 0;
+  int incl = 0, rows_first = 0;
   for (int base = 0; base < E; base += 64) {
     grp = base + lane < E ? group_of(a.offsets, base + lane, a.M) : Group{0, 0};
     incl = wave_prefix(group_tiles<BM>(grp));
     sum += __builtin_amdgcn_readlane(incl, 63);
+    if (base == 0) rows_first = __builtin_amdgcn_readlane(grp.first, 0);
   }
+  const int rows_last = __builtin_amdgcn_readlane(grp.first + grp.count, (E - 1) & 63);
   // (offsets that overlap could name more tiles than the launch has)
   const uint32_t most = gridDim.x / tiles_n;
   const uint32_t total = (uint32_t)__builtin_amdgcn_readfirstlane((int)(sum < most ? sum : most));
-  if (blockIdx.x >= total * tiles_n) return {-1, 0, 0, 0, 0};
+  if (blockIdx.x >= total * tiles_n) return {-1, 0, 0, 0, 0, rows_first, rows_last};
   const TileCoord tc = tile_of_workgroup<4>(blockIdx.x, total, tiles_n);
   const int tm = __builtin_amdgcn_readfirstlane((int)tc.m);
   int before = 0, base = 0;
@@ -188,7 +220,7 @@ __device__ __forceinline__ GroupTile tile_of_groups(const GroupedArgs &a) {
   const int l = __builtin_ctzll(__ballot(before + incl > tm));
   const int tiles = __builtin_amdgcn_readlane(group_tiles<BM>(grp), l);
   return {base + l, __builtin_amdgcn_readlane(grp.first, l), __builtin_amdgcn_readlane(grp.count, l), tm - (before + __builtin_amdgcn_readlane(incl, l) - tiles),
-          __builtin_amdgcn_readfirstlane((int)tc.n)};
+          __builtin_amdgcn_readfirstlane((int)tc.n), rows_first, rows_last};
 }
 
 template <int D_DT, int BIAS_DT, int MI, int NJ, int PS, int KW, bool EARLY, int PER_CU>
@@ -196,6 +228,7 @@ __global__ __launch_bounds__(256, PER_CU) void linear_grouped_tile_kernel(Groupe
   extern __shared__ __attribute__((aligned(16))) char plds[];
   constexpr int BM = 64 * MI, BN = 64 * NJ;
   const GroupTile t = tile_of_groups<BM, BN>(a);
+  if (a.whole) zero_other_rows<D_DT>(a, t.rows_first, t.rows_last);
   if (t.e < 0) return;
   const int64_t kb = a.K >> 1, e = t.e;
   LinearArgs la{a.D, a.A, a.B + e * a.N * kb, a.A_sf, a.B_sf + e * (a.K >> 6) * a.Np, a.A_gs, a.B_gs + e * a.B_gs_stride, nullptr,
@@ -311,8 +344,8 @@ extern "C" __attribute__((visibility("default"))) int64_t ac4k_linear_grouped_nv
   return K / 64 * align_up(M, 16) * 4;
 }
 
-extern "C" __attribute__((visibility("default"))) int ac4k_linear_grouped_nvfp4(
-    void *D, int d_dtype, const void *A, const void *A_sf, const float *A_gs, int64_t T, const int32_t *rows, const void *B, const void *B_sf,
+static int grouped_linear(
+    bool whole, void *D, int d_dtype, const void *A, const void *A_sf, const float *A_gs, int64_t T, const int32_t *rows, const void *B, const void *B_sf,
     const float *B_gs, int64_t B_gs_stride, const void *bias, int bias_dtype, const int32_t *offsets, int64_t M, int64_t N, int64_t K, int64_t E,
     void *workspace, int64_t workspace_bytes, ac4k_stream_t stream) {
   AC4K_REQUIRE(D && A && A_sf && A_gs && B && B_sf && B_gs && offsets, "null pointer argument");
@@ -325,7 +358,7 @@ extern "C" __attribute__((visibility("default"))) int ac4k_linear_grouped_nvfp4(
   AC4K_REQUIRE(M < (1ll << 27) && N < (1ll << 27) && T < (1ll << 31) - 16 && K < (1ll << 22) && E <= 65535, "problem too large");
   AC4K_REQUIRE(ceil_div(N, R16_ROWS) * (64 * R16_WAVES) < (1ll << 32), "problem too large");
   GroupedArgs a{D, static_cast<const uint8_t *>(A), static_cast<const uint32_t *>(A_sf), A_gs, rows, static_cast<const uint8_t *>(B),
-                static_cast<const uint32_t *>(B_sf), B_gs, B_gs_stride, bias, offsets, T, align_up(T, 16), M, N, align_up(N, 16), K, E};
+                static_cast<const uint32_t *>(B_sf), B_gs, B_gs_stride, bias, offsets, T, align_up(T, 16), M, N, align_up(N, 16), K, E, whole};
   hipStream_t st = (hipStream_t)stream;
   const GroupedKind kind = grouped_kind(T, M, N, K, E, rows != nullptr);
   const int64_t need = ac4k_linear_grouped_nvfp4_workspace_bytes(T, M, N, K, E, rows != nullptr);
@@ -345,6 +378,22 @@ extern "C" __attribute__((visibility("default"))) int ac4k_linear_grouped_nvfp4(
   if (rc) return rc;
   g_last_grouped_kernel = kind;
   return check_launch("ac4k_linear_grouped_nvfp4");
+}
+
+extern "C" __attribute__((visibility("default"))) int ac4k_linear_grouped_nvfp4(
+    void *D, int d_dtype, const void *A, const void *A_sf, const float *A_gs, int64_t T, const int32_t *rows, const void *B, const void *B_sf,
+    const float *B_gs, int64_t B_gs_stride, const void *bias, int bias_dtype, const int32_t *offsets, int64_t M, int64_t N, int64_t K, int64_t E,
+    void *workspace, int64_t workspace_bytes, ac4k_stream_t stream) {
+  return grouped_linear(false, D, d_dtype, A, A_sf, A_gs, T, rows, B, B_sf, B_gs, B_gs_stride, bias, bias_dtype, offsets, M, N, K, E, workspace,
+                        workspace_bytes, stream);
+}
+
+extern "C" __attribute__((visibility("default"))) int ac4k_linear_grouped_nvfp4_whole(
+    void *D, int d_dtype, const void *A, const void *A_sf, const float *A_gs, int64_t T, const int32_t *rows, const void *B, const void *B_sf,
+    const float *B_gs, int64_t B_gs_stride, const void *bias, int bias_dtype, const int32_t *offsets, int64_t M, int64_t N, int64_t K, int64_t E,
+    void *workspace, int64_t workspace_bytes, ac4k_stream_t stream) {
+  return grouped_linear(true, D, d_dtype, A, A_sf, A_gs, T, rows, B, B_sf, B_gs, B_gs_stride, bias, bias_dtype, offsets, M, N, K, E, workspace,
+                        workspace_bytes, stream);
 }
 
 extern "C" __attribute__((visibility("default"))) int ac4k_debug_last_grouped_kernel(void) { return ac4k::g_last_grouped_kernel; }

@@ -78,12 +78,13 @@ def grouped_linear(x, x_scale, x_global_scale, weight, weight_scale, weight_glob
 
     x [T, K/2] and weight [E, N, K/2] are packed e2m1 (uint8), as `quantize(x, 0, 1)` and `quantize(w, 1, 2)` return them, x_scale [K/64,
     align_up(T,16), 4] and weight_scale [E, K/64, align_up(N,16), 4] their e4m3 scales, the global scales fp32, that of the weights
-    0-dim or [E].  offsets int32 [E+1] on the GPU, rising from 0; the call does not wait for it, and rows of y that no range holds
-    stay as they are.  rows int32 [M] (GPU): the row of x of each row of y, so that the tokens of a top-k routing are
+    0-dim or [E].  offsets int32 [E+1] on the GPU, rising; the call does not wait for it.  Rows of y that no range holds
+    (in front of offsets[0], from offsets[E] on) are zero in a new tensor, and stay as they are in `out`.  rows int32 [M] (GPU): the row of x of each row of y, so that the tokens of a top-k routing are
     quantized once; None: row i, M = T.  bias [E, N] in bf16/fp16/fp32; out defaults to a new bf16 [M, N] and may be bf16, fp16 or fp32.
     K must be a multiple of 64.
     """
-    if out is None:
+    fresh = out is None
+    if fresh:
         out = torch.empty((x.size(0) if rows is None else rows.size(0), weight.size(1)), dtype=torch.bfloat16, device=x.device)
-    _rocm_ops.linear_grouped_nvfp4(out, x, x_scale, x_global_scale, weight, weight_scale, weight_global_scale, offsets, rows, bias)
+    _rocm_ops.linear_grouped_nvfp4(out, x, x_scale, x_global_scale, weight, weight_scale, weight_global_scale, offsets, rows, bias, fresh)
     return out

@@ -379,7 +379,13 @@ int ac4k_linear_grouped_nvfp4(void *D, int d_dtype, const void *A, const void *A
                               const void *bias, int bias_dtype, const int32_t *offsets, int64_t M, int64_t N, int64_t K,
                               int64_t E, void *workspace, int64_t workspace_bytes, ac4k_stream_t stream);
 
-/* Introspection for tests (no counterpart in the reference): which kernel the calling host thread's last ac4k_linear_grouped_nvfp4 launched: 0 none yet, 1 sixteen
+/* The same for a D that is new memory: rows in front of offsets[0] and from offsets[E] on are set to zero. */
+int ac4k_linear_grouped_nvfp4_whole(void *D, int d_dtype, const void *A, const void *A_sf, const float *A_gs, int64_t T,
+                                    const int32_t *rows, const void *B, const void *B_sf, const float *B_gs, int64_t B_gs_stride,
+                                    const void *bias, int bias_dtype, const int32_t *offsets, int64_t M, int64_t N, int64_t K,
+                                    int64_t E, void *workspace, int64_t workspace_bytes, ac4k_stream_t stream);
+
+/* Introspection for tests (no counterpart in the reference): which kernel the calling host thread's last grouped linear launched: 0 none yet, 1 sixteen
  * weight rows a workgroup, 2 tiles of 64 x 128, 3 of 64 x 256, 4 of 256 x 256 (behind the launch that gathers scales, where there are `rows`). */
 int ac4k_debug_last_grouped_kernel(void);
 

@@ -117,3 +117,23 @@ def test_graph_replays_with_other_groups(kernel, m, n, k, e):
             assert torch.equal(out, call())
         check(p, graphs[0][1])
         assert torch.equal(graphs[0][1], graphs[1][1])
+
+
+@pytest.mark.parametrize("kernel,m,n,k,e", [(ROWS16, 28, 1000, 2048, 2), *TABLES[1:]])
+@pytest.mark.parametrize("before,behind", [(0, 9), (6, 0), (5, 7)])
+def test_rows_of_no_range_in_a_new_tensor_are_zero(kernel, m, n, k, e, before, behind):
+    """Also where the memory of the new tensor held something else before; no range at all; no experts."""
+    inner = m - before - behind
+    p = Problem([inner // e] * (e - 1) + [inner - inner // e * (e - 1)], n, k, rows_of=60, seed=4, before=before, behind=behind)
+    def run():
+        junk = torch.full((m, n), float("nan"), dtype=torch.bfloat16, device="cuda")
+        del junk
+        return p.run()
+    y = run()
+    assert ran() == kernel
+    check(p, y)
+    assert (y[:before] == 0).all() and (y[m - behind:] == 0).all()
+    p.offsets = torch.full((e + 1,), m // 2, dtype=torch.int32)
+    assert (run() == 0).all()
+    none = ops().grouped_linear(*p.x, p.w[0][:0], p.w[1][:0], p.w[2][:0], torch.zeros(1, dtype=torch.int32, device="cuda"), rows=p.rows.cuda())
+    assert none.shape == (m, n) and (none == 0).all()
