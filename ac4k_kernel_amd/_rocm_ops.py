@@ -808,6 +808,12 @@ def linear_grouped_nvfp4(D, A, A_sf, A_global_scale, B, B_sf, B_global_scale, of
             D.zero_()
         return
     _check(T > 0, "rows of an empty a")
+    if not whole:  # (otherwise D is new memory)
+        first = D.data_ptr()
+        end = first + M * N * D.element_size()
+        for t in (A, A_sf, A_global_scale, B, B_sf, B_global_scale, offsets, rows, bias):  # all contiguous
+            if t is not None and t.data_ptr() < end and first < t.data_ptr() + t.nbytes:
+                _check(False, "out must not overlap an operand")
     nbytes = _L.ac4k_linear_grouped_nvfp4_workspace_bytes(T, M, N, K, E, int(rows is not None))
     ws = D.new_empty((nbytes,), dtype=torch.uint8) if nbytes > 0 else None
     call = _L.ac4k_linear_grouped_nvfp4_whole if whole else _L.ac4k_linear_grouped_nvfp4

@@ -1,0 +1,54 @@
+"""Outputs that share memory with an operand: refused where another workgroup could still read what one has overwritten, accepted where they only touch.
+Operands are laid into a buffer of bytes, the output over their first or last ones, or right beside them."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+AT = 4096  # of the operand in its buffer
+
+
+def ops():
+    from ac4k_kernel_amd import ops as o
+    return o
+
+
+def laid(t):
+    """(buffer of bytes, copy of t at AT in it, bytes of t)"""
+    n = t.numel() * t.element_size()
+    buf = torch.zeros(3 * AT + n, dtype=torch.uint8, device="cuda")
+    copy = buf[AT:AT + n].view(t.dtype).reshape(t.shape)
+    copy.copy_(t)
+    return buf, copy, n
+
+
+def at(buf, first, shape, dtype):
+    n = math.prod(shape) * torch.empty((), dtype=dtype).element_size()
+    return buf[first:first + n].view(dtype).reshape(shape)
+
+
+def around(t, shape, dtype):
+    """Copy of t, outputs of shape over its first and its last element, and outputs right in front of it and behind it."""
+    buf, copy, n = laid(t)
+    size = torch.empty((), dtype=dtype).element_size()
+    out = math.prod(shape) * size
+    step = -(-n // size) * size
+    meet = [at(buf, AT + size - out, shape, dtype), at(buf, AT + (n - 1) // size * size, shape, dtype)]
+    return copy, meet, [at(buf, AT - out, shape, dtype), at(buf, AT + step, shape, dtype)]
+
+
+def test_grouped_linear():
+    x = ops().quantize(torch.ones((6, 64), dtype=torch.bfloat16, device="cuda"), 0, 1)
+    w = ops().quantize(torch.ones((2, 4, 64), dtype=torch.bfloat16, device="cuda"), 1, 2)
+    args = {"x": x[0], "x_scale": x[1], "x_global_scale": x[2], "weight": w[0], "weight_scale": w[1], "weight_global_scale": w[2],
+            "offsets": torch.tensor([0, 2, 6], dtype=torch.int32, device="cuda"), "rows": torch.arange(6, dtype=torch.int32, device="cuda"),
+            "bias": torch.ones((2, 4), dtype=torch.bfloat16, device="cuda")}
+    want = ops().grouped_linear(**args)
+    for name, t in args.items():
+        copy, meet, beside = around(t, (6, 4), torch.bfloat16)
+        for out in meet:
+            with pytest.raises(RuntimeError, match="overlap"):
+                ops().grouped_linear(**{**args, name: copy}, out=out)
+        for out in beside:
+            assert torch.equal(ops().grouped_linear(**{**args, name: copy}, out=out), want)
