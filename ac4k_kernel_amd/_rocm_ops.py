@@ -694,7 +694,7 @@ def rope(outs, xs, table, sections, positions, grid, bnhd: bool, interleaved: bo
     if x.get_device() != dev or table.get_device() != dev:
         _same_device(x, table)
     args, used = _RopePair(), 0
-    made = []
+    made, spans = [], []  # spans: first and end address of the caller's outputs
     for i, t in enumerate(xs):
         if i:
             if t.get_device() != dev or t.dtype is not x.dtype or t.dim() != 4 or t.shape[0] != B or t.shape[1 if bnhd else 2] != N or t.shape[3] != D:
@@ -717,6 +717,10 @@ def rope(outs, xs, table, sections, positions, grid, bnhd: bool, interleaved: bo
         if t.numel() == 0:
             continue
         o_b, o_n, o_h, _ = o.stride()
+        if outs is not None:
+            first = o.data_ptr()
+            last = sum([(n - 1) * s for n, s in zip(o.shape, (o_b, o_n, o_h, 1))])
+            spans.append((first, first + (1 + last) * (4 if tag == 2 else 2)))
         args[used] = ((t.data_ptr(), o.data_ptr(), t_b, t_n, t_h, o_b, o_n, o_h, t.shape[2]) if bnhd else
                       (t.data_ptr(), o.data_ptr(), t_b, t_h, t_n, o_b, o_h, o_n, t.shape[1]))
         used += 1
@@ -735,6 +739,13 @@ def rope(outs, xs, table, sections, positions, grid, bnhd: bool, interleaved: bo
         _check(grid is not None and len(grid) == axes and min(grid) >= 1, "grid must have one size of at least 1 for each axis")
         _check(max(grid) <= length, "the table has {} positions, the grid {}", length, max(grid))
         grid_arg = (_lib._i64 * axes)(*grid)
+    for first, end in spans:
+        at = table.data_ptr()
+        if at < end and first < at + length * pairs * 8:
+            _check(False, "out must not overlap the table")
+        if pos_ptr is not None and pos_ptr < end:
+            last = sum([(n - 1) * s for n, s in zip(positions.shape, pos_strides)])
+            _check(first >= pos_ptr + (1 + last) * pos_bytes, "out must not overlap the positions")
     if used:
         _lib.check(_L.ac4k_rope(args, used, tag, B, N, D, table.data_ptr(), length, pairs, section_arg, axes, pos_ptr, pos_bytes, *pos_strides,
                                 grid_arg, interleaved, inverse, _stream()))

@@ -52,3 +52,21 @@ def test_grouped_linear():
                 ops().grouped_linear(**{**args, name: copy}, out=out)
         for out in beside:
             assert torch.equal(ops().grouped_linear(**{**args, name: copy}, out=out), want)
+
+
+def test_rope():
+    table, pos = ops().rope_table(8, 12), torch.arange(10, dtype=torch.int32, device="cuda").reshape(1, 2, 5)
+    for dtype in (torch.bfloat16, torch.float32):
+        q, k = (torch.ones((2, 5, h, 16), dtype=dtype, device="cuda") for h in (3, 1))
+        want = ops().rope((q, k), table, positions=pos)
+        for name, t in (("table", table), ("positions", pos), ("positions", pos.long())):
+            args = {"table": table, "positions": pos}
+            for x, y in ((q, want[0]), (k, want[1])):
+                copy, meet, beside = around(t, x.shape, dtype)
+                for out in meet:
+                    with pytest.raises(RuntimeError, match="overlap"):
+                        ops().rope(x, **{**args, name: copy}, out=out)
+                    with pytest.raises(RuntimeError, match="overlap"):  # the second of a pair
+                        ops().rope((q, x), **{**args, name: copy}, out=(torch.empty_like(q), out))
+                for out in beside:
+                    assert torch.equal(ops().rope(x, **{**args, name: copy}, out=out), y)
