@@ -648,7 +648,7 @@ def dequantize(out, q, sf, global_scale=None, dtype=None, cols=None):
         _same_device(out)
         *out_lead, cols = out.shape
         _check(out.is_contiguous() and out_lead == [*lead, R] and cols <= W, "out must be contiguous of [.., {}, up to {}]", R, W)
-        _check(not _may_overlap(out, q) and not _may_overlap(out, sf), "out must not overlap the quantized operands")
+        _check(not any(_may_overlap(out, t) for t in (q, sf, global_scale) if t is not None), "out must not overlap the quantized operands")
     if planes and R and cols:
         _lib.check(_L.ac4k_dequantize(out.data_ptr(), tag, q.data_ptr(), sf.data_ptr(), gs_ptr, gs_step, planes, R, W, cols, number, _stream()))
     return out

@@ -70,3 +70,17 @@ def test_rope():
                         ops().rope((q, x), **{**args, name: copy}, out=(torch.empty_like(q), out))
                 for out in beside:
                     assert torch.equal(ops().rope(x, **{**args, name: copy}, out=out), y)
+
+
+@pytest.mark.parametrize("precision", ["nvfp4", "fp8e4m3", "int8"])
+def test_dequantize(precision):
+    quantized = ops().rms_norm(torch.ones((5, 64), dtype=torch.bfloat16, device="cuda"), precision=precision)
+    want = ops().dequantize(*quantized)
+    for i, t in enumerate(quantized):
+        copy, meet, beside = around(t, want.shape, want.dtype)
+        operands = [copy if j == i else u for j, u in enumerate(quantized)]
+        for out in meet:
+            with pytest.raises(RuntimeError, match="overlap"):
+                ops().dequantize(*operands, out=out)
+        for out in beside:
+            assert torch.equal(ops().dequantize(*operands, out=out), want)
