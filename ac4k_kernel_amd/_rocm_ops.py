@@ -565,7 +565,8 @@ def rms_norm(out, sf, global_scale, given_scale: bool, x, weight, residual, resi
             for t in (x, residual):
                 _check(_same_rows(t, residual_out) or not _may_overlap(t, residual_out),
                        "residual_out may be x or residual itself, but not overlap them otherwise")
-            _check(weight is None or not _may_overlap(weight, residual_out), "residual_out must not overlap weight")
+            for t in (weight, global_scale):
+                _check(t is None or not _may_overlap(t, residual_out), "residual_out must not overlap weight or global_scale")
     out_step = K
     if not fresh:
         if precision is None:

@@ -84,3 +84,16 @@ def test_dequantize(precision):
                 ops().dequantize(*operands, out=out)
         for out in beside:
             assert torch.equal(ops().dequantize(*operands, out=out), want)
+
+
+def test_norm_with_a_given_scale():
+    x = torch.ones((5, 64), dtype=torch.bfloat16, device="cuda")
+    scale = torch.tensor(0.01, device="cuda")
+    want = ops().rms_norm(x, residual=x, precision="nvfp4", global_scale=scale)
+    copy, meet, beside = around(scale, x.shape, x.dtype)
+    for out in meet:
+        with pytest.raises(RuntimeError, match="overlap"):
+            ops().rms_norm(x, residual=x, residual_out=out, precision="nvfp4", global_scale=copy)
+    for out in beside:
+        got = ops().rms_norm(x, residual=x, residual_out=out, precision="nvfp4", global_scale=copy)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[3], want[3])
