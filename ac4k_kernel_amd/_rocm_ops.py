@@ -587,6 +587,8 @@ def rms_norm(out, sf, global_scale, given_scale: bool, x, weight, residual, resi
         _check_tensor(global_scale, torch.float32, "global_scale")
         _check(global_scale.dim() == 0, "global_scale must be a scalar")
     if rows == 0:
+        if global_scale is not None and not given_scale:
+            global_scale.zero_()  # that of a tensor of zeros
         return
     ws_ptr, nbytes = None, 0
     if number == 3 and not given_scale:

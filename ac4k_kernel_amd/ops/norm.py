@@ -21,7 +21,7 @@ def rms_norm(x, weight=None, eps=1e-6, residual=None, residual_out=None, precisi
       "nvfp4"           (output [rows, align_up(K,64)/2] u8, sf [align_up(K,64)/64, align_up(rows,16), 4] e4m3, global_scale)
       "fp8e4m3"/"int8"  (output [rows, align_up(K,16)], sf [align_up(rows,16)] fp32)
     A positive 0-dim fp32 global_scale that is passed in is used as it is and saves finding the maximum over all rows.
-    Rows whose largest |y| is under 2^-100 (nvfp4: tensors) give zero codes and zero scales.
+    Rows whose largest |y| is under 2^-100 (nvfp4: tensors, and tensors of no rows) give zero codes and zero scales.
     With a residual, h is returned behind the rest; residual_out says where to (default a new tensor; x or residual themselves
     are allowed).
     """
