@@ -501,12 +501,28 @@ def _rows_view(t, name: str):
 
 
 def _may_overlap(a, b) -> bool:
-    """Whether the memory between the first and the last element of two tensors meets."""
-    def ends(t):
-        first = t.data_ptr()
-        return first, first + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
-    (a0, a1), (b0, b1) = ends(a), ends(b)
-    return a0 < b1 and b0 < a1
+    """Whether two tensors can share memory: not if one ends before the other begins, nor if, of every length of some stride, each has a part
+    of its own (columns of the rows of one buffer, heads of one projection)."""
+    if not (a.numel() and b.numel()):
+        return False
+    a0, b0, size_a, size_b = a.data_ptr(), b.data_ptr(), a.element_size(), b.element_size()
+    if a0 <= b0:
+        if a0 + size_a * (1 + sum([(n - 1) * s for n, s in zip(a.shape, a.stride())])) <= b0:
+            return False
+    elif b0 + size_b * (1 + sum([(n - 1) * s for n, s in zip(b.shape, b.stride())])) <= a0:
+        return False
+    dims_a = [(s * size_a, n) for s, n in zip(a.stride(), a.shape) if n > 1]
+    dims_b = [(s * size_b, n) for s, n in zip(b.stride(), b.shape) if n > 1]
+    steps = {s for s, _ in dims_a + dims_b}
+    for step in steps:
+        if step and not any(s > step and s % step for s in steps):
+            # the longer strides are whole steps: every element is inside [0, part) of the place of the first one, in steps
+            part_a = size_a + sum((n - 1) * s for s, n in dims_a if s < step)
+            part_b = size_b + sum((n - 1) * s for s, n in dims_b if s < step)
+            away = (b0 - a0) % step
+            if part_a <= away and away + part_b <= step:
+                return False
+    return True
 
 
 def _places_of_their_own(t) -> bool:
@@ -728,8 +744,8 @@ def rope(outs, xs, table, sections, positions, grid, bnhd: bool, interleaved: bo
                       (t.data_ptr(), o.data_ptr(), t_b, t_h, t_n, o_b, o_h, o_n, t.shape[1]))
         used += 1
     if count == 2 and outs is not None:
-        _check(not any(_may_overlap(o, t) for o, t in ((outs[0], xs[1]), (outs[1], xs[0]), (outs[0], outs[1])) if o.numel() and t.numel())
-               or _interleaved_heads(outs, xs), "the two tensors must not overlap each other")
+        _check(not any(_may_overlap(o, t) for o, t in ((outs[0], xs[1]), (outs[1], xs[0]), (outs[0], outs[1]))),
+               "the two tensors must not overlap each other")
     pos_ptr, pos_bytes, pos_strides, grid_arg = None, 0, (0, 0, 0), None
     if positions is not None:
         if grid is not None or positions.dtype not in _POSITIONS or positions.shape != (axes, B, N) or positions.get_device() != dev:
@@ -753,38 +769,6 @@ def rope(outs, xs, table, sections, positions, grid, bnhd: bool, interleaved: bo
         _lib.check(_L.ac4k_rope(args, used, tag, B, N, D, table.data_ptr(), length, pairs, section_arg, axes, pos_ptr, pos_bytes, *pos_strides,
                                 grid_arg, interleaved, inverse, _stream()))
     return outs or tuple(made)
-
-
-def _interleaved_heads(outs, xs) -> bool:
-    """Whether two tensors are slices of the heads of one (q and k of a packed projection): same strides, apart by whole heads that neither
-    reaches into, and each output its input or memory of its own."""
-    (a, b), (c, d) = xs, outs
-    for p, q in ((a, b), (c, d), (c, b), (a, d)):
-        if not _may_overlap(p, q):
-            continue
-        if p.stride() != q.stride():
-            return False
-        away = (q.data_ptr() - p.data_ptr()) // p.element_size()
-        lo, hi = (p, q) if away >= 0 else (q, p)
-        away = abs(away)
-        # rows of the outermost strides stay apart when a row of `lo` ends before `hi` begins and `hi` ends before the next row of `lo`
-        dims = sorted((s, n) for s, n in zip(lo.stride(), lo.shape) if n > 1)
-        reach, step = 1, None
-        for s, n in dims:
-            if s > away:
-                step = s
-                break
-            reach = max(reach, (n - 1) * s + reach)
-        if step is None or reach > away:
-            return False
-        reach_hi = 1
-        for s, n in sorted((s, n) for s, n in zip(hi.stride(), hi.shape) if n > 1):
-            if s >= step:
-                break
-            reach_hi += (n - 1) * s
-        if away + reach_hi > step:
-            return False
-    return True
 
 
 def linear_grouped_nvfp4(D, A, A_sf, A_global_scale, B, B_sf, B_global_scale, offsets, rows=None, bias=None, whole=False) -> None:

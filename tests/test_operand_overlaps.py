@@ -97,3 +97,23 @@ def test_norm_with_a_given_scale():
     for out in beside:
         got = ops().rms_norm(x, residual=x, residual_out=out, precision="nvfp4", global_scale=copy)
         assert torch.equal(got[0], want[0]) and torch.equal(got[3], want[3])
+
+
+def test_columns_of_one_buffer():
+    """Inputs and outputs that are slices of the same rows share nothing and are taken."""
+    wide = torch.randn((33, 5, 3, 64), generator=torch.Generator().manual_seed(1)).bfloat16().cuda()
+    rows = wide.reshape(165, 192)
+    x, y, z = rows[:, :64], rows[:, 64:128], rows[:, 128:]
+    want = ops().rms_norm(x.clone(), residual=z.clone())
+    assert ops().rms_norm(x, residual=z, residual_out=z, out=y)[0] is y
+    assert torch.equal(y, want[0]) and torch.equal(z, want[1])
+    table = ops().rope_table(32, 8)
+    turned = ops().rope(x.clone().reshape(33, 5, 1, 64), table)
+    assert torch.equal(ops().rope(wide[:, :, :1], table, out=wide[:, :, 1:2]), turned)
+    with pytest.raises(RuntimeError, match="overlap"):
+        ops().rms_norm(x, out=rows[:, 63:127])
+
+
+def test_outputs_without_elements():
+    x, outs = torch.empty((2, 0, 64), device="cuda"), [torch.empty((2, 0, 64), device="cuda") for _ in range(2)]
+    assert ops().rms_norm(x, residual=x, residual_out=outs[0], out=outs[1])[0] is outs[1]
