@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from test_gpu_norm import ops
+from test_gpu_norm import DTYPES, EPS, check_plain, check_quantized, data, ops, reference
 
 pytestmark = pytest.mark.gpu
 
@@ -18,3 +18,20 @@ def test_scale_of_no_rows():
     given = torch.tensor(0.5, device="cuda")
     assert ops().rms_norm(x, precision="nvfp4", global_scale=given)[2].item() == 0.5
     assert ops().dequantize(q, sf, scale).shape == (0, 64)
+
+
+@pytest.mark.parametrize("rows,k", [(1, 16385), (3, 20000), (40, 32768), (300, 24581)])
+@pytest.mark.parametrize("dtype,w32,residual", [("bf16", False, True), ("fp16", True, False), ("fp32", True, True)])
+def test_rows_of_sixteen_to_thirty_two_thousand(rows, k, dtype, w32, residual):
+    """Rows of which a lane holds three and four vectors: every output."""
+    x, w = data((rows, k), DTYPES[dtype], rows + k), (data((k,), torch.float32, 3, 0.2) + 1).to(torch.float32 if w32 else DTYPES[dtype])
+    r = data((rows, k), DTYPES[dtype], 7, 3.0) if residual else None
+    h, exact, y32 = reference(x, w, r)
+    for precision in (None, "nvfp4", "fp8e4m3", "int8"):
+        got = ops().rms_norm(x.cuda(), w.cuda(), eps=EPS, residual=None if r is None else r.cuda(), precision=precision)
+        if residual:
+            assert torch.equal(got[-1].cpu(), h)
+        if precision is None:
+            check_plain(got[0] if residual else got, exact)
+        else:
+            check_quantized(got, y32, precision)
