@@ -22,6 +22,8 @@ def rms_norm(x, weight=None, eps=1e-6, residual=None, residual_out=None, precisi
       "fp8e4m3"/"int8"  (output [rows, align_up(K,16)], sf [align_up(rows,16)] fp32)
     A positive 0-dim fp32 global_scale that is passed in is used as it is and saves finding the maximum over all rows.
     Rows whose largest |y| is under 2^-100 (nvfp4: tensors, and tensors of no rows) give zero codes and zero scales.
+    A row with a NaN or an infinite element has NaN in it.  To nvfp4 it makes a global scale that is found NaN, and with it all rows; with a given
+    one the other rows are as without it.
     With a residual, h is returned behind the rest; residual_out says where to (default a new tensor; x or residual themselves
     are allowed).
     """

@@ -35,3 +35,23 @@ def test_rows_of_sixteen_to_thirty_two_thousand(rows, k, dtype, w32, residual):
             check_plain(got[0] if residual else got, exact)
         else:
             check_quantized(got, y32, precision)
+
+
+@pytest.mark.parametrize("rows,k", [(8, 300), (40, 300), (600, 1040)])
+def test_rows_that_are_not_finite_to_nvfp4(rows, k):
+    """One scale for all rows: a row with an infinite or a NaN element makes a found one NaN, and with it every row.  With a given scale the rows without
+    such elements keep their bits; of the others, NaN rows are NaN, and rows with an infinite element have NaN in its block and zeros elsewhere."""
+    x = data((rows, k), torch.bfloat16, 1)
+    given = ops().rms_norm(x.cuda(), precision="nvfp4")
+    bad = x.clone()
+    bad[5, 39] = float("inf")
+    bad[6, k - 1] = float("nan")
+    q, sf, scale = ops().rms_norm(bad.cuda(), precision="nvfp4")
+    assert torch.isnan(scale) and torch.isnan(ops().dequantize(q, sf, scale, cols=k)).all()
+    q, sf, scale = ops().rms_norm(bad.cuda(), precision="nvfp4", global_scale=given[2])
+    keep = torch.tensor([i for i in range(rows) if i not in (5, 6)], device="cuda")
+    assert torch.equal(q[keep], given[0][keep])
+    assert torch.equal(sf.view(torch.uint8)[:, keep], given[1].view(torch.uint8)[:, keep])
+    d = ops().dequantize(q, sf, scale, cols=k)
+    assert torch.isnan(d[6]).all() and torch.isnan(d[5, 32:48]).all()
+    assert (d[5, :32] == 0).all() and (d[5, 48:] == 0).all() and torch.isfinite(d[keep]).all()
