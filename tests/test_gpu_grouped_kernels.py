@@ -137,3 +137,16 @@ def test_rows_of_no_range_in_a_new_tensor_are_zero(kernel, m, n, k, e, before, b
     assert (run() == 0).all()
     none = ops().grouped_linear(*p.x, p.w[0][:0], p.w[1][:0], p.w[2][:0], torch.zeros(1, dtype=torch.int32, device="cuda"), rows=p.rows.cuda())
     assert none.shape == (m, n) and (none == 0).all()
+
+
+@pytest.mark.parametrize("kernel,sizes,n", [(TILES_64_128, [30, 1, 65, 129], 2047), (TILES_64_256, [1500, 0, 1, 1490], 1023),
+                                            (TILES_256, [9000, 0, 1, 22990], 257)])
+@pytest.mark.parametrize("k", [128, 192])
+@pytest.mark.parametrize("gather", [False, True])
+def test_one_and_two_stages(kernel, sizes, n, k, gather):
+    """A K of fewer stages than a kernel keeps under way, a whole one and one that starts in front of the row."""
+    p = Problem(sizes, n, k, rows_of=97 if gather else None, seed=n + k, bias="fp32", before=2, behind=1)
+    y = p.run()
+    assert ran() == kernel
+    check(p, y)
+    assert (y[:2] == 0).all() and (y[-1:] == 0).all()
