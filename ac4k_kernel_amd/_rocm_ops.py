@@ -475,7 +475,8 @@ def _same_device(*tensors) -> None:
     """Kernels run on the current device and its stream: every operand has to be there."""
     dev = _current_device()
     for t in tensors:
-        if t is not None and t.get_device() != dev:
+        if t is not None and not (isinstance(t, torch.Tensor) and t.get_device() == dev):
+            _check(isinstance(t, torch.Tensor), "operands must be tensors, not {}", type(t).__name__)
             _check(False, "operands must be on the current device, {}: got one on {}", dev, t.device)
 
 
@@ -549,6 +550,9 @@ def rms_norm(out, sf, global_scale, given_scale: bool, x, weight, residual, resi
     number = _PRECISIONS.get(precision)
     if number is None:
         _check(False, "precision must be one of {}", list(_PRECISIONS))
+    if global_scale is not None:
+        _check_tensor(global_scale, torch.float32, "global_scale")
+        _check(global_scale.dim() == 0, "global_scale must be a scalar")
     dev = _current_device()
     if x.get_device() != dev or not fresh or global_scale is not None:
         _same_device(x, residual_out, out, sf, global_scale)
@@ -599,9 +603,6 @@ def rms_norm(out, sf, global_scale, given_scale: bool, x, weight, residual, resi
             _check(list(out.shape) == [rows, _align_up(K, 64) // 2 if nvfp4 else _align_up(K, 16)], "meet invalid out shape")
             _check_tensor(sf, torch.float8_e4m3fn if nvfp4 else torch.float32, "sf")
             _check(list(sf.shape) == ([_align_up(K, 64) // 64, _align_up(rows, 16), 4] if nvfp4 else [_align_up(rows, 16)]), "meet invalid sf shape")
-    if global_scale is not None:
-        _check_tensor(global_scale, torch.float32, "global_scale")
-        _check(global_scale.dim() == 0, "global_scale must be a scalar")
     if rows == 0:
         if global_scale is not None and not given_scale:
             global_scale.zero_()  # that of a tensor of zeros

@@ -85,6 +85,10 @@ def grouped_linear(x, x_scale, x_global_scale, weight, weight_scale, weight_glob
     """
     fresh = out is None
     if fresh:
+        if not isinstance(x, torch.Tensor) or x.dim() != 2 or not isinstance(weight, torch.Tensor) or weight.dim() != 3:
+            raise RuntimeError("x must be [rows, K/2] and weight [experts, N, K/2]")
+        if rows is not None and not (isinstance(rows, torch.Tensor) and rows.dim() == 1):
+            raise RuntimeError("rows must be a tensor of one dim")
         out = torch.empty((x.size(0) if rows is None else rows.size(0), weight.size(1)), dtype=torch.bfloat16, device=x.device)
     _rocm_ops.linear_grouped_nvfp4(out, x, x_scale, x_global_scale, weight, weight_scale, weight_global_scale, offsets, rows, bias, fresh)
     return out

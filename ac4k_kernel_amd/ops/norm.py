@@ -35,6 +35,8 @@ def rms_norm(x, weight=None, eps=1e-6, residual=None, residual_out=None, precisi
         view = _rocm_ops._rows_view(x, "x")
     fresh = out is None
     if residual is not None:
+        if not isinstance(residual, torch.Tensor):
+            raise RuntimeError("residual must be a tensor")
         if not residual.is_contiguous() and _rocm_ops._rows_view(residual, "residual") is None:
             if residual_out is residual:
                 raise RuntimeError("residual_out must have rows of contiguous elements, evenly apart")
