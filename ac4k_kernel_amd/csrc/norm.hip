@@ -7,7 +7,8 @@
 // scales of 16 and one fp32 scale max|y| / 2688, from the values in 32 bits: there is no rounding to 16 bits in between.
 //
 // The sum of squares is held in 64 bits.  A code next to a border of its format goes by the last place of r, and with 64 bits r is the
-// correctly rounded factor for every order of the sum: splits of a row over 1, 4 or 16 waves give the same codes.
+// correctly rounded factor for every order of the sum, but for about one row in ten million (see norm_factor): splits of a row over 1, 4
+// or 16 waves give the same codes, but for these.
 //
 // Rows that are all zero (or whose largest |y| is under 2^-100, where the scale would leave the normal fp32 numbers) quantize to zero
 // codes and a zero scale.
@@ -68,8 +69,8 @@ __device__ __forceinline__ double group_sum(double v) {
   return v;
 }
 
-// 1 / sqrt(x) to 2^-50: the hardware's estimate and a step of Newton's method.  Rounded to fp32 it is the correctly rounded value but for one
-// row in ten million; a division behind a square root took twenty times the instructions.
+// 1 / sqrt(x) to 2^-50: the hardware's estimate and two steps of Newton's method.  An error of 2^-50 crosses the middle of two fp32 numbers, 2^-24 apart, in
+// one row of ten million at the most, and so does another order of the sum; a division behind a square root took twenty times the instructions.
 __device__ __forceinline__ float norm_factor(double x) {
   const double e = __builtin_amdgcn_rsq(x);
   const double half = 0.5 * x * e;

@@ -328,7 +328,7 @@ enum { AC4K_PRECISION_NONE = 0, AC4K_PRECISION_FP8 = 1, AC4K_PRECISION_INT8 = 2,
  *   NVFP4: out [rows, align_up(K,64)/2], sf [align_up(K,64)/64, align_up(rows,16), 4]; *global_scale is read where given_scale != 0, otherwise
  *   written: max|y| / 2688 over all rows.
  * (Divisions by 448, 127 and 2688 are products with their fp32 reciprocals, and codes are rounded from y times 448 or 127 times the reciprocal of max|y|.)
- * Every byte of out and sf is written, zeros in the padding.  A row (nvfp4: a tensor) whose max|y| is under 2^-100 gives zero codes and
+ * Every byte of out and sf is written, zeros in the padding (NaN in that of a row of NaN in e4m3, and of a tensor whose scale is NaN in nvfp4).  A row (nvfp4: a tensor) whose max|y| is under 2^-100 gives zero codes and
  * scales, and so does a given scale under 2^-112 or a negative one.  K <= AC4K_NORM_MAX_COLS.  `workspace`: ac4k_rms_norm_workspace_bytes, on 4 bytes, contents irrelevant, NULL when that is 0
  * (it is for everything but nvfp4 whose scale is to be found). */
 int64_t ac4k_rms_norm_workspace_bytes(int64_t rows, int64_t K, int dtype, int precision, int given_scale);
