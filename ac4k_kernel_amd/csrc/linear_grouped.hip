@@ -44,14 +44,14 @@ __device__ __forceinline__ Group group_of(const int32_t *offsets, int64_t e, int
   return {first, end > first ? end - first : 0};
 }
 
-// The rows of D that no range holds, in front of `first` and from `last` on, by all workgroups of the launch in equal shares, before their own work.  (A clearing launch in front would write all of D a second time: half a gigabyte of the 1.4 ms of 16384 x 14336.)
+// The rows of D that no range holds, in front of `first` and from `last` on, by the workgroups of the launch along x in equal shares, before their own work.  (A clearing launch in front would write all of D a second time: half a gigabyte of the 1.4 ms of 16384 x 14336.)
 template <int D_DT>
 __device__ __forceinline__ void zero_other_rows(const GroupedArgs &a, int64_t first, int64_t last) {
   using T = typename Elem<D_DT>::T;
   constexpr int V = 16 / sizeof(T);
   if (last < first) last = first;
   if (first == 0 && last == a.M) return;
-  const int64_t at = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * blockDim.x + threadIdx.x, step = (int64_t)gridDim.x * gridDim.y * blockDim.x;
+  const int64_t at = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, step = (int64_t)gridDim.x * blockDim.x;
   auto zero = [&](int64_t row, int64_t rows) {
     T *p = static_cast<T *>(a.D) + row * a.N;
     const int64_t n = rows * a.N;
@@ -79,10 +79,7 @@ template <int D_DT, int BIAS_DT, int MT>
 __global__ __launch_bounds__(64 * R16_WAVES, 2) void linear_grouped_rows16_kernel(GroupedArgs a) {
   __shared__ float4 part[R16_WAVES][MT][64];
   const Group grp = group_of(a.offsets, blockIdx.y, a.M);
-  if (a.whole) {
-    const Group end = group_of(a.offsets, a.E - 1, a.M);
-    zero_other_rows<D_DT>(a, group_of(a.offsets, 0, a.M).first, end.first + end.count);
-  }
+  if (a.whole && blockIdx.y == gridDim.y - 1) zero_other_rows<D_DT>(a, group_of(a.offsets, 0, a.M).first, grp.first + grp.count);
   if (grp.count == 0) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
   const int64_t e = blockIdx.y, n0 = (int64_t)blockIdx.x * R16_ROWS, kb = a.K >> 1;
