@@ -8,10 +8,10 @@
 // clamped to x: a wrong table gives wrong rows, not an access outside of the operands.  Output rows that no group holds stay as they are, or
 // become zero where the caller's output is new memory.
 //
-// Few rows an expert are bound by the weights' bytes, many by the matrix cores.  128 rows on 64 experts of 2048 x 4096 61-65 us (55 of bytes at the rate of a
-// copy; 440 tiles on 256 CUs leave some a tile less), 16384 rows on 8 experts of 14336 x 4096 1396-1450 us, 1.33-1.38 PFLOP/s, matrix cores busy for 82 % of the
-// time, 4004 rows in uneven groups on 32 experts of 1003 x 2880 41-43 us where the products need 19: half-filled tiles and prologues, matrix cores
-// busy for 38 %.
+// Few rows an expert are bound by the weights' bytes, many by the matrix cores.  128 rows on 64 experts of 2048 x 4096 61-68 us (55 of bytes at the rate of a
+// copy; 440 tiles on 256 CUs leave some a tile less), 16384 rows on 8 experts of 14336 x 4096 1399-1540 us by the card, 1.25-1.38 PFLOP/s, matrix cores busy for
+// 82 % of the time, 4004 rows in uneven groups on 32 experts of 1003 x 2880 42-44 us (45-46 under the profiler) where the products need 19: half-filled tiles and
+// prologues, matrix cores busy for 39 %.
 #include <math.h>
 
 #include "linear_tile.h"

@@ -15,11 +15,12 @@
 //
 // Bound by memory: a row is read once and stays in registers between the sum, the maximum and the conversion; the counters show every byte
 // read and written once.  75600 x 5120 bf16 262 us, 5.9 TB/s (the vector port is busy for 60 % of that); 1000000 x 128 90 us, 5.7 TB/s; one row of 8192
-// 3.8 us, a chain of load, sum, maximum and store.  4001 x 5003 to int8 with fp32 weights, 20.5 us where its bytes need 13, is bound by vector
-// instructions: 147 for eight elements, the port busy for 80 %.
+// 3.7 us, a chain of load, sum, maximum and store.  4001 x 5003 to int8 with fp32 weights, 20-21 us where its bytes need 13, is bound by vector
+// instructions: 144 for eight elements, the port busy for 80 %.
 // nvfp4 without a given global scale takes a second launch, which reads h again (from the memory-side cache where it fits) with r at
-// hand: 8192 x 4096 with a residual 45 + 25 us under the profiler, 56 in a graph, for 46 of bytes; up to 32768 elements one workgroup does all: 1 x 8192 5 us.
-// Rows of more than 32768 elements spill some of their 16 vectors' registers.
+// hand: 8192 x 4096 with a residual 38 + 23 us under the profiler, 59 a call of many, for 46 of bytes; with the scale given 47 and 44.5; up to 32768 elements
+// one workgroup does all: 1 x 8192 4.6 us.  Long rows have fewer waves to hide a row's chain: 8192 x 16384 bf16 106 us (5.1 TB/s), to e4m3 114 (3.5).
+// Rows of more than 32768 elements (fp32 to nvfp4 with a given scale: 16384) spill 40 to 90 registers: 2048 x 65536 162 (3.3), to e4m3 186 (2.2).
 #include "elements.h"
 
 namespace ac4k {
@@ -487,7 +488,7 @@ struct DequantArgs {
 
 // A wave takes 512 columns of four rows, a workgroup 16 rows, whose nvfp4 scales are whole 64-byte runs.  A lane takes eight elements of a row,
 // as one vector of 16 bytes of the output or two, so that a wave's stores are whole runs of a kilobyte.
-// 8192 x 4096 nvfp4 to bf16 14.6 us, 5.9 TB/s.
+// 8192 x 4096 nvfp4 to bf16 14.4 us, 6.1 TB/s; 300000 x 128, a quarter of the lanes at work, 26 us, 3.7 TB/s.
 template <int DT, int PRECISION>
 __global__ __launch_bounds__(256) void dequantize_kernel(DequantArgs a) {
   using T = typename Elem<DT>::T;

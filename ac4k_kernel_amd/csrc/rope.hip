@@ -8,7 +8,7 @@
 //
 // Bound by memory: every element is read and written once.  A thread keeps its token and its place inside the head and goes over the heads, so
 // that it reads its four to eight entries of the table once, while the first heads are under way.  75600 tokens of 80 heads of 128, bf16, 535 us, 5.8 TB/s,
-// every byte read and written once; fp32 2 x 4001 x 24 heads of 64 20 us, 5.0 TB/s; 32 tokens of 48 heads 4.9 us: position, table row and store,
+// every byte read and written once; fp32 2 x 4001 x 24 heads of 64 19-20 us, 4.9-5.1 TB/s; 32 tokens of 48 heads 4.7 us: position, table row and store,
 // one after the other.
 #include "elements.h"
 
@@ -41,7 +41,7 @@ struct RopeArgs {
 
 // WHOLE: no vector is cut by the end of the pairs or of the head, or the last one is moved back to end there, and two threads write the same
 // values to what lies in both (not in place, where one could read what the other has turned).  Four vectors are under way at a time then, with
-// no branch between their loads (with the loads of cut vectors in between, every load was waited for by itself: 20000 x 48 heads of 40, halves, 54 us, now 30).
+// no branch between their loads (with the loads of cut vectors in between, every load was waited for by itself: 20000 x 48 heads of 40, halves, 54 us, now 36; in place still 54).
 template <int DT, bool INTERLEAVED, bool WHOLE>
 __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
   using T = typename Elem<DT>::T;

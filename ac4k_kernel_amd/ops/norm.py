@@ -79,5 +79,6 @@ def dequantize(output, sf, global_scale=None, dtype=torch.bfloat16, cols=None, o
     output [.., R, W/2] u8 (nvfp4) or [.., R, W] e4m3 or int8; sf in the layout of `quantize`; global_scale, for nvfp4, 0-dim or
     one per leading plane.  Returns [.., R, cols] of dtype (bf16, fp16 or fp32), cols up to the padded width W, the
     default.  Each value is the product in fp32, rounded to dtype once.
+    With `out`, contiguous [.., R, up to W] and apart from the operands, its type and columns count instead of dtype and cols.
     """
     return _rocm_ops.dequantize(out, output, sf, global_scale, dtype, cols)
