@@ -150,3 +150,24 @@ def test_one_and_two_stages(kernel, sizes, n, k, gather):
     assert ran() == kernel
     check(p, y)
     assert (y[:2] == 0).all() and (y[-1:] == 0).all()
+
+
+@pytest.mark.parametrize("kernel,m,n,k,e", [(ROWS16, 28, 1000, 2048, 2), *TABLES[1:]])
+def test_graph_of_a_fixed_capacity(kernel, m, n, k, e):
+    """One captured call for up to m rows: replayed with fewer, the rows behind the last range are zero, also where a replay before left values."""
+    p = Problem([m // e] * (e - 1) + [m - m // e * (e - 1)], n, k, rows_of=60, seed=6)
+    rows, offsets = p.rows.cuda(), p.offsets.cuda()
+    call = lambda: ops().grouped_linear(*p.x, *p.w, offsets, rows=rows)
+    call()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = call()
+    assert ran() == kernel
+    for used in (m, m // 3, 0, m - 1, 1):
+        p.offsets = torch.tensor([used * i // e for i in range(e + 1)], dtype=torch.int32)
+        offsets.copy_(p.offsets.cuda())
+        g.replay()
+        torch.cuda.synchronize()
+        check(p, out)
+        assert (out[used:] == 0).all() and torch.equal(out, call())
