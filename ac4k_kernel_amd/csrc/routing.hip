@@ -1,0 +1,523 @@
+// Routing of tokens to experts with the plan that the grouped linears read, and the weighted return of the experts' rows to their tokens.
+//
+//   score_e = exp(l_e) / sum exp(l), or 1 / (1 + exp(-l_e))      key_e = score_e + bias_e
+// A token takes the `k` experts of largest key, ties to the lowest index; with groups only those of the `top_groups` groups whose `best` (1 or 2)
+// largest keys have the largest sum.  An expert whose logit or key is -inf is never taken; a NaN counts as the largest key.  weight = score, over the sum of the
+// chosen ones with renormalize, times scale.
+//
+// Without a bias and without sums of two keys the order of the keys is that of the logits, which are compared as they are: no rounding decides.
+// Otherwise scores and keys are held in 64 bits, so that keys next to each other are told apart as the formula does.
+//
+// The plan is a counting sort by expert that keeps the order of the tokens: a block of 16 tokens keeps, for each expert, the set of its tokens as bits;
+// counts of the blocks in front and bits below a token's own are its place.  Bits are set by atomic ors, whose order does not matter, so every
+// call gives the same plan.
+#include "elements.h"
+
+namespace ac4k {
+
+struct RouteArgs {
+  const void *logits;
+  int64_t stride;           // elements between rows
+  const float *bias;        // or null
+  float *weights;           // [T, k]
+  int32_t *experts;         // [T, k]
+  int32_t *offsets;         // [E + 1]
+  int32_t *rows;            // [T * k]
+  int32_t *places;          // [T, k]
+  uint16_t *masks;          // [blocks, E]: tokens of the block that take the expert
+  int32_t *bases;           // [blocks, E]: rows of the expert in front of the block
+  int32_t *totals;          // [E]
+  int64_t T, blocks;
+  int E, k, groups, top_groups, best, group_size, group_lanes;
+  bool sigmoid, renormalize;
+  double scale;
+};
+
+constexpr int ROUTE_TOKENS = 16;        // of a block
+constexpr int ROUTE_ONE_TOKENS = 64;    // of a call that one workgroup takes
+constexpr int ROUTE_SCAN_EXPERTS = 16;  // of a workgroup of the scan
+
+// Floats and doubles as unsigned numbers of the same order; 0 is -inf (not to be taken), all ones NaN
+__device__ __forceinline__ uint32_t ordered(float x) {
+  if (x != x) return 0xffffffffu;
+  const uint32_t b = __float_as_uint(x + 0.0f);  // -0 is 0
+  return x == -__builtin_inff() ? 0u : b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float unordered(uint32_t k) {
+  return k == 0u ? -__builtin_inff() : k == 0xffffffffu ? __builtin_nanf("") : __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
+__device__ __forceinline__ uint64_t ordered(double x) {
+  if (x != x) return ~0ull;
+  const uint64_t b = __builtin_bit_cast(uint64_t, x + 0.0);
+  return x == -__builtin_inf() ? 0ull : b >> 63 ? ~b : b | 0x8000000000000000ull;
+}
+__device__ __forceinline__ double unordered(uint64_t k) {
+  return k == 0ull ? -__builtin_inf() : k == ~0ull ? __builtin_nan("") : __builtin_bit_cast(double, k >> 63 ? k & 0x7fffffffffffffffull : ~k);
+}
+
+// what the lane at the other end of a step of a reduction holds
+template <int STEP, typename U>
+__device__ __forceinline__ U lane_step(U v) {
+  auto move = [](uint32_t w) {
+    if constexpr (STEP == 1) return dpp_u32<DPP_QUAD_XOR1>(w);
+    else if constexpr (STEP == 2) return dpp_u32<DPP_QUAD_XOR2>(w);
+    else if constexpr (STEP == 4) return dpp_u32<DPP_ROW_HALF_MIRROR>(w);
+    else if constexpr (STEP == 8) return dpp_u32<DPP_ROW_MIRROR>(w);
+    else if constexpr (STEP == 16) return (uint32_t)__builtin_amdgcn_ds_swizzle((int)w, 0x401F);
+    else return (uint32_t)__shfl_xor((int)w, 32);
+  };
+  if constexpr (sizeof(U) == 4) {
+    return __builtin_bit_cast(U, move(__builtin_bit_cast(uint32_t, v)));
+  } else {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    return __builtin_bit_cast(U, (uint64_t)move((uint32_t)(b >> 32)) << 32 | move((uint32_t)b));
+  }
+}
+// reduction over aligned groups of `lanes` (a power of two, the same in the whole wave), in every lane of the group; MOST: of any call
+template <int MOST, typename U, typename F>
+__device__ __forceinline__ U lanes_reduce(U v, int lanes, F f) {
+  if (lanes > 1) v = f(v, lane_step<1>(v));
+  if (lanes > 2) v = f(v, lane_step<2>(v));
+  if (lanes > 4) v = f(v, lane_step<4>(v));
+  if (lanes > 8) v = f(v, lane_step<8>(v));
+  if constexpr (MOST > 16) {
+    if (lanes > 16) v = f(v, lane_step<16>(v));
+    if (lanes > 32) v = f(v, lane_step<32>(v));
+  }
+  return v;
+}
+
+// One token on L lanes, PER experts each, the experts of a group in neighbouring lanes.  Lane s < k returns the token's s-th expert (-1: none) and its weight.
+// All lanes of the wave take part; `valid` false: a token behind the last one.
+template <int DT, int L, int PER, bool WIDE>
+__device__ __forceinline__ void route_token(const RouteArgs &a, int64_t token, bool valid, int sub, int &my_expert, float &my_weight) {
+  using Key = typename std::conditional<WIDE, uint64_t, uint32_t>::type;
+  using T = typename Elem<DT>::T;
+  const T *row = static_cast<const T *>(a.logits) + token * a.stride;
+  const int lg = L == 64 ? a.group_lanes : L;  // (fewer lanes have one group)
+  const int group = L == 64 ? sub / lg : 0, at = (sub - group * lg) * PER, e0 = group * a.group_size + at;
+  float x[PER];
+#pragma unroll
+  for (int j = 0; j < PER; ++j) x[j] = valid && group < a.groups && at + j < a.group_size ? Elem<DT>::load(row, e0 + j) : -__builtin_inff();
+  auto larger = [](Key p, Key q) { return p > q ? p : q; };
+  auto add = [](double p, double q) { return p + q; };
+  Key key[PER];
+  float top;         // the largest logit
+  double sum = 1.0;  // of the softmax
+  if constexpr (WIDE) {
+    double score[PER];
+    if (a.sigmoid) {
+#pragma unroll
+      for (int j = 0; j < PER; ++j) score[j] = 1.0 / (1.0 + exp(-(double)x[j]));
+      top = 0.0f;
+    } else {
+      top = x[0];
+#pragma unroll
+      for (int j = 1; j < PER; ++j) top = fmaxf(top, x[j]);
+      top = lanes_reduce<L>(top, L, [](float p, float q) { return fmaxf(p, q); });
+      sum = 0.0;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        score[j] = x[j] == -__builtin_inff() ? 0.0 : exp((double)x[j] - (double)top);
+        sum += score[j];
+      }
+      sum = lanes_reduce<L>(sum, L, add);
+#pragma unroll
+      for (int j = 0; j < PER; ++j) score[j] /= sum;
+    }
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const bool allowed = x[j] != -__builtin_inff();
+      double v = score[j];
+      if (a.bias && allowed) v += (double)a.bias[e0 + j];
+      key[j] = allowed ? ordered(v) : 0;
+    }
+  } else {
+    Key m = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      key[j] = ordered(x[j]);
+      m = larger(m, key[j]);
+    }
+    top = unordered(lanes_reduce<L>(m, L, larger));
+    if (!a.sigmoid && !a.renormalize) {
+      float s = 0.0f;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) s += x[j] == -__builtin_inff() ? 0.0f : expf(x[j] - top);
+      sum = lanes_reduce<L>((double)s, L, add);
+    }
+  }
+  // the lane's largest key and the expert that has it, the lowest one
+  auto best_of = [&](const Key(&k)[PER], Key &m, int &e) {
+    m = k[0], e = e0;
+#pragma unroll
+    for (int j = 1; j < PER; ++j)
+      if (k[j] > m) m = k[j], e = e0 + j;
+  };
+  if (L == 64 && a.groups > 1) {
+    Key m;
+    int e;
+    best_of(key, m, e);
+    Key total = lanes_reduce<L>(m, lg, larger);
+    if (WIDE && a.best == 2 && a.group_size > 1) {
+      // the second one: the largest of all but the first
+      const int first = lanes_reduce<L>(m == total ? e : 0x7fffffff, lg, [](int p, int q) { return p < q ? p : q; });
+      Key second = 0;
+#pragma unroll
+      for (int j = 0; j < PER; ++j)
+        if (e0 + j != first) second = larger(second, key[j]);
+      second = lanes_reduce<L>(second, lg, larger);
+      if constexpr (WIDE)
+        if (second) total = ordered(unordered(total) + unordered(second));
+    }
+    int rank = 0;  // groups in front of this one
+    for (int g = 0; g < a.groups; ++g) {
+      Key other;
+      if constexpr (WIDE)
+        other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(total >> 32), g * lg) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)total, g * lg);
+      else
+        other = (uint32_t)__builtin_amdgcn_readlane((int)total, g * lg);
+      rank += other > total || (other == total && g < group) ? 1 : 0;
+    }
+    if (rank >= a.top_groups) {
+#pragma unroll
+      for (int j = 0; j < PER; ++j) key[j] = 0;
+    }
+  }
+  my_expert = -1;
+  for (int s = 0; s < a.k; ++s) {
+    Key m;
+    int e;
+    best_of(key, m, e);
+    const Key most = lanes_reduce<L>(m, L, larger);
+    const int taken = lanes_reduce<L>(m == most ? e : 0x7fffffff, L, [](int p, int q) { return p < q ? p : q; });
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if (e0 + j == taken) key[j] = 0;
+    if (sub == s && most != 0) my_expert = taken;
+  }
+  double w = 0.0;
+  if (my_expert >= 0) {
+    const double v = (double)Elem<DT>::load(row, my_expert);
+    w = a.sigmoid ? 1.0 / (1.0 + exp(-v)) : exp(v - (double)top) / sum;
+  }
+  if (a.renormalize) {
+    const double all = lanes_reduce<L>(w, L, add);
+    w = all == 0.0 ? 0.0 : w / all;
+  }
+  my_weight = (float)(w * a.scale);
+}
+
+// The places of a block's tokens: `base` rows of expert e in front of the block (its range's start among them)
+template <typename Base>
+__device__ __forceinline__ void route_place(const RouteArgs &a, int64_t t, int slot, int e, uint64_t mask, int in_block, Base base) {
+  const int64_t i = t * a.k + slot;
+  int place = -1;
+  if (e >= 0) {
+    place = base(e) + __popcll(mask & ((1ull << in_block) - 1));
+    a.rows[place] = (int32_t)t;
+  }
+  a.places[i] = place;
+}
+
+// Start of each expert's range from the counts in `count` [E] (LDS), in place, behind a barrier; returns the number of rows.  Whole workgroup.
+template <int THREADS>
+__device__ __forceinline__ int route_starts(int *count, int E, int *wave_sum) {
+  constexpr int MOST = (AC4K_ROUTE_MAX_EXPERTS + THREADS - 1) / THREADS;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int c[MOST], sum = 0;
+#pragma unroll
+  for (int j = 0; j < MOST; ++j) {
+    const int e = tid * MOST + j;
+    c[j] = e < E ? count[e] : 0;
+    sum += c[j];
+  }
+  int before = sum;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int v = __shfl_up(before, d);
+    if (lane >= d) before += v;
+  }
+  if (lane == 63) wave_sum[wave] = before;
+  __syncthreads();
+  int total = 0;
+  before -= sum;
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) {
+    if (w < wave) before += wave_sum[w];
+    total += wave_sum[w];
+  }
+#pragma unroll
+  for (int j = 0; j < MOST; ++j) {
+    const int e = tid * MOST + j;
+    if (e < E) count[e] = before;
+    before += c[j];
+  }
+  __syncthreads();
+  return total;
+}
+
+// Scores, choice and weights of a block's tokens and the sets of its experts
+template <int DT, int L, int PER, bool WIDE>
+__global__ __launch_bounds__(256) void route_kernel(RouteArgs a) {
+  __shared__ uint32_t mask[AC4K_ROUTE_MAX_EXPERTS];
+  constexpr int AT_ONCE = 256 / L;
+  const int tid = threadIdx.x, sub = tid % L;
+  for (int e = tid; e < a.E; e += 256) mask[e] = 0;
+  __syncthreads();
+  const int64_t t0 = (int64_t)blockIdx.x * ROUTE_TOKENS;
+#pragma unroll 1
+  for (int b = tid / L; b < ROUTE_TOKENS; b += AT_ONCE) {
+    const int64_t t = t0 + b;
+    int e;
+    float w;
+    route_token<DT, L, PER, WIDE>(a, t, t < a.T, sub, e, w);
+    if (t < a.T && sub < a.k) {
+      a.experts[t * a.k + sub] = e;
+      a.weights[t * a.k + sub] = w;
+      if (e >= 0) atomicOr(&mask[e], 1u << b);
+    }
+  }
+  __syncthreads();
+  for (int e = tid; e < a.E; e += 256) a.masks[(int64_t)blockIdx.x * a.E + e] = (uint16_t)mask[e];
+}
+
+// Counts of each expert in the blocks in front of each block: 64 runs of blocks and 16 experts a workgroup
+__global__ __launch_bounds__(64 * ROUTE_SCAN_EXPERTS) void route_scan_kernel(RouteArgs a) {
+  __shared__ int part[64][ROUTE_SCAN_EXPERTS];
+  const int x = threadIdx.x % ROUTE_SCAN_EXPERTS, run = threadIdx.x / ROUTE_SCAN_EXPERTS;
+  const int e = blockIdx.x * ROUTE_SCAN_EXPERTS + x;
+  const int64_t length = ceil_div(a.blocks, 64), b0 = run * length, b1 = b0 + length < a.blocks ? b0 + length : a.blocks;
+  int sum = 0;
+  if (e < a.E) {
+#pragma unroll 8
+    for (int64_t b = b0; b < b1; ++b) sum += __popc((uint32_t)a.masks[b * a.E + e]);
+  }
+  part[run][x] = sum;
+  __syncthreads();
+  int before = 0;
+  for (int r = 0; r < run; ++r) before += part[r][x];
+  if (e >= a.E) return;
+  if (run == 63) a.totals[e] = before + sum;
+#pragma unroll 8
+  for (int64_t b = b0; b < b1; ++b) {
+    a.bases[b * a.E + e] = before;
+    before += __popc((uint32_t)a.masks[b * a.E + e]);
+  }
+}
+
+__global__ __launch_bounds__(256) void route_place_kernel(RouteArgs a) {
+  __shared__ int start[AC4K_ROUTE_MAX_EXPERTS];
+  __shared__ int wave_sum[4];
+  const int tid = threadIdx.x;
+  for (int e = tid; e < a.E; e += 256) start[e] = a.totals[e];
+  __syncthreads();
+  const int total = route_starts<256>(start, a.E, wave_sum);
+  if (blockIdx.x == 0) {
+    for (int e = tid; e < a.E; e += 256) a.offsets[e] = start[e];
+    if (tid == 0) a.offsets[a.E] = total;
+  }
+  const int64_t t0 = (int64_t)blockIdx.x * ROUTE_TOKENS;
+  const int here = (int)(a.T - t0 < ROUTE_TOKENS ? a.T - t0 : ROUTE_TOKENS) * a.k;
+  const int64_t row = (int64_t)blockIdx.x * a.E;
+  for (int i = tid; i < here; i += 256) {
+    const int b = i / a.k, slot = i - b * a.k;
+    const int e = a.experts[t0 * a.k + i];
+    route_place(a, t0 + b, slot, e, e >= 0 ? a.masks[row + e] : 0, b, [&](int x) { return start[x] + a.bases[row + x]; });
+    if (t0 * a.k + i >= total) a.rows[t0 * a.k + i] = -1;
+  }
+}
+
+// All of a small call in one workgroup
+template <int DT, int L, int PER, bool WIDE>
+__global__ __launch_bounds__(1024) void route_one_kernel(RouteArgs a) {
+  __shared__ unsigned long long mask[AC4K_ROUTE_MAX_EXPERTS];
+  __shared__ int start[AC4K_ROUTE_MAX_EXPERTS];
+  __shared__ int wave_sum[16];
+  constexpr int AT_ONCE = 1024 / L, TURNS = ROUTE_ONE_TOKENS / AT_ONCE;
+  const int tid = threadIdx.x, sub = tid % L;
+  for (int e = tid; e < a.E; e += 1024) mask[e] = 0;
+  __syncthreads();
+  int mine[TURNS];
+#pragma unroll
+  for (int i = 0; i < TURNS; ++i) {
+    const int t = i * AT_ONCE + tid / L;
+    mine[i] = -1;
+    if (i * AT_ONCE >= a.T) continue;
+    float w;
+    route_token<DT, L, PER, WIDE>(a, t, t < a.T, sub, mine[i], w);
+    if (t < a.T && sub < a.k) {
+      a.experts[(int64_t)t * a.k + sub] = mine[i];
+      a.weights[(int64_t)t * a.k + sub] = w;
+      if (mine[i] >= 0) atomicOr(&mask[mine[i]], 1ull << t);
+    }
+  }
+  __syncthreads();
+  for (int e = tid; e < a.E; e += 1024) start[e] = __popcll(mask[e]);
+  __syncthreads();
+  const int total = route_starts<1024>(start, a.E, wave_sum);
+  for (int e = tid; e < a.E; e += 1024) a.offsets[e] = start[e];
+  if (tid == 0) a.offsets[a.E] = total;
+#pragma unroll
+  for (int i = 0; i < TURNS; ++i) {
+    const int t = i * AT_ONCE + tid / L;
+    if (t < a.T && sub < a.k) route_place(a, t, sub, mine[i], mine[i] >= 0 ? mask[mine[i]] : 0, t, [&](int x) { return start[x]; });
+  }
+  for (int i = total + tid; i < a.T * a.k; i += 1024) a.rows[i] = -1;
+}
+
+template <int DT, int L, int PER, bool WIDE>
+static void launch_route(const RouteArgs &a, hipStream_t st) {
+  if (a.T <= ROUTE_ONE_TOKENS) {
+    hipLaunchKernelGGL((route_one_kernel<DT, L, PER, WIDE>), dim3(1), dim3(1024), 0, st, a);
+    return;
+  }
+  hipLaunchKernelGGL((route_kernel<DT, L, PER, WIDE>), dim3((unsigned)a.blocks), dim3(256), 0, st, a);
+  hipLaunchKernelGGL(route_scan_kernel, dim3((unsigned)ceil_div(a.E, ROUTE_SCAN_EXPERTS)), dim3(64 * ROUTE_SCAN_EXPERTS), 0, st, a);
+  hipLaunchKernelGGL(route_place_kernel, dim3((unsigned)a.blocks), dim3(256), 0, st, a);
+}
+template <int DT, bool WIDE>
+static int route_shape(RouteArgs a, hipStream_t st) {
+  if (a.groups == 1 && a.k <= 16 && a.E <= 128) {
+    a.group_lanes = 16;
+    if (a.E <= 16) launch_route<DT, 16, 1, WIDE>(a, st);
+    else if (a.E <= 32) launch_route<DT, 16, 2, WIDE>(a, st);
+    else if (a.E <= 64) launch_route<DT, 16, 4, WIDE>(a, st);
+    else launch_route<DT, 16, 8, WIDE>(a, st);
+    return 0;
+  }
+  a.group_lanes = 64;
+  while (a.group_lanes * a.groups > 64) a.group_lanes /= 2;
+  const int64_t per = ceil_div(a.group_size, a.group_lanes);
+  if (per <= 1) launch_route<DT, 64, 1, WIDE>(a, st);
+  else if (per <= 2) launch_route<DT, 64, 2, WIDE>(a, st);
+  else if (per <= 4) launch_route<DT, 64, 4, WIDE>(a, st);
+  else if (per <= 8) launch_route<DT, 64, 8, WIDE>(a, st);
+  else if (per <= 16) launch_route<DT, 64, 16, WIDE>(a, st);
+  else launch_route<DT, 64, 32, WIDE>(a, st);
+  return 0;
+}
+template <int DT>
+static int route_width(const RouteArgs &a, hipStream_t st) {
+  const bool wide = a.bias || (a.groups > 1 && a.best == 2);
+  return wide ? route_shape<DT, true>(a, st) : route_shape<DT, false>(a, st);
+}
+
+static int64_t route_workspace(int64_t T, int64_t E) {
+  if (T <= ROUTE_ONE_TOKENS) return 0;
+  const int64_t blocks = ceil_div(T, ROUTE_TOKENS);
+  return 4 * align_up(E, 4) + 4 * align_up(blocks * E, 4) + 2 * blocks * E;
+}
+
+// ---------------------------------------------------------------------------
+// the experts' rows back to their tokens
+// ---------------------------------------------------------------------------
+struct CombineArgs {
+  void *out;
+  const void *y, *residual;
+  const float *weights;
+  const int32_t *places;
+  int64_t T, M, N, y_stride, residual_stride, out_stride;
+  int k;
+};
+
+// A thread takes eight columns of a token; its places and weights are scalars of the wave.  Rows are read four at a time.
+template <int DT>
+__global__ __launch_bounds__(256) void combine_kernel(CombineArgs a, uint32_t spans) {
+  using T = typename Elem<DT>::T;
+  const uint32_t token = blockIdx.x / spans, span = blockIdx.x - token * spans;
+  const int64_t c = (int64_t)span * 2048 + threadIdx.x * 8;
+  if (c >= a.N) return;
+  const int32_t *places = a.places + (int64_t)token * a.k;
+  const float *weights = a.weights + (int64_t)token * a.k;
+  float sum[8] = {};
+  if (a.residual) {
+    Vec8<DT> r;
+    vec8_load(r, static_cast<const T *>(a.residual) + token * a.residual_stride, c, a.N);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum[i] = vec8_get(r, i);
+  }
+  for (int s0 = 0; s0 < a.k; s0 += 4) {
+    Vec8<DT> v[4];
+    float w[4];
+    bool here[4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const int64_t place = s0 + s < a.k ? places[s0 + s] : -1;
+      here[s] = place >= 0 && place < a.M;
+      w[s] = here[s] ? weights[s0 + s] : 0.0f;
+      if (here[s]) vec8_load(v[s], static_cast<const T *>(a.y) + place * a.y_stride, c, a.N);
+    }
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+      if (here[s]) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum[i] = __builtin_fmaf(vec8_get(v[s], i), w[s], sum[i]);
+      }
+  }
+  Vec8<DT> o;
+  vec8_set(o, sum);
+  vec8_store(static_cast<T *>(a.out) + token * a.out_stride, o, c, a.N);
+}
+
+}  // namespace ac4k
+
+using namespace ac4k;
+
+static bool float_tag(int d) { return d == AC4K_DTYPE_BF16 || d == AC4K_DTYPE_FP16 || d == AC4K_DTYPE_FP32; }
+
+extern "C" __attribute__((visibility("default"))) int64_t ac4k_route_experts_workspace_bytes(int64_t T, int64_t E, int64_t k) {
+  if (T < 1 || E < 1 || E > AC4K_ROUTE_MAX_EXPERTS || k < 1 || k > AC4K_ROUTE_MAX_K) return 0;
+  return route_workspace(T, E);
+}
+
+extern "C" __attribute__((visibility("default"))) int ac4k_route_experts(
+    float *weights, int32_t *experts, int32_t *offsets, int32_t *rows, int32_t *places, const void *logits, int dtype, int64_t stride, const float *bias,
+    int64_t T, int64_t E, int64_t k, int scoring, int64_t groups, int64_t top_groups, int best, int renormalize, double scale, void *workspace,
+    int64_t workspace_bytes, ac4k_stream_t stream) {
+  AC4K_REQUIRE(weights && experts && offsets && rows && places && logits, "null pointer argument");
+  AC4K_REQUIRE(float_tag(dtype), "logits must be bfloat16, half or float (dtype tag %d)", dtype);
+  AC4K_REQUIRE(T >= 1 && E >= 1 && E <= AC4K_ROUTE_MAX_EXPERTS, "tokens must be positive and experts 1 to %d (T=%lld E=%lld)", (int)AC4K_ROUTE_MAX_EXPERTS,
+               (long long)T, (long long)E);
+  AC4K_REQUIRE(scoring == AC4K_SCORE_SOFTMAX || scoring == AC4K_SCORE_SIGMOID, "unknown scoring %d", scoring);
+  AC4K_REQUIRE(groups >= 1 && groups <= 64 && E % groups == 0, "groups must be 1 to 64 and divide the %lld experts, got %lld", (long long)E, (long long)groups);
+  AC4K_REQUIRE(top_groups >= 1 && top_groups <= groups, "top_groups must be 1 to %lld, got %lld", (long long)groups, (long long)top_groups);
+  AC4K_REQUIRE(best == 1 || best == 2, "a group's score is that of its best one or two, not %d", best);
+  AC4K_REQUIRE(k >= 1 && k <= AC4K_ROUTE_MAX_K && k <= E / groups * top_groups, "k must be 1 to %d and at most the %lld experts of the groups taken, got %lld",
+               (int)AC4K_ROUTE_MAX_K, (long long)(E / groups * top_groups), (long long)k);
+  AC4K_REQUIRE(T * k < (1ll << 27) && T < (1ll << 27), "too many tokens (%lld of %lld experts)", (long long)T, (long long)k);
+  const int64_t need = route_workspace(T, E);
+  AC4K_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 3) == 0), "workspace of %lld bytes needed, on 4 bytes", (long long)need);
+  RouteArgs a{};
+  a.logits = logits, a.stride = stride, a.bias = bias, a.weights = weights, a.experts = experts, a.offsets = offsets, a.rows = rows, a.places = places;
+  a.T = T, a.blocks = ceil_div(T, ROUTE_TOKENS), a.E = (int)E, a.k = (int)k;
+  a.groups = (int)(top_groups == groups ? 1 : groups), a.top_groups = (int)top_groups, a.best = best, a.group_size = (int)(E / a.groups);
+  a.sigmoid = scoring == AC4K_SCORE_SIGMOID, a.renormalize = renormalize != 0, a.scale = scale;
+  a.totals = static_cast<int32_t *>(workspace);
+  a.bases = a.totals + align_up(E, 4);
+  a.masks = reinterpret_cast<uint16_t *>(a.bases + align_up(a.blocks * E, 4));
+  hipStream_t st = (hipStream_t)stream;
+  int rc;
+  if (dtype == AC4K_DTYPE_BF16) rc = route_width<AC4K_DTYPE_BF16>(a, st);
+  else if (dtype == AC4K_DTYPE_FP16) rc = route_width<AC4K_DTYPE_FP16>(a, st);
+  else rc = route_width<AC4K_DTYPE_FP32>(a, st);
+  if (rc) return rc;
+  return check_launch("ac4k_route_experts");
+}
+
+extern "C" __attribute__((visibility("default"))) int ac4k_combine_experts(
+    void *out, int64_t out_stride, const void *y, int64_t y_stride, const float *weights, const int32_t *places, const void *residual, int64_t residual_stride,
+    int64_t T, int64_t k, int64_t M, int64_t N, int dtype, ac4k_stream_t stream) {
+  AC4K_REQUIRE(out && (y || M == 0) && weights && places, "null pointer argument");
+  AC4K_REQUIRE(float_tag(dtype), "y must be bfloat16, half or float (dtype tag %d)", dtype);
+  AC4K_REQUIRE(T >= 1 && k >= 1 && M >= 0 && N >= 1, "sizes must be positive (T=%lld k=%lld N=%lld)", (long long)T, (long long)k, (long long)N);
+  const int64_t spans = ceil_div(N, 2048);
+  AC4K_REQUIRE(k < (1ll << 16) && M < (1ll << 31) && T < (1ll << 24) && spans < (1ll << 24) && T * spans < (1ll << 24), "problem too large");  // 2^32 threads a launch
+  const CombineArgs a{out, y, residual, weights, places, T, M, N, y_stride, residual_stride, out_stride, (int)k};
+  hipStream_t st = (hipStream_t)stream;
+  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)(T * spans)), dim3(256), 0, st, a, (uint32_t)spans); };
+  if (dtype == AC4K_DTYPE_BF16) go(combine_kernel<AC4K_DTYPE_BF16>);
+  else if (dtype == AC4K_DTYPE_FP16) go(combine_kernel<AC4K_DTYPE_FP16>);
+  else go(combine_kernel<AC4K_DTYPE_FP32>);
+  return check_launch("ac4k_combine_experts");
+}

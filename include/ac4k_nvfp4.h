@@ -389,6 +389,30 @@ int ac4k_linear_grouped_nvfp4_whole(void *D, int d_dtype, const void *A, const v
  * weight rows a workgroup, 2 tiles of 64 x 128, 3 of 64 x 256, 4 of 256 x 256 (behind the launch that gathers scales, where there are `rows`). */
 int ac4k_debug_last_grouped_kernel(void);
 
+/* Routing of tokens to experts (no counterpart in the reference), with the plan that ac4k_linear_grouped_nvfp4 reads.
+ *   logits [T, E] of dtype (stride: elements between rows);  score = softmax(l) over the E experts, or 1 / (1 + exp(-l));  key = score + bias (fp32 [E], or NULL).
+ * A token takes the k experts of largest key, in falling order, ties to the lowest index; with top_groups < groups only from those of the `groups` equal
+ * ranges of experts whose `best` (1 or 2) largest keys have the largest sum.  Experts with a logit or key of -inf are not taken; where fewer than k are
+ * left, the other slots have expert -1, weight 0, place -1.  A NaN is the largest key.
+ *   weights fp32 [T, k]: score * scale, with renormalize != 0 over the sum of the token's chosen scores (0 where that is 0);
+ *   experts int32 [T, k];
+ *   offsets int32 [E + 1]: range of rows of each expert, in it the tokens in rising order;  rows int32 [T * k]: the token of each row, -1 from offsets[E] on;
+ *   places int32 [T, k]: the row of each slot.
+ * Without a bias and with best == 1, logits are compared as they are; otherwise keys in 64 bits.  Every call gives the same results again.
+ * `workspace`: ac4k_route_experts_workspace_bytes(T, E, k), on 4 bytes, contents irrelevant, NULL when that is 0. */
+enum { AC4K_SCORE_SOFTMAX = 0, AC4K_SCORE_SIGMOID = 1 };
+#define AC4K_ROUTE_MAX_EXPERTS 1024
+#define AC4K_ROUTE_MAX_K 64
+int64_t ac4k_route_experts_workspace_bytes(int64_t T, int64_t E, int64_t k);
+int ac4k_route_experts(float *weights, int32_t *experts, int32_t *offsets, int32_t *rows, int32_t *places, const void *logits, int dtype,
+                       int64_t stride, const float *bias, int64_t T, int64_t E, int64_t k, int scoring, int64_t groups, int64_t top_groups,
+                       int best, int renormalize, double scale, void *workspace, int64_t workspace_bytes, ac4k_stream_t stream);
+
+/* The experts' rows back to their tokens:  out[t] = residual[t] + sum over s of weights[t, s] * y[places[t, s]], the sum in fp32 in the order of the slots.
+ * y [M, N], residual [T, N] (or NULL) and out [T, N] of dtype, strides in elements between rows; out may be residual.  A place below 0 or from M on adds nothing. */
+int ac4k_combine_experts(void *out, int64_t out_stride, const void *y, int64_t y_stride, const float *weights, const int32_t *places,
+                         const void *residual, int64_t residual_stride, int64_t T, int64_t k, int64_t M, int64_t N, int dtype, ac4k_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
