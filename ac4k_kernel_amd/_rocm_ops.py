@@ -824,59 +824,75 @@ def linear_grouped_nvfp4(D, A, A_sf, A_global_scale, B, B_sf, B_global_scale, of
 _SCORING = {"softmax": 0, "sigmoid": 1}
 
 
-def route_experts(weights, experts, offsets, rows, places, logits, bias, scoring, groups: int, top_groups: int, best: int, renormalize: bool,
-                  scale: float, view=None) -> None:
-    """weights, experts and places [T, k], offsets [E + 1] and rows [T * k], new dense tensors, <- the k experts of each row of logits.  view:
+def route_experts(logits, k: int, bias, scoring, groups: int, top_groups: int, best: int, renormalize: bool, scale: float, view=None):
+    """The k experts of each row of logits: new tensors weights, experts [.., k], offsets [E + 1], rows [T * k] and places [.., k].  view:
     _rows_view(logits), where the caller has it."""
     tag = _check_float(logits, "logits")
     view = view or _rows_view(logits, "logits")
-    _check(view is not None, "logits must have rows of contiguous elements, evenly apart")
+    if view is None:
+        _check(False, "logits must have rows of contiguous elements, evenly apart")
     T, E, stride = view
-    k = weights.shape[-1]
     number = _SCORING.get(scoring)
     if number is None:
         _check(False, "scoring must be one of {}", list(_SCORING))
-    for t, dtype, count, name in ((weights, torch.float32, T * k, "weights"), (experts, torch.int32, T * k, "experts"), (offsets, torch.int32, E + 1, "offsets"),
-                                  (rows, torch.int32, T * k, "rows"), (places, torch.int32, T * k, "places")):
-        _check_tensor(t, dtype, name)
-        _check(t.numel() == count, "{} must have {} elements", name, count)
+    if E > 1024 or not 1 <= groups <= 64 or E % groups or not 1 <= top_groups <= groups or not 1 <= best <= 2 or not 1 <= k <= min(64, E // groups * top_groups):
+        _check(E <= 1024, "at most 1024 experts, got {}", E)
+        _check(1 <= groups <= 64 and E % groups == 0, "groups must be 1 to 64 and divide the {} experts, got {}", E, groups)
+        _check(1 <= top_groups <= groups and 1 <= best <= 2, "top_groups must be 1 to {} and group_best 1 or 2, got {} and {}", groups, top_groups, best)
+        _check(False, "top_k must be 1 to 64 and at most the {} experts of the groups taken, got {}", E // groups * top_groups, k)
     bias_ptr = None
     if bias is not None:
         _check_tensor(bias, torch.float32, "bias")
-        _check(bias.shape == (E,), "bias must be [{}]", E)
+        if bias.shape != (E,):
+            _check(False, "bias must be [{}]", E)
         bias_ptr = bias.data_ptr()
-    _same_device(logits, bias, weights, experts, offsets, rows, places)
+        _same_device(bias)
+    if logits.get_device() != _current_device():
+        _same_device(logits)
+    shape, new = (*logits.shape[:-1], k), logits.new_empty
+    weights, experts, places = new(shape, dtype=torch.float32), new(shape, dtype=torch.int32), new(shape, dtype=torch.int32)
+    offsets, rows = new((E + 1,), dtype=torch.int32), new((T * k,), dtype=torch.int32)
     if T == 0:
         offsets.zero_()
-        return
-    nbytes = _L.ac4k_route_experts_workspace_bytes(T, E, k)
-    ws = logits.new_empty((nbytes,), dtype=torch.uint8) if nbytes > 0 else None
+        return weights, experts, offsets, rows, places
+    nbytes = _L.ac4k_route_experts_workspace_bytes(T, E, k) if T > 64 else 0
+    ws_ptr = None
+    if nbytes > 0:
+        ws = new((nbytes,), dtype=torch.uint8)
+        ws_ptr = ws.data_ptr()
     _lib.check(_L.ac4k_route_experts(weights.data_ptr(), experts.data_ptr(), offsets.data_ptr(), rows.data_ptr(), places.data_ptr(), logits.data_ptr(), tag,
-                                     stride, bias_ptr, T, E, k, number, groups, top_groups, best, int(bool(renormalize)), scale,
-                                     None if ws is None else ws.data_ptr(), nbytes, _stream()))
+                                     stride, bias_ptr, T, E, k, number, groups, top_groups, best, bool(renormalize), scale, ws_ptr, nbytes, _stream()))
+    return weights, experts, offsets, rows, places
 
 
-def combine_experts(out, y, weights, places, residual=None, fresh=False) -> None:
-    """out [.., N] <- residual + the rows of y [M, N] that places [.., k] name, times weights.  fresh: out is a new dense tensor that overlaps nothing."""
+def combine_experts(out, y, weights, places, residual=None):
+    """out [.., N] (None: a new tensor) <- residual + the rows of y [M, N] that places [.., k] name, times weights; returns out."""
     tag = _check_float(y, "y")
-    _check(y.dim() == 2, "y must be a 2d matrix")
+    if y.dim() != 2:
+        _check(False, "y must be a 2d matrix")
     view = _rows_view(y, "y")
-    _check(view is not None, "y must have rows of contiguous elements, evenly apart")
+    if view is None:
+        _check(False, "y must have rows of contiguous elements, evenly apart")
     M, N, y_step = view
     _check_tensor(weights, torch.float32, "weights")
     _check_tensor(places, torch.int32, "places")
-    _check(places.dim() >= 1 and places.shape[-1] >= 1, "places must be [.., k]")
-    _check(weights.shape == places.shape, "weights must have the shape of places")
+    if not places.shape or places.shape[-1] < 1 or weights.shape != places.shape:
+        _check(places.dim() >= 1 and places.shape[-1] >= 1, "places must be [.., k]")
+        _check(False, "weights must have the shape of places")
     *lead, k = places.shape
     T = places.numel() // k
     _same_device(y, weights, places, residual, out)
     residual_ptr, residual_step, out_step = None, 0, N
     if residual is not None:
-        _check(_check_float(residual, "residual") == tag and list(residual.shape) == [*lead, N], "residual must have the type of y and shape {}", [*lead, N])
+        if _check_float(residual, "residual") != tag or residual.shape != (*lead, N):
+            _check(False, "residual must have the type of y and shape {}", [*lead, N])
         v = _rows_view(residual, "residual")
-        _check(v is not None, "residual must have rows of contiguous elements, evenly apart")
+        if v is None:
+            _check(False, "residual must have rows of contiguous elements, evenly apart")
         residual_ptr, residual_step = residual.data_ptr(), v[2]
-    if not fresh:
+    if out is None:
+        out = y.new_empty((*lead, N))
+    else:
         _check(_check_float(out, "out") == tag and list(out.shape) == [*lead, N], "out must have the type of y and shape {}", [*lead, N])
         v = _rows_view(out, "out")
         _check(v is not None and (T <= 1 or v[2] >= N), "out must have rows of contiguous elements, evenly apart")
@@ -886,3 +902,4 @@ def combine_experts(out, y, weights, places, residual=None, fresh=False) -> None
     if T:
         _lib.check(_L.ac4k_combine_experts(out.data_ptr(), out_step, y.data_ptr(), y_step, weights.data_ptr(), places.data_ptr(), residual_ptr, residual_step,
                                            T, k, M, N, tag, _stream()))
+    return out

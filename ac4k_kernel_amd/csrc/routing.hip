@@ -24,32 +24,36 @@ struct RouteArgs {
   int32_t *offsets;         // [E + 1]
   int32_t *rows;            // [T * k]
   int32_t *places;          // [T, k]
-  uint16_t *masks;          // [blocks, E]: tokens of the block that take the expert
+  uint16_t *masks;          // [blocks, Ep]: tokens of the block that take the expert; rows of whole vectors of eight
   int32_t *bases;           // [blocks, E]: rows of the expert in front of the block
   int32_t *totals;          // [E]
   int64_t T, blocks;
-  int E, k, groups, top_groups, best, group_size, group_lanes;
+  int E, Ep, k, groups, top_groups, best, group_size, group_lanes;
   bool sigmoid, renormalize;
   double scale;
 };
 
 constexpr int ROUTE_TOKENS = 16;        // of a block
 constexpr int ROUTE_ONE_TOKENS = 64;    // of a call that one workgroup takes
+constexpr int ROUTE_PLAN_BLOCKS = 16;   // of a workgroup that makes the plan in one launch, where all of them read at most so many masks
+constexpr int64_t ROUTE_PLAN_MASKS = 1 << 25;
 constexpr int ROUTE_SCAN_EXPERTS = 16;  // of a workgroup of the scan
 
 // Floats and doubles as unsigned numbers of the same order; 0 is -inf (not to be taken), all ones NaN
 __device__ __forceinline__ uint32_t ordered(float x) {
-  if (x != x) return 0xffffffffu;
   const uint32_t b = __float_as_uint(x + 0.0f);  // -0 is 0
-  return x == -__builtin_inff() ? 0u : b & 0x80000000u ? ~b : b | 0x80000000u;
+  uint32_t k = b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+  k = x == -__builtin_inff() ? 0u : k;
+  return x != x ? 0xffffffffu : k;
 }
 __device__ __forceinline__ float unordered(uint32_t k) {
   return k == 0u ? -__builtin_inff() : k == 0xffffffffu ? __builtin_nanf("") : __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 __device__ __forceinline__ uint64_t ordered(double x) {
-  if (x != x) return ~0ull;
   const uint64_t b = __builtin_bit_cast(uint64_t, x + 0.0);
-  return x == -__builtin_inf() ? 0ull : b >> 63 ? ~b : b | 0x8000000000000000ull;
+  uint64_t k = b ^ ((uint64_t)((int64_t)b >> 63) | 0x8000000000000000ull);
+  k = x == -__builtin_inf() ? 0ull : k;
+  return x != x ? ~0ull : k;
 }
 __device__ __forceinline__ double unordered(uint64_t k) {
   return k == 0ull ? -__builtin_inf() : k == ~0ull ? __builtin_nan("") : __builtin_bit_cast(double, k >> 63 ? k & 0x7fffffffffffffffull : ~k);
@@ -87,6 +91,36 @@ __device__ __forceinline__ U lanes_reduce(U v, int lanes, F f) {
   return v;
 }
 
+// The largest of a wave's unsigned numbers, a scalar: inside rows of 16 lanes, then the four rows.
+__device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
+  v = lanes_reduce<16>(v, 16, [](uint32_t p, uint32_t q) { return umax32(p, q); });
+  const uint32_t a = (uint32_t)__builtin_amdgcn_readlane((int)v, 0), b = (uint32_t)__builtin_amdgcn_readlane((int)v, 16);
+  const uint32_t c = (uint32_t)__builtin_amdgcn_readlane((int)v, 32), d = (uint32_t)__builtin_amdgcn_readlane((int)v, 48);
+  return umax32(umax32(a, b), umax32(c, d));
+}
+// The largest key of the L lanes of a token and the lowest expert that has it, from each lane's largest key m and its expert e; experts rise with
+// the lanes.  64-bit keys: the high words first, the low ones of those that share it.
+template <int L, typename Key>
+__device__ __forceinline__ Key choose(Key m, int e, int &taken) {
+  if constexpr (L == 64) {
+    const uint32_t hi = sizeof(Key) == 8 ? (uint32_t)((uint64_t)m >> 32) : (uint32_t)m;
+    const uint32_t most = wave_umax(hi);
+    uint64_t lanes = __ballot(hi == most);
+    if constexpr (sizeof(Key) == 8) {
+      if (lanes & (lanes - 1)) {
+        const uint32_t lo = hi == most ? (uint32_t)m : 0u;
+        lanes &= __ballot(lo == wave_umax(lo));
+      }
+    }
+    taken = __builtin_amdgcn_readlane(e, __builtin_ctzll(lanes));
+    return most;  // (of 64 bits the high ones: they are 0 for no allowed key)
+  } else {
+    const Key most = lanes_reduce<L>(m, L, [](Key p, Key q) { return p > q ? p : q; });
+    taken = lanes_reduce<L>(m == most ? e : 0x7fffffff, L, [](int p, int q) { return p < q ? p : q; });
+    return most;
+  }
+}
+
 // One token on L lanes, PER experts each, the experts of a group in neighbouring lanes.  Lane s < k returns the token's s-th expert (-1: none) and its weight.
 // All lanes of the wave take part; `valid` false: a token behind the last one.
 template <int DT, int L, int PER, bool WIDE>
@@ -97,8 +131,22 @@ __device__ __forceinline__ void route_token(const RouteArgs &a, int64_t token, b
   const int lg = L == 64 ? a.group_lanes : L;  // (fewer lanes have one group)
   const int group = L == 64 ? sub / lg : 0, at = (sub - group * lg) * PER, e0 = group * a.group_size + at;
   float x[PER];
+  const int here = valid && group < a.groups ? a.group_size - at : 0;
+  if (here >= PER) {
+    typedef T Run __attribute__((ext_vector_type(PER)));
+    typedef Run RunElem __attribute__((aligned(sizeof(T))));  // global memory takes vector accesses at any address
+    Run v;
+    if constexpr (PER > 1) v = *reinterpret_cast<const RunElem *>(row + e0);
+    else v[0] = row[e0];
 #pragma unroll
-  for (int j = 0; j < PER; ++j) x[j] = valid && group < a.groups && at + j < a.group_size ? Elem<DT>::load(row, e0 + j) : -__builtin_inff();
+    for (int j = 0; j < PER; ++j) {
+      const T one = v[j];
+      x[j] = Elem<DT>::load(&one, 0);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) x[j] = j < here ? Elem<DT>::load(row, e0 + j) : -__builtin_inff();
+  }
   auto larger = [](Key p, Key q) { return p > q ? p : q; };
   auto add = [](double p, double q) { return p + q; };
   Key key[PER];
@@ -118,19 +166,19 @@ __device__ __forceinline__ void route_token(const RouteArgs &a, int64_t token, b
       sum = 0.0;
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
-        score[j] = x[j] == -__builtin_inff() ? 0.0 : exp((double)x[j] - (double)top);
+        score[j] = exp(x[j] == -__builtin_inff() ? -1000.0 : (double)x[j] - (double)top);  // (0 for an expert that is not allowed)
         sum += score[j];
       }
       sum = lanes_reduce<L>(sum, L, add);
+      const double share = 1.0 / sum;
 #pragma unroll
-      for (int j = 0; j < PER; ++j) score[j] /= sum;
+      for (int j = 0; j < PER; ++j) score[j] *= share;
     }
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      const bool allowed = x[j] != -__builtin_inff();
-      double v = score[j];
-      if (a.bias && allowed) v += (double)a.bias[e0 + j];
-      key[j] = allowed ? ordered(v) : 0;
+      const int e = e0 + j < a.E ? e0 + j : a.E - 1;
+      const double v = a.bias ? score[j] + (double)a.bias[e] : score[j];
+      key[j] = x[j] != -__builtin_inff() ? ordered(v) : 0;
     }
   } else {
     Key m = 0;
@@ -185,27 +233,43 @@ __device__ __forceinline__ void route_token(const RouteArgs &a, int64_t token, b
     }
   }
   my_expert = -1;
+  float my_logit = 0.0f;
   for (int s = 0; s < a.k; ++s) {
     Key m;
     int e;
     best_of(key, m, e);
-    const Key most = lanes_reduce<L>(m, L, larger);
-    const int taken = lanes_reduce<L>(m == most ? e : 0x7fffffff, L, [](int p, int q) { return p < q ? p : q; });
+    int taken;
+    const Key most = choose<L>(m, e, taken);
 #pragma unroll
     for (int j = 0; j < PER; ++j)
       if (e0 + j == taken) key[j] = 0;
-    if (sub == s && most != 0) my_expert = taken;
+    if (sub == s && most != 0) {
+      my_expert = taken;
+      if constexpr (!WIDE) my_logit = unordered(most);
+    }
   }
   double w = 0.0;
   if (my_expert >= 0) {
-    const double v = (double)Elem<DT>::load(row, my_expert);
-    w = a.sigmoid ? 1.0 / (1.0 + exp(-v)) : exp(v - (double)top) / sum;
+    if constexpr (WIDE) my_logit = Elem<DT>::load(row, my_expert);
+    const double v = (double)my_logit;
+    const double power = exp(a.sigmoid ? -v : v - (double)top);
+    w = a.sigmoid ? 1.0 / (1.0 + power) : power / sum;
   }
   if (a.renormalize) {
     const double all = lanes_reduce<L>(w, L, add);
     w = all == 0.0 ? 0.0 : w / all;
   }
   my_weight = (float)(w * a.scale);
+}
+
+__device__ __forceinline__ int wave_prefix(int v) {  // inclusive: inside rows of 16 lanes, then the last lane of a row to those behind it
+  v += (int)dpp_u32<DPP_ROW_SHR(1)>((uint32_t)v);
+  v += (int)dpp_u32<DPP_ROW_SHR(2)>((uint32_t)v);
+  v += (int)dpp_u32<DPP_ROW_SHR(4)>((uint32_t)v);
+  v += (int)dpp_u32<DPP_ROW_SHR(8)>((uint32_t)v);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15 to rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31 to rows 2 and 3
+  return v;
 }
 
 // The places of a block's tokens: `base` rows of expert e in front of the block (its range's start among them)
@@ -232,12 +296,7 @@ __device__ __forceinline__ int route_starts(int *count, int E, int *wave_sum) {
     c[j] = e < E ? count[e] : 0;
     sum += c[j];
   }
-  int before = sum;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const int v = __shfl_up(before, d);
-    if (lane >= d) before += v;
-  }
+  int before = wave_prefix(sum);
   if (lane == 63) wave_sum[wave] = before;
   __syncthreads();
   int total = 0;
@@ -259,27 +318,23 @@ __device__ __forceinline__ int route_starts(int *count, int E, int *wave_sum) {
 
 // Scores, choice and weights of a block's tokens and the sets of its experts
 template <int DT, int L, int PER, bool WIDE>
-__global__ __launch_bounds__(256) void route_kernel(RouteArgs a) {
+__global__ __launch_bounds__(ROUTE_TOKENS * L) void route_kernel(RouteArgs a) {
   __shared__ uint32_t mask[AC4K_ROUTE_MAX_EXPERTS];
-  constexpr int AT_ONCE = 256 / L;
-  const int tid = threadIdx.x, sub = tid % L;
-  for (int e = tid; e < a.E; e += 256) mask[e] = 0;
+  constexpr int THREADS = ROUTE_TOKENS * L;
+  const int tid = threadIdx.x, sub = tid % L, b = tid / L;
+  for (int e = tid; e < a.Ep; e += THREADS) mask[e] = 0;
   __syncthreads();
-  const int64_t t0 = (int64_t)blockIdx.x * ROUTE_TOKENS;
-#pragma unroll 1
-  for (int b = tid / L; b < ROUTE_TOKENS; b += AT_ONCE) {
-    const int64_t t = t0 + b;
-    int e;
-    float w;
-    route_token<DT, L, PER, WIDE>(a, t, t < a.T, sub, e, w);
-    if (t < a.T && sub < a.k) {
-      a.experts[t * a.k + sub] = e;
-      a.weights[t * a.k + sub] = w;
-      if (e >= 0) atomicOr(&mask[e], 1u << b);
-    }
+  const int64_t t = (int64_t)blockIdx.x * ROUTE_TOKENS + b;
+  int e;
+  float w;
+  route_token<DT, L, PER, WIDE>(a, t, t < a.T, sub, e, w);
+  if (t < a.T && sub < a.k) {
+    a.experts[t * a.k + sub] = e;
+    a.weights[t * a.k + sub] = w;
+    if (e >= 0) atomicOr(&mask[e], 1u << b);
   }
   __syncthreads();
-  for (int e = tid; e < a.E; e += 256) a.masks[(int64_t)blockIdx.x * a.E + e] = (uint16_t)mask[e];
+  for (int e = tid; e < a.Ep; e += THREADS) a.masks[(int64_t)blockIdx.x * a.Ep + e] = (uint16_t)mask[e];
 }
 
 // Counts of each expert in the blocks in front of each block: 64 runs of blocks and 16 experts a workgroup
@@ -291,7 +346,7 @@ __global__ __launch_bounds__(64 * ROUTE_SCAN_EXPERTS) void route_scan_kernel(Rou
   int sum = 0;
   if (e < a.E) {
 #pragma unroll 8
-    for (int64_t b = b0; b < b1; ++b) sum += __popc((uint32_t)a.masks[b * a.E + e]);
+    for (int64_t b = b0; b < b1; ++b) sum += __popc((uint32_t)a.masks[b * a.Ep + e]);
   }
   part[run][x] = sum;
   __syncthreads();
@@ -302,7 +357,7 @@ __global__ __launch_bounds__(64 * ROUTE_SCAN_EXPERTS) void route_scan_kernel(Rou
 #pragma unroll 8
   for (int64_t b = b0; b < b1; ++b) {
     a.bases[b * a.E + e] = before;
-    before += __popc((uint32_t)a.masks[b * a.E + e]);
+    before += __popc((uint32_t)a.masks[b * a.Ep + e]);
   }
 }
 
@@ -319,31 +374,123 @@ __global__ __launch_bounds__(256) void route_place_kernel(RouteArgs a) {
   }
   const int64_t t0 = (int64_t)blockIdx.x * ROUTE_TOKENS;
   const int here = (int)(a.T - t0 < ROUTE_TOKENS ? a.T - t0 : ROUTE_TOKENS) * a.k;
-  const int64_t row = (int64_t)blockIdx.x * a.E;
+  const int64_t row = (int64_t)blockIdx.x * a.E, mask_row = (int64_t)blockIdx.x * a.Ep;
   for (int i = tid; i < here; i += 256) {
     const int b = i / a.k, slot = i - b * a.k;
     const int e = a.experts[t0 * a.k + i];
-    route_place(a, t0 + b, slot, e, e >= 0 ? a.masks[row + e] : 0, b, [&](int x) { return start[x] + a.bases[row + x]; });
+    route_place(a, t0 + b, slot, e, e >= 0 ? a.masks[mask_row + e] : 0, b, [&](int x) { return start[x] + a.bases[row + x]; });
     if (t0 * a.k + i >= total) a.rows[t0 * a.k + i] = -1;
   }
 }
 
+// The same in one launch where there are few masks: every workgroup counts all of them itself and places the tokens of ROUTE_PLAN_BLOCKS
+// blocks.  A thread counts eight experts in every runs-th block; a thread's counts are under 2^16 (16 tokens a mask, at most 2^25 masks in all workgroups),
+// and the runs' counts meet as pairs.  (By an atomic add for each thread and expert the launch took 8.5 us at 16384 x 128.)
+__global__ __launch_bounds__(1024) void route_plan_kernel(RouteArgs a) {
+  constexpr int THREADS = 1024;
+  __shared__ int total[AC4K_ROUTE_MAX_EXPERTS];   // rows of the expert, then the start of its range
+  __shared__ int before[AC4K_ROUTE_MAX_EXPERTS];  // of them, in front of this workgroup's blocks
+  __shared__ uint16_t base[ROUTE_PLAN_BLOCKS][AC4K_ROUTE_MAX_EXPERTS], mask[ROUTE_PLAN_BLOCKS][AC4K_ROUTE_MAX_EXPERTS];
+  __shared__ uint32_t part[2][THREADS * 4];       // [run][pair of experts]
+  __shared__ int wave_sum[THREADS / 64];
+  const int tid = threadIdx.x, E = a.E, columns = a.Ep / 8, runs = THREADS / columns, pairs = columns * 4;
+  const int64_t b0 = (int64_t)blockIdx.x * ROUTE_PLAN_BLOCKS;
+  const int mine = (int)(a.blocks - b0 < ROUTE_PLAN_BLOCKS ? a.blocks - b0 : ROUTE_PLAN_BLOCKS);
+  // the experts of the first slots are under way while the masks are counted
+  const int64_t t0 = b0 * ROUTE_TOKENS;
+  const int slots = (int)(a.T - t0 < ROUTE_PLAN_BLOCKS * ROUTE_TOKENS ? a.T - t0 : ROUTE_PLAN_BLOCKS * ROUTE_TOKENS) * a.k;
+  int expert[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) expert[i] = tid + i * THREADS < slots ? a.experts[t0 * a.k + tid + i * THREADS] : -1;
+  for (int e = tid; e < E; e += THREADS) total[e] = before[e] = 0;
+  for (int b = tid >> 6; b < mine; b += THREADS / 64)
+    for (int e = tid & 63; e < E; e += 64) mask[b][e] = a.masks[(b0 + b) * a.Ep + e];
+  const int run = tid / columns, column = tid - run * columns;
+  if (run < runs) {
+    int all[8] = {}, front[8] = {};
+    constexpr int CHUNK = 8;  // loads under way at once: the masks come from other XCDs, a microsecond away
+    for (int64_t b = run; b < a.blocks; b += CHUNK * runs) {
+      u32x4 v[CHUNK];
+#pragma unroll
+      for (int c = 0; c < CHUNK; ++c) {
+        const int64_t at = b + c * runs;
+        v[c] = at < a.blocks ? *reinterpret_cast<const u32x4 *>(a.masks + at * a.Ep + column * 8) : (u32x4){0, 0, 0, 0};
+      }
+#pragma unroll
+      for (int c = 0; c < CHUNK; ++c) {
+        const u32x4 f = b + c * runs < b0 ? v[c] : (u32x4){0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          all[i] += __popc(i & 1 ? v[c][i / 2] >> 16 : v[c][i / 2] & 0xffffu);
+          front[i] += __popc(i & 1 ? f[i / 2] >> 16 : f[i / 2] & 0xffffu);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      part[0][run * pairs + column * 4 + i] = (uint32_t)(front[2 * i] | front[2 * i + 1] << 16);
+      part[1][run * pairs + column * 4 + i] = (uint32_t)(all[2 * i] | all[2 * i + 1] << 16);
+    }
+  }
+  __syncthreads();
+  {
+    const int shares = THREADS / pairs, share = tid / pairs, pair = tid - share * pairs;
+    if (share < shares) {
+      uint32_t f0 = 0, f1 = 0, t0 = 0, t1 = 0;
+      for (int r = share; r < runs; r += shares) {
+        const uint32_t f = part[0][r * pairs + pair], t = part[1][r * pairs + pair];
+        f0 += f & 0xffffu, f1 += f >> 16, t0 += t & 0xffffu, t1 += t >> 16;
+      }
+      if (2 * pair < E) {
+        atomicAdd(&before[2 * pair], (int)f0);
+        atomicAdd(&total[2 * pair], (int)t0);
+      }
+      if (2 * pair + 1 < E) {
+        atomicAdd(&before[2 * pair + 1], (int)f1);
+        atomicAdd(&total[2 * pair + 1], (int)t1);
+      }
+    }
+  }
+  for (int e = tid; e < E; e += THREADS) {
+    int sum = 0, m[ROUTE_PLAN_BLOCKS];
+#pragma unroll
+    for (int b = 0; b < ROUTE_PLAN_BLOCKS; ++b) m[b] = b < mine ? mask[b][e] : 0;
+#pragma unroll
+    for (int b = 0; b < ROUTE_PLAN_BLOCKS; ++b) {
+      base[b][e] = (uint16_t)sum;
+      sum += __popc((uint32_t)m[b]);
+    }
+  }
+  __syncthreads();
+  const int rows = route_starts<THREADS>(total, E, wave_sum);
+  if (blockIdx.x == 0) {
+    for (int e = tid; e < E; e += THREADS) a.offsets[e] = total[e];
+    if (tid == 0) a.offsets[E] = rows;
+  }
+  for (int i = tid, n = 0; i < slots; i += THREADS, ++n) {
+    const int t = i / a.k, slot = i - t * a.k, b = t / ROUTE_TOKENS;
+    const int e = n == 0 ? expert[0] : n == 1 ? expert[1] : a.experts[t0 * a.k + i];
+    route_place(a, t0 + t, slot, e, e >= 0 ? mask[b][e] : 0, t % ROUTE_TOKENS, [&](int x) { return total[x] + before[x] + base[b][x]; });
+    if (t0 * a.k + i >= rows) a.rows[t0 * a.k + i] = -1;
+  }
+}
+
 // All of a small call in one workgroup
-template <int DT, int L, int PER, bool WIDE>
-__global__ __launch_bounds__(1024) void route_one_kernel(RouteArgs a) {
+template <int DT, int L, int PER, bool WIDE, int THREADS>
+__global__ __launch_bounds__(THREADS) void route_one_kernel(RouteArgs a) {
   __shared__ unsigned long long mask[AC4K_ROUTE_MAX_EXPERTS];
   __shared__ int start[AC4K_ROUTE_MAX_EXPERTS];
-  __shared__ int wave_sum[16];
-  constexpr int AT_ONCE = 1024 / L, TURNS = ROUTE_ONE_TOKENS / AT_ONCE;
+  __shared__ int wave_sum[THREADS / 64];
+  constexpr int AT_ONCE = THREADS / L, TURNS = THREADS == 256 ? 1 : ROUTE_ONE_TOKENS / AT_ONCE;
   const int tid = threadIdx.x, sub = tid % L;
-  for (int e = tid; e < a.E; e += 1024) mask[e] = 0;
+  for (int e = tid; e < a.E; e += THREADS) mask[e] = 0;
   __syncthreads();
   int mine[TURNS];
 #pragma unroll
   for (int i = 0; i < TURNS; ++i) {
     const int t = i * AT_ONCE + tid / L;
     mine[i] = -1;
-    if (i * AT_ONCE >= a.T) continue;
+    if (i * AT_ONCE + (tid & ~63) / L >= a.T) continue;  // a whole wave
     float w;
     route_token<DT, L, PER, WIDE>(a, t, t < a.T, sub, mine[i], w);
     if (t < a.T && sub < a.k) {
@@ -353,26 +500,32 @@ __global__ __launch_bounds__(1024) void route_one_kernel(RouteArgs a) {
     }
   }
   __syncthreads();
-  for (int e = tid; e < a.E; e += 1024) start[e] = __popcll(mask[e]);
+  for (int e = tid; e < a.E; e += THREADS) start[e] = __popcll(mask[e]);
   __syncthreads();
-  const int total = route_starts<1024>(start, a.E, wave_sum);
-  for (int e = tid; e < a.E; e += 1024) a.offsets[e] = start[e];
+  const int total = route_starts<THREADS>(start, a.E, wave_sum);
+  for (int e = tid; e < a.E; e += THREADS) a.offsets[e] = start[e];
   if (tid == 0) a.offsets[a.E] = total;
 #pragma unroll
   for (int i = 0; i < TURNS; ++i) {
     const int t = i * AT_ONCE + tid / L;
     if (t < a.T && sub < a.k) route_place(a, t, sub, mine[i], mine[i] >= 0 ? mask[mine[i]] : 0, t, [&](int x) { return start[x]; });
   }
-  for (int i = total + tid; i < a.T * a.k; i += 1024) a.rows[i] = -1;
+  for (int i = total + tid; i < a.T * a.k; i += THREADS) a.rows[i] = -1;
 }
 
 template <int DT, int L, int PER, bool WIDE>
 static void launch_route(const RouteArgs &a, hipStream_t st) {
   if (a.T <= ROUTE_ONE_TOKENS) {
-    hipLaunchKernelGGL((route_one_kernel<DT, L, PER, WIDE>), dim3(1), dim3(1024), 0, st, a);
+    if (a.T * L <= 256) hipLaunchKernelGGL((route_one_kernel<DT, L, PER, WIDE, 256>), dim3(1), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((route_one_kernel<DT, L, PER, WIDE, 1024>), dim3(1), dim3(1024), 0, st, a);
     return;
   }
-  hipLaunchKernelGGL((route_kernel<DT, L, PER, WIDE>), dim3((unsigned)a.blocks), dim3(256), 0, st, a);
+  hipLaunchKernelGGL((route_kernel<DT, L, PER, WIDE>), dim3((unsigned)a.blocks), dim3(ROUTE_TOKENS * L), 0, st, a);
+  const int64_t groups = ceil_div(a.blocks, ROUTE_PLAN_BLOCKS);
+  if (groups * a.blocks * a.E <= ROUTE_PLAN_MASKS) {
+    hipLaunchKernelGGL(route_plan_kernel, dim3((unsigned)groups), dim3(1024), 0, st, a);
+    return;
+  }
   hipLaunchKernelGGL(route_scan_kernel, dim3((unsigned)ceil_div(a.E, ROUTE_SCAN_EXPERTS)), dim3(64 * ROUTE_SCAN_EXPERTS), 0, st, a);
   hipLaunchKernelGGL(route_place_kernel, dim3((unsigned)a.blocks), dim3(256), 0, st, a);
 }
@@ -406,7 +559,7 @@ static int route_width(const RouteArgs &a, hipStream_t st) {
 static int64_t route_workspace(int64_t T, int64_t E) {
   if (T <= ROUTE_ONE_TOKENS) return 0;
   const int64_t blocks = ceil_div(T, ROUTE_TOKENS);
-  return 4 * align_up(E, 4) + 4 * align_up(blocks * E, 4) + 2 * blocks * E;
+  return 4 * align_up(E, 4) + 4 * align_up(blocks * E, 4) + 2 * blocks * align_up(E, 8);
 }
 
 // ---------------------------------------------------------------------------
@@ -421,7 +574,7 @@ struct CombineArgs {
   int k;
 };
 
-// A thread takes eight columns of a token; its places and weights are scalars of the wave.  Rows are read four at a time.
+// A thread takes eight columns of a token; its places and weights are scalars of the wave.  Rows are read eight at a time.
 template <int DT>
 __global__ __launch_bounds__(256) void combine_kernel(CombineArgs a, uint32_t spans) {
   using T = typename Elem<DT>::T;
@@ -437,19 +590,19 @@ __global__ __launch_bounds__(256) void combine_kernel(CombineArgs a, uint32_t sp
 #pragma unroll
     for (int i = 0; i < 8; ++i) sum[i] = vec8_get(r, i);
   }
-  for (int s0 = 0; s0 < a.k; s0 += 4) {
-    Vec8<DT> v[4];
-    float w[4];
-    bool here[4];
+  for (int s0 = 0; s0 < a.k; s0 += 8) {
+    Vec8<DT> v[8];
+    float w[8];
+    bool here[8];
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
+    for (int s = 0; s < 8; ++s) {
       const int64_t place = s0 + s < a.k ? places[s0 + s] : -1;
       here[s] = place >= 0 && place < a.M;
       w[s] = here[s] ? weights[s0 + s] : 0.0f;
       if (here[s]) vec8_load(v[s], static_cast<const T *>(a.y) + place * a.y_stride, c, a.N);
     }
 #pragma unroll
-    for (int s = 0; s < 4; ++s)
+    for (int s = 0; s < 8; ++s)
       if (here[s]) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) sum[i] = __builtin_fmaf(vec8_get(v[s], i), w[s], sum[i]);
@@ -485,12 +638,12 @@ extern "C" __attribute__((visibility("default"))) int ac4k_route_experts(
   AC4K_REQUIRE(best == 1 || best == 2, "a group's score is that of its best one or two, not %d", best);
   AC4K_REQUIRE(k >= 1 && k <= AC4K_ROUTE_MAX_K && k <= E / groups * top_groups, "k must be 1 to %d and at most the %lld experts of the groups taken, got %lld",
                (int)AC4K_ROUTE_MAX_K, (long long)(E / groups * top_groups), (long long)k);
-  AC4K_REQUIRE(T * k < (1ll << 27) && T < (1ll << 27), "too many tokens (%lld of %lld experts)", (long long)T, (long long)k);
+  AC4K_REQUIRE(T * k < (1ll << 27) && T < (1ll << 26), "too many tokens (%lld of %lld experts)", (long long)T, (long long)k);
   const int64_t need = route_workspace(T, E);
-  AC4K_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 3) == 0), "workspace of %lld bytes needed, on 4 bytes", (long long)need);
+  AC4K_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0), "workspace of %lld bytes needed, on 16 bytes", (long long)need);
   RouteArgs a{};
   a.logits = logits, a.stride = stride, a.bias = bias, a.weights = weights, a.experts = experts, a.offsets = offsets, a.rows = rows, a.places = places;
-  a.T = T, a.blocks = ceil_div(T, ROUTE_TOKENS), a.E = (int)E, a.k = (int)k;
+  a.T = T, a.blocks = ceil_div(T, ROUTE_TOKENS), a.E = (int)E, a.Ep = (int)align_up(E, 8), a.k = (int)k;
   a.groups = (int)(top_groups == groups ? 1 : groups), a.top_groups = (int)top_groups, a.best = best, a.group_size = (int)(E / a.groups);
   a.sigmoid = scoring == AC4K_SCORE_SIGMOID, a.renormalize = renormalize != 0, a.scale = scale;
   a.totals = static_cast<int32_t *>(workspace);

@@ -27,23 +27,9 @@ def route_experts(logits, top_k, scoring="softmax", bias=None, groups=1, top_gro
     if view is None:
         logits = logits.contiguous()
         view = _rocm_ops._rows_view(logits, "logits")
-    tokens, experts, _ = view
-    top_k, groups, group_best = int(top_k), int(groups), int(group_best)
-    top_groups = groups if top_groups is None else int(top_groups)
-    if experts > 1024:
-        raise RuntimeError(f"at most 1024 experts, got {experts}")
-    if not 1 <= groups <= 64 or experts % groups or not 1 <= top_groups <= groups or group_best not in (1, 2):
-        raise RuntimeError(f"groups must be 1 to 64 and divide the {experts} experts, top_groups 1 to groups, group_best 1 or 2")
-    if not 1 <= top_k <= min(64, experts // groups * top_groups):
-        raise RuntimeError(f"top_k must be 1 to 64 and at most the {experts // groups * top_groups} experts of the groups taken, got {top_k}")
-    lead = logits.shape[:-1]
-    weights = logits.new_empty((*lead, top_k), dtype=torch.float32)
-    chosen = logits.new_empty((*lead, top_k), dtype=torch.int32)
-    offsets = logits.new_empty((experts + 1,), dtype=torch.int32)
-    rows = logits.new_empty((tokens * top_k,), dtype=torch.int32)
-    places = logits.new_empty((*lead, top_k), dtype=torch.int32)
-    _rocm_ops.route_experts(weights, chosen, offsets, rows, places, logits, bias, scoring, groups, top_groups, group_best, renormalize, float(scale), view)
-    return weights, chosen, offsets, rows, places
+    groups = int(groups)
+    return _rocm_ops.route_experts(logits, int(top_k), bias, scoring, groups, groups if top_groups is None else int(top_groups), int(group_best), renormalize,
+                                   float(scale), view)
 
 
 def combine_experts(y, weights, places, residual=None, out=None):
@@ -61,8 +47,4 @@ def combine_experts(y, weights, places, residual=None, out=None):
         if out is residual:
             raise RuntimeError("out must have rows of contiguous elements, evenly apart")
         residual = residual.contiguous()
-    fresh = out is None
-    if fresh:
-        out = y.new_empty((*places.shape[:-1], y.shape[1]))
-    _rocm_ops.combine_experts(out, y, weights, places, residual, fresh)
-    return out
+    return _rocm_ops.combine_experts(out, y, weights, places, residual)

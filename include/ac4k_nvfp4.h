@@ -399,7 +399,7 @@ int ac4k_debug_last_grouped_kernel(void);
  *   offsets int32 [E + 1]: range of rows of each expert, in it the tokens in rising order;  rows int32 [T * k]: the token of each row, -1 from offsets[E] on;
  *   places int32 [T, k]: the row of each slot.
  * Without a bias and with best == 1, logits are compared as they are; otherwise keys in 64 bits.  Every call gives the same results again.
- * `workspace`: ac4k_route_experts_workspace_bytes(T, E, k), on 4 bytes, contents irrelevant, NULL when that is 0. */
+ * `workspace`: ac4k_route_experts_workspace_bytes(T, E, k), on 16 bytes, contents irrelevant, NULL when that is 0. */
 enum { AC4K_SCORE_SOFTMAX = 0, AC4K_SCORE_SIGMOID = 1 };
 #define AC4K_ROUTE_MAX_EXPERTS 1024
 #define AC4K_ROUTE_MAX_K 64
