@@ -903,3 +903,124 @@ def combine_experts(out, y, weights, places, residual=None):
         _lib.check(_L.ac4k_combine_experts(out.data_ptr(), out_step, y.data_ptr(), y_step, weights.data_ptr(), places.data_ptr(), residual_ptr, residual_step,
                                            T, k, M, N, tag, _stream()))
     return out
+
+
+_KINDS = {"rms": 0, "layer": 1}
+
+
+def _norm_vector(t, name: str, shape, tag: int, dev):
+    """(address, elements between vectors, rows that share one; 0: all) of one of a block's vectors, [K] or with leading dims that are those of x or,
+    from some dim on, 1."""
+    if t is None:
+        return None, 0, 0
+    _check(t.get_device() == dev, "{} must be on the current device", name)
+    *lead, K = t.shape
+    x_lead = shape[:-1]
+    if K != shape[-1]:
+        _check(False, "{} must have a last dim of {}", name, shape[-1])
+    count = 1
+    for n in lead:
+        count *= n
+    if count == 1 and (len(lead) == len(x_lead) or len(lead) == 0):
+        _check(K == 1 or t.stride(-1) == 1, "{} must have contiguous vectors, evenly apart", name)
+        return t.data_ptr(), 0, 0
+    rows, same = 1, len(x_lead)
+    if len(lead) == len(x_lead):
+        while same and lead[same - 1] == 1:
+            same -= 1
+            rows *= x_lead[same]
+    _check(len(lead) == len(x_lead) and tuple(lead[:same]) == tuple(x_lead[:same]), "{} must be [{}], or have the leading dims of x or 1 from some dim on, not {}", name,
+           K, list(t.shape))
+    v = _rows_view(t, name)
+    _check(v is not None, "{} must have contiguous vectors, evenly apart", name)
+    return t.data_ptr(), v[2], rows
+
+
+def block_norm(out, sf, global_scale, given_scale: bool, x, residual, residual_out, weight, post_weight, gate, scale, shift, kind, residual_scale: float,
+               precision, eps: float, view=None, fresh=False) -> None:
+    """out (and sf, global_scale) <- norm and modulation of the rows of x, or of residual_scale * residual + gate * (norm of x * post_weight), which residual_out
+    receives.  view: _rows_view(x), where the caller has it; fresh: out, sf and residual_out are new dense tensors of the right shapes and overlap nothing."""
+    tag = _check_float(x, "x")
+    view = view or _rows_view(x, "x")
+    _check(view is not None, "x must have rows of contiguous elements, evenly apart")
+    rows, K, x_step = view
+    number, kind_number = _PRECISIONS.get(precision), _KINDS.get(kind)
+    if number is None or kind_number is None:
+        _check(number is not None, "precision must be one of {}", list(_PRECISIONS))
+        _check(False, "kind must be one of {}", list(_KINDS))
+    if global_scale is not None:
+        _check_tensor(global_scale, torch.float32, "global_scale")
+        _check(global_scale.dim() == 0, "global_scale must be a scalar")
+    dev = _current_device()
+    if x.get_device() != dev or not fresh or global_scale is not None:
+        _same_device(x, residual_out, out, sf, global_scale)
+    if (residual is None) != (residual_out is None):
+        _check(False, "a residual comes with residual_out, and the other way round")
+    vector_tag = None
+    vectors = (("weight", weight), ("post_weight", post_weight), ("gate", gate), ("scale", scale), ("shift", shift))
+    for name, t in vectors:
+        if t is not None:
+            t_tag = _check_float(t, name)
+            if t_tag != tag and t_tag != 2 or vector_tag not in (None, t_tag):
+                _check(t_tag == tag or t_tag == 2, "{} must have the type of x or be float", name)
+                _check(False, "weight, post_weight, gate, scale and shift must have one type")
+            vector_tag = t_tag
+    for name, t in vectors[:2]:
+        if t is not None and (t.shape != (K,) or not t.is_contiguous() or t.get_device() != dev):
+            _same_device(t)
+            _check(False, "{} must be contiguous of [{}]", name, K)
+    shape = x.shape
+    gate_at, scale_at, shift_at = _norm_vector(gate, "gate", shape, tag, dev), _norm_vector(scale, "scale", shape, tag, dev), _norm_vector(shift, "shift", shape, tag, dev)
+    residual_ptr = sum_ptr = None
+    residual_step = sum_step = 0
+    if residual is not None:
+        if _check_float(residual, "residual") != tag or residual.shape != shape or residual.get_device() != dev:
+            _same_device(residual)
+            _check(False, "residual must have the type and shape of x")
+        v = _rows_view(residual, "residual")
+        if v is None:
+            _check(False, "residual must have rows of contiguous elements, evenly apart")
+        residual_ptr, residual_step, sum_ptr, sum_step = residual.data_ptr(), v[2], residual_out.data_ptr(), K
+        if not fresh:
+            _check(_check_float(residual_out, "residual_out") == tag and residual_out.shape == shape, "residual_out must have the type and shape of x")
+            v = _rows_view(residual_out, "residual_out")
+            _check(v is not None and (rows <= 1 or v[2] >= K), "residual_out must have rows of contiguous elements, evenly apart")
+            sum_step = v[2]
+            for t in (x, residual):
+                _check(_same_rows(t, residual_out) or not _may_overlap(t, residual_out),
+                       "residual_out may be x or residual itself, but not overlap them otherwise")
+            for t in (weight, post_weight, gate, scale, shift, global_scale):
+                _check(t is None or not _may_overlap(t, residual_out), "residual_out must not overlap a vector or global_scale")
+    elif gate is not None or post_weight is not None:
+        _check(False, "a gate or a post_weight comes with a residual")
+    out_step = K
+    if not fresh:
+        if precision is None:
+            _check(_check_float(out, "out") == tag and out.shape == shape, "out must have the type and shape of x")
+            v = _rows_view(out, "out")
+            _check(v is not None and (rows <= 1 or v[2] >= K), "out must have rows of contiguous elements, evenly apart")
+            out_step = v[2]
+            _check(_same_rows(out, x) or not _may_overlap(out, x), "out may be x itself, but not overlap it otherwise")
+            for t in (residual, residual_out, weight, post_weight, gate, scale, shift):
+                _check(t is None or not _may_overlap(out, t), "out must not overlap residual, residual_out or a vector")
+        else:
+            nvfp4 = precision == "nvfp4"
+            _check_tensor(out, torch.uint8 if nvfp4 else torch.float8_e4m3fn if precision == "fp8e4m3" else torch.int8, "out")
+            _check(list(out.shape) == [rows, _align_up(K, 64) // 2 if nvfp4 else _align_up(K, 16)], "meet invalid out shape")
+            _check_tensor(sf, torch.float8_e4m3fn if nvfp4 else torch.float32, "sf")
+            _check(list(sf.shape) == ([_align_up(K, 64) // 64, _align_up(rows, 16), 4] if nvfp4 else [_align_up(rows, 16)]), "meet invalid sf shape")
+    if rows == 0:
+        if global_scale is not None and not given_scale:
+            global_scale.zero_()  # that of a tensor of zeros
+        return
+    ws_ptr, nbytes = None, 0
+    if number == 3 and not given_scale:
+        nbytes = _L.ac4k_block_norm_workspace_bytes(rows, K, tag, number, 0)
+        if nbytes > 0:
+            ws = x.new_empty((nbytes,), dtype=torch.uint8)
+            ws_ptr = ws.data_ptr()
+    _lib.check(_L.ac4k_block_norm(out.data_ptr(), out_step, None if sf is None else sf.data_ptr(), None if global_scale is None else global_scale.data_ptr(),
+                                  int(given_scale), x.data_ptr(), x_step, residual_ptr, residual_step, sum_ptr, sum_step,
+                                  None if weight is None else weight.data_ptr(), None if post_weight is None else post_weight.data_ptr(), *gate_at, *scale_at,
+                                  *shift_at, tag if vector_tag is None else vector_tag, rows, K, tag, number, kind_number, residual_scale, eps, ws_ptr, nbytes,
+                                  _stream()))

@@ -5,7 +5,7 @@ quantized output, linears grouped by expert.  The sparse-attention operator of t
 from .attention import attention, mha_int8_x_fp8_fwd, mha_nvfp4_fwd
 from .experts import combine_experts, route_experts
 from .linear import fused_linear, grouped_linear, linear, linear_nvfp4, linear_prepacked, prepack_weight
-from .norm import dequantize, rms_norm
+from .norm import block_norm, dequantize, rms_norm
 from .rope import rope, rope_table
 from .quant import quantize, quantize_fp8, quantize_int8, quantize_nvfp4
 
@@ -13,5 +13,5 @@ __all__ = [
     "quantize", "linear", "fused_linear", "prepack_weight", "linear_prepacked",
     "quantize_nvfp4", "quantize_fp8", "quantize_int8", "linear_nvfp4", "attention", "mha_nvfp4_fwd", "mha_int8_x_fp8_fwd",
     "rms_norm", "dequantize", "rope", "rope_table", "grouped_linear",
-    "route_experts", "combine_experts",
+    "route_experts", "combine_experts", "block_norm",
 ]

@@ -413,6 +413,22 @@ int ac4k_route_experts(float *weights, int32_t *experts, int32_t *offsets, int32
 int ac4k_combine_experts(void *out, int64_t out_stride, const void *y, int64_t y_stride, const float *weights, const int32_t *places,
                          const void *residual, int64_t residual_stride, int64_t T, int64_t k, int64_t M, int64_t N, int dtype, ac4k_stream_t stream);
 
+/* Norms around a block (no counterpart in the reference): rows of x [rows, K], and of everything else, as in ac4k_rms_norm.
+ *   u = x, or norm(x) * post_weight;   h = residual_scale * residual + gate * u rounded to dtype, written to `sum` (x itself without a residual);
+ *   y = norm(h) * weight * (1 + scale) + shift,   norm(v) = (v - mean(v)) / sqrt(var(v) + eps) for kind LAYER, v / sqrt(mean(v^2) + eps) for RMS.
+ * weight and post_weight [K]; gate, scale and shift: row i takes the vector at p + (i / rows) * stride elements, every row the first one where rows is 0; all of
+ * vector_dtype (dtype or fp32), each of them NULL for one that is left out.  residual_scale is taken in fp32.  sum may be x or residual itself, out (precision NONE) x.
+ * out, sf, global_scale and precision as in ac4k_rms_norm.  K <= AC4K_BLOCK_NORM_MAX_COLS.  `workspace`: ac4k_block_norm_workspace_bytes, on 4 bytes,
+ * contents irrelevant, NULL when that is 0. */
+enum { AC4K_NORM_RMS = 0, AC4K_NORM_LAYER = 1 };
+#define AC4K_BLOCK_NORM_MAX_COLS 32768
+int64_t ac4k_block_norm_workspace_bytes(int64_t rows, int64_t K, int dtype, int precision, int given_scale);
+int ac4k_block_norm(void *out, int64_t out_stride, void *sf, float *global_scale, int given_scale, const void *x, int64_t x_stride,
+                    const void *residual, int64_t residual_stride, void *sum, int64_t sum_stride, const void *weight, const void *post_weight,
+                    const void *gate, int64_t gate_stride, int64_t gate_rows, const void *scale, int64_t scale_stride, int64_t scale_rows,
+                    const void *shift, int64_t shift_stride, int64_t shift_rows, int vector_dtype, int64_t rows, int64_t K, int dtype,
+                    int precision, int kind, double residual_scale, double eps, void *workspace, int64_t workspace_bytes, ac4k_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
