@@ -53,12 +53,14 @@ extern "C" __attribute__((visibility("default"))) int ac4k_block_norm(
   a.alpha = (float)residual_scale;
   a.centred = kind == AC4K_NORM_LAYER;
   hipStream_t st = (hipStream_t)stream;
-  int rc;
-  auto go = [&](auto kernels) { rc = kernels(a, precision, find, static_cast<float *>(workspace), dtype, st); };
+  auto go = [&](auto whole, auto cut) { return (K % 8 == 0 ? whole : cut)(a, precision, find, static_cast<float *>(workspace), dtype, st); };
+#define AC4K_BLOCK(DT, VT) go(norm_dtype<NORM_BLOCK, AC4K_DTYPE_##DT, AC4K_DTYPE_##VT>, norm_dtype<NORM_BLOCK_CUT, AC4K_DTYPE_##DT, AC4K_DTYPE_##VT>)
   const bool v32 = vector_dtype == AC4K_DTYPE_FP32;
-  if (dtype == AC4K_DTYPE_FP32) go(norm_dtype<true, AC4K_DTYPE_FP32, AC4K_DTYPE_FP32>);
-  else if (dtype == AC4K_DTYPE_BF16) v32 ? go(norm_dtype<true, AC4K_DTYPE_BF16, AC4K_DTYPE_FP32>) : go(norm_dtype<true, AC4K_DTYPE_BF16, AC4K_DTYPE_BF16>);
-  else v32 ? go(norm_dtype<true, AC4K_DTYPE_FP16, AC4K_DTYPE_FP32>) : go(norm_dtype<true, AC4K_DTYPE_FP16, AC4K_DTYPE_FP16>);
+  int rc;
+  if (dtype == AC4K_DTYPE_FP32) rc = AC4K_BLOCK(FP32, FP32);
+  else if (dtype == AC4K_DTYPE_BF16) rc = v32 ? AC4K_BLOCK(BF16, FP32) : AC4K_BLOCK(BF16, BF16);
+  else rc = v32 ? AC4K_BLOCK(FP16, FP32) : AC4K_BLOCK(FP16, FP16);
+#undef AC4K_BLOCK
   if (rc) return rc;
   return check_launch("ac4k_block_norm");
 }

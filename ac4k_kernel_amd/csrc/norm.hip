@@ -171,9 +171,9 @@ extern "C" __attribute__((visibility("default"))) int ac4k_rms_norm(
   int rc;
   auto go = [&](auto kernels) { rc = kernels(a, precision, find, static_cast<float *>(workspace), dtype, st); };
   const bool w32 = weight && weight_dtype == AC4K_DTYPE_FP32;
-  if (dtype == AC4K_DTYPE_FP32) go(norm_dtype<false, AC4K_DTYPE_FP32, AC4K_DTYPE_FP32>);
-  else if (dtype == AC4K_DTYPE_BF16) w32 ? go(norm_dtype<false, AC4K_DTYPE_BF16, AC4K_DTYPE_FP32>) : go(norm_dtype<false, AC4K_DTYPE_BF16, AC4K_DTYPE_BF16>);
-  else w32 ? go(norm_dtype<false, AC4K_DTYPE_FP16, AC4K_DTYPE_FP32>) : go(norm_dtype<false, AC4K_DTYPE_FP16, AC4K_DTYPE_FP16>);
+  if (dtype == AC4K_DTYPE_FP32) go(norm_dtype<NORM_ROWS, AC4K_DTYPE_FP32, AC4K_DTYPE_FP32>);
+  else if (dtype == AC4K_DTYPE_BF16) w32 ? go(norm_dtype<NORM_ROWS, AC4K_DTYPE_BF16, AC4K_DTYPE_FP32>) : go(norm_dtype<NORM_ROWS, AC4K_DTYPE_BF16, AC4K_DTYPE_BF16>);
+  else w32 ? go(norm_dtype<NORM_ROWS, AC4K_DTYPE_FP16, AC4K_DTYPE_FP32>) : go(norm_dtype<NORM_ROWS, AC4K_DTYPE_FP16, AC4K_DTYPE_FP16>);
   if (rc) return rc;
   return check_launch("ac4k_rms_norm");
 }

@@ -8,6 +8,9 @@ namespace ac4k {
 
 enum NormOut { NORM_PLAIN = 0, NORM_FP8 = 1, NORM_INT8 = 2, NORM_NVFP4 = 3, NORM_STATS = 4, NORM_NVFP4_SECOND = 5, NORM_NVFP4_ONE = 6 };
 
+// Rows of block_norm come in two kernels: without a vector that is cut by the row's end there is half the code, which keeps a third fewer registers.
+enum NormMode { NORM_ROWS = 0, NORM_BLOCK = 1, NORM_BLOCK_CUT = 2 };
+
 // one of a block's vectors of K: the same for all rows (rows 0), or one for so many rows each
 struct NormVector {
   const void *p;
@@ -89,14 +92,15 @@ __device__ __forceinline__ void row_vector(Vec8<DT> &v, const void *row, int64_t
 
 // BW waves a workgroup, LPR lanes a row, NV vectors of eight elements a lane: K <= 8 * LPR * NV.  A workgroup takes rows_per_block rows, a
 // multiple of the rows that it has lanes for.
-template <bool BLOCK, int DT, int WT, int OUT, int BW, int LPR, int NV>
+template <int MODE, int DT, int WT, int OUT, int BW, int LPR, int NV>
 __global__ __launch_bounds__(64 * BW) void norm_rows_kernel(NormArgs a, int rows_per_block) {
   using T = typename Elem<DT>::T;
+  constexpr bool BLOCK = MODE != NORM_ROWS;
   constexpr int GROUPS = 64 * BW / LPR, WPR = LPR / 64;  // WPR: waves a row, 0 where a wave has several
   constexpr int IN_WAVE = LPR < 64 ? LPR : 64;
   constexpr bool NVFP4 = OUT == NORM_NVFP4 || OUT == NORM_NVFP4_SECOND || OUT == NORM_NVFP4_ONE;
   constexpr bool SUMS = OUT != NORM_NVFP4_SECOND;  // x is normalized here, not by an earlier launch
-  __shared__ double part[BLOCK ? 2 : 1][WPR > 1 ? BW : 1];
+  __shared__ double part[BLOCK ? 2 : 1][WPR > 1 ? BLOCK ? 2 * BW : BW : 1];
   __shared__ uint32_t part_max[BW];
   __shared__ float lut[NVFP4 ? 128 : 1];
   const int tid = threadIdx.x, sub = tid % LPR, wave = tid >> 6;
@@ -126,13 +130,13 @@ __global__ __launch_bounds__(64 * BW) void norm_rows_kernel(NormArgs a, int rows
     alpha = g == 0.0f ? 0.0f : 1.0f / g;
     if (blockIdx.x == 0 && tid == 0) *a.gs = g;
   };
-  const int cut = (int)(a.K & 7);
+  const int cut = MODE == NORM_BLOCK ? 0 : (int)(a.K & 7);
   const int64_t k_cut = a.K - cut;
   const bool cut_mine = cut != 0 && (int)(k_cut / 8 % LPR) == sub;
   // the weights, once for all rows of the workgroup, and under way before the first row's sum is known; rows of eight vectors leave no
-  // registers for them, and read them where they are used
-  constexpr bool HELD = NV <= 4;
-  static_assert(!BLOCK || HELD, "a block's rows are at most 32768 elements");
+  // registers for them, and read them where they are used, as rows of blocks do all their vectors
+  constexpr bool HELD = NV <= 4 && !BLOCK;
+  static_assert(!BLOCK || NV <= 4, "a block's rows are at most 32768 elements");
   Vec8<WT> w[HELD ? NV : 1];
   const bool weighted = a.weight != nullptr;
   if (HELD && weighted) {
@@ -141,45 +145,72 @@ __global__ __launch_bounds__(64 * BW) void norm_rows_kernel(NormArgs a, int rows
 #pragma unroll
     for (int j = 0; j < (HELD ? NV : 0); ++j) row_vector(w[j], a.weight, (j * LPR + sub) * 8, a.K, w_cut);
   }
-  // BLOCK: sum over a row; parts of one sum and of the next one lie apart, so that a barrier each is enough
-  int flip = 0;
-  auto row_sum = [&](double s) {
-    s = group_sum<IN_WAVE>(s);
-    if constexpr (WPR > 1) {
-      if ((tid & 63) == 0) part[BLOCK ? flip : 0][wave] = s;
-      __syncthreads();
-      s = 0.0;
+  const int Ks = (int)a.K;
+  // BLOCK: vector k of one of a block's rows of K; behind the row it is zero with `zero`, otherwise any of the row's vectors or zero
+  auto row_piece = [&](auto &v, const auto *p, int k, bool zero) {
+    if constexpr (MODE == NORM_BLOCK) {
+      vec8_load_all(v, p + (k < Ks ? k : Ks - 8));  // no branch
+      if (zero) {
 #pragma unroll
-      for (int i = 0; i < WPR; ++i) s += part[BLOCK ? flip : 0][group * WPR + i];
+        for (uint32_t &w : v.w) w = k < Ks ? w : 0u;
+      }
+    } else {
+      int at = k;
+      asm("" : "+v"(at));  // compared here, not once for all pieces (whose masks spill scalar registers)
+      vec8_load(v, p, at, Ks);
+    }
+  };
+  // BLOCK: two sums over a row; parts of these and of the next ones lie apart, so that a barrier each time is enough
+  int flip = 0;
+  auto row_sums = [&](double &s, double &t) {
+    s = group_sum<IN_WAVE>(s);
+    t = group_sum<IN_WAVE>(t);
+    if constexpr (WPR > 1) {
+      if ((tid & 63) == 0) part[flip][wave] = s, part[flip][BW + wave] = t;
+      __syncthreads();
+      s = t = 0.0;
+#pragma unroll
+      for (int i = 0; i < WPR; ++i) s += part[flip][group * WPR + i], t += part[flip][BW + group * WPR + i];
       flip ^= 1;
     }
-    return s;
   };
-  // BLOCK: mean (in two pieces; 0 where rows are not centred) and factor of a row
+  // BLOCK: mean (in two pieces; 0 where rows are not centred) and factor of a row.  Sums of 16-bit elements and of their squares lose nothing next to 64 bits, and the
+  // variance is their difference; elements of 32 bits are squared without the mean.
   auto row_stats = [&](const Vec8<DT>(&v)[NV], float &m1, float &m2, float &r) {
-    double s = 0.0, mean = 0.0;
+    double s = 0.0, q = 0.0, mean = 0.0, var;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const double d = (double)vec8_get(v[j], i);
+        if (a.centred) s += d;
+        q = __builtin_fma(d, d, q);
+      }
+    row_sums(s, q);
+    var = q * a.inverse_K;
     if (a.centred) {
+      mean = s / (double)a.K;  // (exact for rows of one value)
+      if constexpr (DT == AC4K_DTYPE_FP32) {
+        q = 0.0;
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
+        for (int j = 0; j < NV; ++j) {
+          const int k = (j * LPR + sub) * 8;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s += (double)vec8_get(v[j], i);
-      mean = row_sum(s) / (double)a.K;  // (exact for rows of one value)
-      s = 0.0;
+          for (int i = 0; i < 8; ++i) {
+            const double d = (MODE == NORM_BLOCK ? k : k + i) < Ks ? (double)vec8_get(v[j], i) - mean : 0.0;
+            q = __builtin_fma(d, d, q);
+          }
+        }
+        row_sums(s, q);
+        var = q * a.inverse_K;
+      } else {
+        var = __builtin_fma(-mean, s, q);
+        var = var < 0.0 ? 0.0 : var * a.inverse_K;  // (NaN stays)
+      }
     }
     m1 = (float)mean;
     m2 = (float)(mean - (double)m1);
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int k = (j * LPR + sub) * 8;
-      const bool whole = k + 8 <= a.K;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        double d = (double)vec8_get(v[j], i) - mean;
-        if (!whole) d = k + i < a.K ? d : 0.0;  // (not 0 where there is no element)
-        s = __builtin_fma(d, d, s);
-      }
-    }
-    r = norm_factor(row_sum(s) * a.inverse_K + a.eps);
+    r = norm_factor(var + a.eps);
   };
   uint32_t block_m = 0;
   const int64_t row0 = (int64_t)blockIdx.x * rows_per_block;
@@ -189,18 +220,18 @@ __global__ __launch_bounds__(64 * BW) void norm_rows_kernel(NormArgs a, int rows
     if (WPR <= 1 && OUT != NORM_NVFP4_ONE && !(OUT == NORM_NVFP4_SECOND && it == 0) && !valid && !(NVFP4 && row < a.Rp)) break;  // (rows of several waves meet at barriers)
     Vec8<DT> h[NV];
     float r = 0.0f, m1 = 0.0f, m2 = 0.0f;
-    Vec8<WT> sc[BLOCK ? NV : 1], sh[BLOCK ? NV : 1];  // BLOCK: scale and shift
-    auto block_vector = [&](const NormVector &p, Vec8<WT>(&v)[BLOCK ? NV : 1]) {
-      using W = typename Elem<WT>::T;
-      const uint32_t at = p.rows == 0 ? 0 : p.rows == 1 ? (uint32_t)row : (uint32_t)row / p.rows;
-      const W *vp = static_cast<const W *>(p.p) + at * p.stride;
-      Vec8<WT> v_cut;
-      cut_load(v_cut, vp, k_cut, cut_mine && valid, cut);
-#pragma unroll
-      for (int j = 0; j < (BLOCK ? NV : 0); ++j) row_vector(v[j], vp, (j * LPR + sub) * 8, valid ? a.K : 0, v_cut);
+    // BLOCK: a vector of this row.  (A row behind the last one is that one again; nothing is kept of it.)
+    using W = typename Elem<WT>::T;
+    const int64_t row_in = BLOCK && !valid ? a.rows - 1 : row;
+    auto vector_of = [&](const NormVector &p) {
+      const uint32_t at = p.rows == 0 ? 0 : p.rows == 1 ? (uint32_t)row_in : (uint32_t)row_in / p.rows;
+      return static_cast<const W *>(p.p) + at * p.stride;
     };
-    {
-      const T *xp = static_cast<const T *>(a.x) + row * a.x_stride;
+    const T *xp = static_cast<const T *>(a.x) + row_in * a.x_stride;
+    if constexpr (BLOCK) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) row_piece(h[j], xp, (j * LPR + sub) * 8, true);
+    } else {
       Vec8<DT> x_cut;
       cut_load(x_cut, xp, k_cut, cut_mine && valid, cut);
 #pragma unroll
@@ -208,48 +239,53 @@ __global__ __launch_bounds__(64 * BW) void norm_rows_kernel(NormArgs a, int rows
     }
     if constexpr (BLOCK) {
       if (SUMS && a.residual) {
-        const T *rp = static_cast<const T *>(a.residual) + row * a.residual_stride;
+        const T *rp = static_cast<const T *>(a.residual) + row_in * a.residual_stride;
         T *sp = static_cast<T *>(a.sum) + row * a.sum_stride;
-        Vec8<DT> q[NV], r_cut;
-        cut_load(r_cut, rp, k_cut, cut_mine && valid, cut);
+        Vec8<DT> q[NV], q_cut;
 #pragma unroll
-        for (int j = 0; j < NV; ++j) row_vector(q[j], rp, (j * LPR + sub) * 8, valid ? a.K : 0, r_cut);
-        Vec8<WT> g[BLOCK ? NV : 1], pw[BLOCK ? NV : 1];
+        for (int j = 0; j < NV; ++j) row_piece(q[j], rp, (j * LPR + sub) * 8, false);
         const bool gated = a.gate.p != nullptr, post = a.post != nullptr;
-        if (gated) block_vector(a.gate, g);
+        const W *gp = vector_of(a.gate), *pp = static_cast<const W *>(a.post);
         float pr = 1.0f;
-        if (post) {
-          block_vector(NormVector{a.post, 0, 0}, pw);
-          row_stats(h, m1, m2, pr);
-        }
+        if (post) row_stats(h, m1, m2, pr);
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
           const int k = (j * LPR + sub) * 8;
           float f[8];
+          Vec8<WT> v;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            f[i] = vec8_get(h[j], i);
-            if (post) f[i] = ((f[i] - m1) - m2) * pr * vec8_get(pw[j], i);
-            if (gated) f[i] *= vec8_get(g[j], i);
-            f[i] = vec8_get(q[j], i) * a.alpha + f[i];
-          }
-          if (k + 8 > a.K) {
+          for (int i = 0; i < 8; ++i) f[i] = vec8_get(h[j], i);
+          if (post) {
+            row_piece(v, pp, k, false);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = k + i < a.K ? f[i] : 0.0f;
+            for (int i = 0; i < 8; ++i) f[i] = ((f[i] - m1) - m2) * pr * vec8_get(v, i);
           }
+          if (gated) {
+            row_piece(v, gp, k, false);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = __builtin_fmaf(f[i], vec8_get(v, i), vec8_get(q[j], i) * a.alpha);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = vec8_get(q[j], i) * a.alpha + f[i];
+          }
+          // behind the row h is 0: all that is loaded there is (NORM_BLOCK_CUT: a row with a mean that is not finite is NaN anyway)
           vec8_set(h[j], f);
-          if (valid && k + 8 <= a.K) vec8_store_all(sp + k, h[j]);
-          else if (k < a.K) r_cut = h[j];
+          if constexpr (MODE == NORM_BLOCK) {
+#pragma unroll
+            for (uint32_t &w : h[j].w) w = k < Ks ? w : 0u;
+            if (valid && k < Ks) vec8_store_all(sp + k, h[j]);
+          } else {
+            if (valid && k + 8 <= Ks) vec8_store_all(sp + k, h[j]);
+            else if (k < Ks) q_cut = h[j];
+          }
         }
-        if (cut_mine && valid) vec8_store_some(sp + k_cut, r_cut, cut);
+        if (MODE == NORM_BLOCK_CUT && cut_mine && valid) vec8_store_some(sp + k_cut, q_cut, cut);
       }
-      if (a.scale.p) block_vector(a.scale, sc);
-      if (a.shift.p) block_vector(a.shift, sh);
       if constexpr (SUMS) {
         row_stats(h, m1, m2, r);
-      } else if (valid) {
-        m1 = a.centred ? a.means[2 * row] : 0.0f;
-        m2 = a.centred ? a.means[2 * row + 1] : 0.0f;
+      } else if (a.centred) {
+        m1 = a.means[2 * row_in];
+        m2 = a.means[2 * row_in + 1];
       }
     } else if constexpr (SUMS) {
       if (a.residual && valid) {
@@ -300,6 +336,7 @@ __global__ __launch_bounds__(64 * BW) void norm_rows_kernel(NormArgs a, int rows
         global_scale(block_max(group_umax<64>(m)));
       }
     }
+    const W *const scp = BLOCK ? vector_of(a.scale) : nullptr, *const shp = BLOCK ? vector_of(a.shift) : nullptr;
     // y of vector j
     auto values = [&](int j, float (&y)[8]) {
       const int k = (j * LPR + sub) * 8;
@@ -307,22 +344,39 @@ __global__ __launch_bounds__(64 * BW) void norm_rows_kernel(NormArgs a, int rows
       for (int i = 0; i < 8; ++i) y[i] = (BLOCK ? (vec8_get(h[j], i) - m1) - m2 : vec8_get(h[j], i)) * r;
       if (weighted) {
         Vec8<WT> &v = w[HELD ? j : 0];
-        if constexpr (!HELD) vec8_load(v, a.weight, k, a.K);
+        if constexpr (BLOCK) row_piece(v, static_cast<const W *>(a.weight), k, false);
+        else if constexpr (!HELD) vec8_load(v, a.weight, k, a.K);
 #pragma unroll
         for (int i = 0; i < 8; ++i) y[i] = y[i] * vec8_get(v, i);
       }
       if constexpr (BLOCK) {
-        if (a.scale.p) {
+        Vec8<WT> v, u;
+        if (a.scale.p && a.shift.p) {
+          row_piece(v, scp, k, false);
+          row_piece(u, shp, k, false);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) y[i] = y[i] * (1.0f + vec8_get(sc[j], i));
-        }
-        if (a.shift.p) {
+          for (int i = 0; i < 8; ++i) y[i] = __builtin_fmaf(y[i], 1.0f + vec8_get(v, i), vec8_get(u, i));
+        } else if (a.scale.p) {
+          row_piece(v, scp, k, false);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) y[i] = y[i] + vec8_get(sh[j], i);
+          for (int i = 0; i < 8; ++i) y[i] = y[i] * (1.0f + vec8_get(v, i));
+        } else if (a.shift.p) {
+          row_piece(v, shp, k, false);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) y[i] = y[i] + vec8_get(v, i);
         }
       }
-      // behind the row the product 0 * r * 0 is not 0 where r is not finite
-      if (k + 8 > a.K) {
+      // behind the row the product 0 * r * 0 is not 0 where r is not finite, and a centred row is not 0
+      if constexpr (BLOCK) {
+        if constexpr (MODE == NORM_BLOCK_CUT && OUT != NORM_PLAIN) {
+          int left = Ks - k;
+          asm("" : "+v"(left));
+          if (left < 8) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = i < left ? y[i] : 0.0f;
+          }
+        }
+      } else if (k + 8 > a.K) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) y[i] = k + i < a.K ? y[i] : 0.0f;
       }
@@ -345,7 +399,7 @@ __global__ __launch_bounds__(64 * BW) void norm_rows_kernel(NormArgs a, int rows
           float y[8];
           values(j, y);
           vec8_set(o, y);
-          if (k + 8 <= a.K) vec8_store_all(op + k, o);
+          if (MODE == NORM_BLOCK || k + 8 <= a.K) vec8_store_all(op + k, o);
           else o_cut = o;
         }
         if (cut_mine) vec8_store_some(op + k_cut, o_cut, cut);
@@ -498,13 +552,13 @@ static NormPlan norm_plan(int64_t rows, int64_t K, bool nvfp4) {
 // vectors of a lane in the kernel that takes a tensor in one workgroup (128 registers)
 constexpr int norm_one_vectors(int dtype) { return dtype == AC4K_DTYPE_FP32 ? 2 : 4; }
 
-template <bool BLOCK, int DT, int WT, int OUT>
+template <int MODE, int DT, int WT, int OUT>
 static int launch_norm(const NormArgs &a, const NormPlan &p, hipStream_t st) {
   const int64_t rows = OUT == NORM_NVFP4 || OUT == NORM_NVFP4_SECOND ? a.Rp : a.rows;
   const int64_t blocks = ceil_div(rows, p.rows_per_block);
   auto go = [&](auto kernel, int bw) { hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(64 * bw), 0, st, a, p.rows_per_block); };
 #define AC4K_NORM(BW, LPR, NV) \
-  if (p.bw == BW && p.lpr == LPR && p.nv == NV) return go(norm_rows_kernel<BLOCK, DT, WT, OUT, BW, LPR, NV>, BW), 0
+  if (p.bw == BW && p.lpr == LPR && p.nv == NV) return go(norm_rows_kernel<MODE, DT, WT, OUT, BW, LPR, NV>, BW), 0
   constexpr int NV1 = norm_one_vectors(DT);
   if constexpr (OUT == NORM_NVFP4_ONE) {
     AC4K_NORM(8, 512, 2);
@@ -524,7 +578,7 @@ static int launch_norm(const NormArgs &a, const NormPlan &p, hipStream_t st) {
     AC4K_NORM(8, 512, 2);
     AC4K_NORM(16, 1024, 2);
     AC4K_NORM(16, 1024, 4);
-    if constexpr (!BLOCK) AC4K_NORM(16, 1024, 8);
+    if constexpr (MODE == NORM_ROWS) AC4K_NORM(16, 1024, 8);
   }
 #undef AC4K_NORM
   return set_error("norm of rows: no kernel for %d lanes a row and %d vectors a lane", p.lpr, p.nv);
@@ -555,26 +609,26 @@ static int64_t norm_workspace(int64_t rows, int64_t K, int dtype) {
   return 4 * (align_up(rows, 64) + ceil_div(rows, norm_stats_plan(rows, K).rows_per_block));
 }
 
-template <bool BLOCK, int DT, int WT>
+template <int MODE, int DT, int WT>
 static int norm_dtype(NormArgs a, int precision, bool find_scale, float *workspace, int dtype, hipStream_t st) {
   if (precision == AC4K_PRECISION_NVFP4 && find_scale) {
     NormPlan p;
-    if (norm_one(a.rows, a.K, dtype, p)) return launch_norm<BLOCK, DT, WT, NORM_NVFP4_ONE>(a, p, st);
+    if (norm_one(a.rows, a.K, dtype, p)) return launch_norm<MODE, DT, WT, NORM_NVFP4_ONE>(a, p, st);
     p = norm_stats_plan(a.rows, a.K);
     a.factors = workspace;
     a.maxima = workspace + align_up(a.rows, 64);
     a.maxima_count = (int)ceil_div(a.rows, p.rows_per_block);
     a.means = a.maxima + a.maxima_count;
-    if (int rc = launch_norm<BLOCK, DT, WT, NORM_STATS>(a, p, st)) return rc;
+    if (int rc = launch_norm<MODE, DT, WT, NORM_STATS>(a, p, st)) return rc;
     if (a.residual) a.x = a.sum, a.x_stride = a.sum_stride;
-    return launch_norm<BLOCK, DT, WT, NORM_NVFP4_SECOND>(a, norm_plan(a.rows, a.K, true), st);
+    return launch_norm<MODE, DT, WT, NORM_NVFP4_SECOND>(a, norm_plan(a.rows, a.K, true), st);
   }
   const NormPlan p = norm_plan(a.rows, a.K, precision == AC4K_PRECISION_NVFP4);
   switch (precision) {
-    case AC4K_PRECISION_NONE: return launch_norm<BLOCK, DT, WT, NORM_PLAIN>(a, p, st);
-    case AC4K_PRECISION_FP8: return launch_norm<BLOCK, DT, WT, NORM_FP8>(a, p, st);
-    case AC4K_PRECISION_INT8: return launch_norm<BLOCK, DT, WT, NORM_INT8>(a, p, st);
-    default: return launch_norm<BLOCK, DT, WT, NORM_NVFP4>(a, p, st);
+    case AC4K_PRECISION_NONE: return launch_norm<MODE, DT, WT, NORM_PLAIN>(a, p, st);
+    case AC4K_PRECISION_FP8: return launch_norm<MODE, DT, WT, NORM_FP8>(a, p, st);
+    case AC4K_PRECISION_INT8: return launch_norm<MODE, DT, WT, NORM_INT8>(a, p, st);
+    default: return launch_norm<MODE, DT, WT, NORM_NVFP4>(a, p, st);
   }
 }
 

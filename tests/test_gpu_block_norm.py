@@ -33,6 +33,11 @@ def normed32(v, kind, eps):
     return ((v.float() - m1) - (mean - m1.double()).float()) * r.float()
 
 
+def fma32(a, b, c):
+    """a * b + c, rounded once (the product of two fp32 numbers is exact in 64 bits)."""
+    return (a.double() * b.double() + c.double()).float()
+
+
 class Reference:
     def __init__(self, x, residual=None, weight=None, gate=None, residual_scale=1.0, post_weight=None, scale=None, shift=None, kind="rms", eps=EPS):
         cpu = [None if t is None else t.cpu() for t in (x, residual, weight, gate, post_weight, scale, shift)]
@@ -43,10 +48,13 @@ class Reference:
             if post_weight is not None:
                 mean, r = stats(x, kind, eps)
                 u, u64 = normed32(x, kind, eps) * post_weight.float(), (x.double() - mean) * r * post_weight.double()
-            if gate is not None:
-                u, u64 = u * gate.float(), u64 * gate.double()
             a = torch.tensor(residual_scale, dtype=torch.float32)
-            self.h = (residual.float() * a + u).to(x.dtype)
+            h = residual.float() * a
+            if gate is not None:
+                h, u64 = fma32(u, gate.float(), h), u64 * gate.double()
+            else:
+                h = h + u
+            self.h = h.to(x.dtype)
             self.h64 = residual.double() * a.double() + u64
             self.h_size = (residual.double() * a.double()).abs() + u64.abs()
         mean, r = stats(self.h, kind, eps)
@@ -55,9 +63,12 @@ class Reference:
         if weight is not None:
             self.y32, n64, size = self.y32 * weight.float(), n64 * weight.double(), size * weight.double().abs()
         if scale is not None:
-            self.y32, n64, size = self.y32 * (1.0 + scale.float()), n64 * (1.0 + scale.double()), size * (1.0 + scale.double()).abs()
+            n64, size = n64 * (1.0 + scale.double()), size * (1.0 + scale.double()).abs()
+            self.y32 = self.y32 * (1.0 + scale.float()) if shift is None else fma32(self.y32, 1.0 + scale.float(), shift.float())
+        elif shift is not None:
+            self.y32 = self.y32 + shift.float()
         if shift is not None:
-            self.y32, n64 = self.y32 + shift.float(), n64 + shift.double()
+            n64 = n64 + shift.double()
         self.y64, self.size = n64, size
 
     def check(self, got, precision=None, gs=None):
