@@ -74,6 +74,7 @@ SIGNATURES = {
     "ac4k_block_norm_workspace_bytes": (_i64, [_i64, _i64, _int, _int, _int]),
     "ac4k_block_norm": (_int, [_vp, _i64, _vp, _vp, _int] + [_vp, _i64] * 3 + [_vp, _vp] + [_vp, _i64, _i64] * 3 + [_int, _i64, _i64] + [_int] * 3 +
                         [ctypes.c_double] * 2 + [_vp, _i64, _vp]),
+    "ac4k_linear_nvfp4_epilogue": (_int, [_vp, _int] + [_vp] * 7 + [_int, _int, _vp] + [_i64] * 4 + [_vp, _i64, _vp]),
     "ac4k_combine_experts": (_int, [_vp, _i64, _vp, _i64, _vp, _vp, _vp] + [_i64] * 5 + [_int, _vp]),
 }
 for _name in ("ac4k_linear_grouped_nvfp4", "ac4k_linear_grouped_nvfp4_whole"):

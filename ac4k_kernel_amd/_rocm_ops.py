@@ -225,6 +225,46 @@ def linear_nvfp4(D, A, A_sf, A_global_scale, B, B_sf, B_global_scale, bias=None)
                                     B_global_scale.data_ptr(), bias_ptr, bias_tag, M, N, K, _stream()))
 
 
+_ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+
+
+def linear_nvfp4_epilogue(D, A, A_sf, A_global_scale, B, B_sf, B_global_scale, bias=None, activation=None, residual=None, fresh=False) -> None:
+    """linear_nvfp4 with D = act(product + bias) + residual, rounded once.  fresh: D is a new tensor that overlaps nothing."""
+    M, N, tag = _check_output(D)
+    number = _ACTIVATIONS.get(activation) if activation is None or isinstance(activation, str) else None
+    if number is None:
+        _check(False, "activation must be one of {}", list(_ACTIVATIONS))
+    if A is None or A_sf is None or A_global_scale is None or B is None or B_sf is None or B_global_scale is None:
+        _check(False, "operands must be tensors, not NoneType")
+    _same_device(D, A, A_sf, A_global_scale, B, B_sf, B_global_scale, bias, residual)
+    _check(A.dim() == 2 and A.size(0) == M, "A size(0) must be {}", M)
+    K = _check_linear_operand(A, A_sf, A_global_scale, M, "a")
+    if K % 16 != 0:
+        _check(False, "A size(1)*2 must be multiple of 16 but see {}", K)
+    _check(B.dim() == 2 and B.size(1) * 2 == K, "B size(1) must equal A size(1)")
+    _check(B.size(0) == N, "B size(0) must be {}", N)
+    _check_linear_operand(B, B_sf, B_global_scale, N, "b")
+    bias_ptr, bias_tag = (None, 0) if bias is None else _bias_args(bias, N)
+    residual_ptr, residual_step = None, 0
+    if residual is not None:
+        if _check_float(residual, "residual") != tag or residual.shape != (M, N):
+            _check(False, "residual must have the type of the output and be [{}, {}]", M, N)
+        if N:
+            v = _rows_view(residual, "residual")
+            _check(v is not None, "residual must have rows of contiguous elements, evenly apart")
+            residual_ptr, residual_step = residual.data_ptr(), v[2]
+        _check(fresh or _same_rows(D, residual) or not _may_overlap(D, residual), "out may be residual itself, but not overlap it otherwise")
+    if not fresh:
+        _check(not any(_may_overlap(D, t) for t in (A, A_sf, A_global_scale, B, B_sf, B_global_scale, bias) if t is not None), "out must not overlap an operand")
+    if M == 0 or N == 0:
+        return
+    nbytes = _L.ac4k_linear_nvfp4_scratch_bytes(M, N, K)
+    ws = D.new_empty((nbytes,), dtype=torch.uint8) if nbytes > 0 else None
+    _lib.check(_L.ac4k_linear_nvfp4_epilogue(D.data_ptr(), tag, A.data_ptr(), A_sf.data_ptr(), A_global_scale.data_ptr(), B.data_ptr(), B_sf.data_ptr(),
+                                             B_global_scale.data_ptr(), bias_ptr, bias_tag, number, residual_ptr, residual_step, M, N, K,
+                                             None if ws is None else ws.data_ptr(), nbytes, _stream()))
+
+
 def prepack_weight_nvfp4(B, B_sf) -> torch.Tensor:
     """Weight image of B [N, K/2] / B_sf [K/64, align_up(N,16), 4] for linear_nvfp4_prepacked: a uint8
     tensor of ac4k_prepack_weight_nvfp4_bytes(N, K) bytes.  K must be a multiple of 128."""

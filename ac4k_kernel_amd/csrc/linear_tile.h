@@ -16,6 +16,7 @@ struct LinearArgs {
   const void *bias;
   int64_t M, N, K, Mp, Np;
   int prepacked = 0;  // B points at a weight image (W_BLOCK_BYTES blocks, see below) and B_sf is unused
+  Epilogue ep = {};
 };
 
 // --- pre-packed weight image -----------------------------------------------------
@@ -336,6 +337,108 @@ __device__ __forceinline__ void store_tile(const f32x16 (&acc)[MI][NJ], char *ld
         if (cols_left > 0 && row_in(p * RP + it * RS)) store_piece<S>(rowp + it * RS * row_bytes + lane_off, v, cols_left);
       }
     }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
+}
+
+// The same with what BIAS_EPILOGUE adds.  The sums are staged in 32 bits, and everything else happens where the rows leave: a lane has the same columns in all
+// rows, so that its bias stays in registers, and reads the residual in the 16 bytes that it stores, G steps of rows ahead.
+template <int OUT_DT, int MI, int NJ, int LDS_BYTES>
+__device__ __forceinline__ void store_tile_epilogue(const f32x16 (&acc)[MI][NJ], char *lds, const LinearArgs &a, float scale, int64_t m0, int64_t n0) {
+  using DE = Elem<OUT_DT>;
+  using DT = typename DE::T;
+  constexpr int S = sizeof(DT), V = 16 / S, WN = 32 * NJ, RP = 32;
+  constexpr int PITCH = WN * 4 + 16;
+  static_assert(4 * RP * PITCH <= LDS_BYTES, "epilogue staging must fit in LDS");
+  constexpr int CPR = WN / V, RS = 64 / CPR, IT = RP / RS, G = IT < 4 ? IT : 4;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+  const int lrow = lane / CPR, lq = lane % CPR;
+  char *stg = lds + wave * (RP * PITCH);
+  const int64_t n = n0 + lq * V;
+  const int64_t cl = a.N - n;
+  const int cols = cl > V ? V : (int)cl;  // columns of this lane's piece inside the matrix
+  const int64_t rl = a.M - m0 - lrow;
+  const int rows_left = cols <= 0 ? 0 : rl > 32 * MI ? 32 * MI : (int)rl;
+  float bias[V];
+#pragma unroll
+  for (int q = 0; q < V; ++q) bias[q] = a.ep.bias && q < cols ? epilogue_bias(a.ep, n + q) : 0.0f;
+  const char *res = static_cast<const char *>(a.ep.residual) + ((m0 + lrow) * a.ep.residual_stride + n) * S;
+  const int64_t res_step = RS * a.ep.residual_stride * S, out_step = RS * a.N * S;
+  char *out = static_cast<char *>(a.D) + ((m0 + lrow) * a.N + n) * S;
+  u32x4 ahead[G];
+  auto fetch = [&](int step) {
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      ahead[g] = (u32x4){0, 0, 0, 0};
+      if (a.ep.residual && (step + g) * RS < rows_left) {
+        const char *p = res + (step + g) * res_step;
+        if (cols == V) {
+          ahead[g] = *reinterpret_cast<const u32x4_elem *>(p);
+        } else {
+#pragma unroll
+          for (int q = 0; q < V; ++q)
+            if (q < cols) {
+              if constexpr (S == 4) ahead[g][q] = reinterpret_cast<const uint32_t *>(p)[q];
+              else ahead[g][q / 2] |= (uint32_t)reinterpret_cast<const uint16_t *>(p)[q] << (16 * (q & 1));
+            }
+        }
+      }
+    }
+  };
+  fetch(0);
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        float v[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          if constexpr (MI * NJ == 16) asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(v[q]) : "a"(acc[i][j][4 * g + q]));  // (see store_tile)
+          else v[q] = acc[i][j][4 * g + q];
+        }
+        *reinterpret_cast<float4 *>(stg + (lane & 31) * PITCH + (j * 32 + g * 8 + half * 4) * 4) = make_float4(v[0] * scale, v[1] * scale, v[2] * scale, v[3] * scale);
+      }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the staging block is private to the wave
+    with_activation(a.ep.activation, [&](auto act) {
+#pragma unroll 1
+      for (int it = 0; it < IT; it += G) {
+        u32x4 now[G];
+#pragma unroll
+        for (int g = 0; g < G; ++g) now[g] = ahead[g];
+        if (i * IT + it + G < MI * IT) fetch(i * IT + it + G);
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          const int step = i * IT + it + g;
+          const float4 *src = reinterpret_cast<const float4 *>(stg + ((it + g) * RS + lrow) * PITCH + lq * V * 4);
+          float v[V];
+#pragma unroll
+          for (int q = 0; q < V; q += 4) {
+            const float4 f = src[q / 4];
+            v[q] = f.x, v[q + 1] = f.y, v[q + 2] = f.z, v[q + 3] = f.w;
+          }
+          u32x4 o;
+#pragma unroll
+          for (int q = 0; q < V; ++q) v[q] = act(v[q] + bias[q]);
+          if (a.ep.residual) {
+#pragma unroll
+            for (int q = 0; q < V; ++q) {
+              DT r[16 / S];
+              __builtin_memcpy(r, &now[g], 16);
+              v[q] += DE::load(r, q);
+            }
+          }
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            if constexpr (S == 2) o[q] = DE::cvt2(v[2 * q], v[2 * q + 1]);
+            else o[q] = __float_as_uint(v[q]);
+          }
+          if (step * RS < rows_left) store_piece<S>(out + step * out_step, o, cols);
+        }
+      }
+    });
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
 }
@@ -671,6 +774,8 @@ __device__ __forceinline__ void tile256p(const LinearArgs &a, const SplitK &sk, 
     if (!GROUPED && sk.partial) {  // split-K: raw fp32 sums of this K range; the reduce kernel scales and converts
       store_tile<AC4K_DTYPE_FP32, BIAS_NONE, true, MI, NJ, PL::LDS_BYTES, false>(
           sums, plds, sk.partial + (int64_t)blockIdx.y * a.M * a.N, nullptr, 1.0f, a.M, a.N, m0, n0, tn * BN, 0);
+    } else if constexpr (BIAS_DT == BIAS_EPILOGUE) {
+      store_tile_epilogue<D_DT, MI, NJ, PL::LDS_BYTES>(sums, plds, a, (*a.A_gs) * (*a.B_gs), m0, n0);
     } else {
       store_tile<D_DT, BIAS_DT, false, MI, NJ, PL::LDS_BYTES, GROUPED>(sums, plds, a.D, a.bias, (*a.A_gs) * (*a.B_gs), a.M, a.N,
                                                              m0, n0, tn * BN, tr.lo);

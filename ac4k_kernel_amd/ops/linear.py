@@ -22,14 +22,30 @@ class Ac4kLinearOp(torch.nn.Module):
         return out
 
 
-def linear(x, x_scale, x_global_scale, weight, weight_scale, weight_global_scale, bias=None, out=None):
-    """y = x @ weight.T + bias on NVFP4 operands.
+def linear(x, x_scale, x_global_scale, weight, weight_scale, weight_global_scale, bias=None, out=None, activation=None, residual=None):
+    """y = act(x @ weight.T + bias) + residual on NVFP4 operands.
 
     x [M, K/2] and weight [N, K/2] are packed e2m1 (uint8), *_scale the e4m3 block scales in the
     [K/64, align_up(rows,16), 4] layout, *_global_scale 0-dim fp32.  bias is [N] or [1, N] in
     bf16/fp16/fp32; out defaults to a new bf16 [M, N] and may be bf16, fp16 or fp32.
+    activation: None, "relu", "gelu" (x Phi(x)), "gelu_tanh" (its approximation by tanh) or "silu".  residual [M, N] has the type of out (bf16
+    without one) and may be out itself; its rows may lie apart.  Both are in the product's epilogue: sum, bias, activation and residual in 32 bits, one rounding.
     """
-    return _LINEAR_OP.forward(x, x_scale, x_global_scale, weight, weight_scale, weight_global_scale, bias, out=out)
+    if activation is None and residual is None:
+        return _LINEAR_OP.forward(x, x_scale, x_global_scale, weight, weight_scale, weight_global_scale, bias, out=out)
+    if not isinstance(x, torch.Tensor) or x.dim() != 2 or not isinstance(weight, torch.Tensor) or weight.dim() != 2:
+        raise RuntimeError("x must be [M, K/2] and weight [N, K/2]")
+    if isinstance(bias, torch.Tensor) and bias.ndim == 1:
+        bias = bias.reshape(1, -1)
+    if isinstance(residual, torch.Tensor) and residual.dim() == 2 and residual.numel() and _rocm_ops._rows_view(residual, "residual") is None:
+        if out is residual:
+            raise RuntimeError("out must be contiguous")
+        residual = residual.contiguous()
+    fresh = out is None
+    if fresh:
+        out = torch.empty((x.size(0), weight.size(0)), dtype=torch.bfloat16, device=x.device)
+    _rocm_ops.linear_nvfp4_epilogue(out, x, x_scale, x_global_scale, weight, weight_scale, weight_global_scale, bias, activation, residual, fresh)
+    return out
 
 
 # one stateless module instance serves every call of the functional form

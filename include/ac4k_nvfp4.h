@@ -429,6 +429,16 @@ int ac4k_block_norm(void *out, int64_t out_stride, void *sf, float *global_scale
                     const void *shift, int64_t shift_stride, int64_t shift_rows, int vector_dtype, int64_t rows, int64_t K, int dtype,
                     int precision, int kind, double residual_scale, double eps, void *workspace, int64_t workspace_bytes, ac4k_stream_t stream);
 
+/* ac4k_linear_nvfp4 with an activation and a residual behind the product (no counterpart in the reference):
+ *   D = round(act((A . B^T) * (*A_gs * *B_gs) + bias) + residual), one rounding, to D's type.
+ * bias [N] or NULL; residual [M, N] of D's type, residual_stride elements between rows, or NULL; it may be D itself.
+ *   RELU max(x, 0);  GELU x Phi(x);  GELU_TANH x / 2 (1 + tanh(sqrt(2 / pi) (x + 0.044715 x^3)));  SILU x / (1 + e^-x).
+ * Operands and kernels as for ac4k_linear_nvfp4.  `workspace`: ac4k_linear_nvfp4_scratch_bytes(M, N, K), on 256 bytes, NULL when that is 0. */
+enum { AC4K_ACTIVATION_NONE = 0, AC4K_ACTIVATION_RELU = 1, AC4K_ACTIVATION_GELU = 2, AC4K_ACTIVATION_GELU_TANH = 3, AC4K_ACTIVATION_SILU = 4 };
+int ac4k_linear_nvfp4_epilogue(void *D, int d_dtype, const void *A, const void *A_sf, const float *A_gs, const void *B, const void *B_sf,
+                               const float *B_gs, const void *bias, int bias_dtype, int activation, const void *residual, int64_t residual_stride,
+                               int64_t M, int64_t N, int64_t K, void *workspace, int64_t workspace_bytes, ac4k_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
