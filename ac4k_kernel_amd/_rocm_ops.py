@@ -889,8 +889,9 @@ def route_experts(logits, k: int, bias, scoring, groups: int, top_groups: int, b
         _same_device(bias)
     if logits.get_device() != _current_device():
         _same_device(logits)
-    shape, new = (*logits.shape[:-1], k), logits.new_empty
-    weights, experts, places = new(shape, dtype=torch.float32), new(shape, dtype=torch.int32), new(shape, dtype=torch.int32)
+    new = logits.new_empty
+    experts = new((*logits.shape[:-1], k), dtype=torch.int32)
+    places, weights = torch.empty_like(experts), torch.empty_like(experts, dtype=torch.float32)
     offsets, rows = new((E + 1,), dtype=torch.int32), new((T * k,), dtype=torch.int32)
     if T == 0:
         offsets.zero_()
@@ -946,34 +947,35 @@ def combine_experts(out, y, weights, places, residual=None):
 
 
 _KINDS = {"rms": 0, "layer": 1}
+_NO_VECTOR = (None, 0, 0, None)
 
 
-def _norm_vector(t, name: str, shape, tag: int, dev):
+def _norm_vector(t, name: str, shape):
     """(address, elements between vectors, rows that share one; 0: all) of one of a block's vectors, [K] or with leading dims that are those of x or,
-    from some dim on, 1."""
-    if t is None:
-        return None, 0, 0
-    _check(t.get_device() == dev, "{} must be on the current device", name)
-    *lead, K = t.shape
-    x_lead = shape[:-1]
-    if K != shape[-1]:
-        _check(False, "{} must have a last dim of {}", name, shape[-1])
-    count = 1
-    for n in lead:
-        count *= n
-    if count == 1 and (len(lead) == len(x_lead) or len(lead) == 0):
-        _check(K == 1 or t.stride(-1) == 1, "{} must have contiguous vectors, evenly apart", name)
-        return t.data_ptr(), 0, 0
-    rows, same = 1, len(x_lead)
-    if len(lead) == len(x_lead):
-        while same and lead[same - 1] == 1:
+    from some dim on, 1; and the tensor that holds it, a copy where no single stride describes it."""
+    t_shape, K = t.shape, shape[-1]
+    if t_shape[-1] != K:
+        _check(False, "{} must have a last dim of {}", name, K)
+    if len(t_shape) == 1:
+        if t.stride(0) != 1 and K > 1:
+            t = t.contiguous()
+        return t.data_ptr(), 0, 0, t
+    same = len(t_shape) - 1
+    if len(t_shape) == len(shape):
+        rows, count = 1, 1
+        while same and t_shape[same - 1] == 1:
             same -= 1
-            rows *= x_lead[same]
-    _check(len(lead) == len(x_lead) and tuple(lead[:same]) == tuple(x_lead[:same]), "{} must be [{}], or have the leading dims of x or 1 from some dim on, not {}", name,
-           K, list(t.shape))
-    v = _rows_view(t, name)
-    _check(v is not None, "{} must have contiguous vectors, evenly apart", name)
-    return t.data_ptr(), v[2], rows
+            rows *= shape[same]
+        for n in t_shape[:same]:
+            count *= n
+        if count == 1 or t_shape[:same] == shape[:same]:
+            view = _rows_view(t, name)
+            if view is None:
+                t = t.contiguous()
+                view = _rows_view(t, name)
+            if t_shape[:same] == shape[:same]:
+                return t.data_ptr(), view[2], 0 if count == 1 else rows, t
+    _check(False, "{} must be [{}], or have the leading dims of x or 1 from some dim on, not {}", name, K, list(t_shape))
 
 
 def block_norm(out, sf, global_scale, given_scale: bool, x, residual, residual_out, weight, post_weight, gate, scale, shift, kind, residual_scale: float,
@@ -996,21 +998,30 @@ def block_norm(out, sf, global_scale, given_scale: bool, x, residual, residual_o
         _same_device(x, residual_out, out, sf, global_scale)
     if (residual is None) != (residual_out is None):
         _check(False, "a residual comes with residual_out, and the other way round")
-    vector_tag = None
-    vectors = (("weight", weight), ("post_weight", post_weight), ("gate", gate), ("scale", scale), ("shift", shift))
-    for name, t in vectors:
-        if t is not None:
-            t_tag = _check_float(t, name)
-            if t_tag != tag and t_tag != 2 or vector_tag not in (None, t_tag):
-                _check(t_tag == tag or t_tag == 2, "{} must have the type of x or be float", name)
-                _check(False, "weight, post_weight, gate, scale and shift must have one type")
-            vector_tag = t_tag
-    for name, t in vectors[:2]:
-        if t is not None and (t.shape != (K,) or not t.is_contiguous() or t.get_device() != dev):
+    vector_type, shape, weight_ptr, post_ptr = None, x.shape, None, None
+    gate_at = scale_at = shift_at = _NO_VECTOR
+    for name, t in (("weight", weight), ("post_weight", post_weight), ("gate", gate), ("scale", scale), ("shift", shift)):
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor) or t.get_device() != dev or (t.dtype is not x.dtype and t.dtype is not torch.float32) or vector_type not in (None, t.dtype):
+            _check_float(t, name)
             _same_device(t)
-            _check(False, "{} must be contiguous of [{}]", name, K)
-    shape = x.shape
-    gate_at, scale_at, shift_at = _norm_vector(gate, "gate", shape, tag, dev), _norm_vector(scale, "scale", shape, tag, dev), _norm_vector(shift, "shift", shape, tag, dev)
+            _check(t.dtype in (x.dtype, torch.float32), "{} must have the type of x or be float", name)
+            _check(False, "weight, post_weight, gate, scale and shift must have one type")
+        vector_type = t.dtype
+        if name == "gate":
+            gate_at = _norm_vector(t, name, shape)
+        elif name == "scale":
+            scale_at = _norm_vector(t, name, shape)
+        elif name == "shift":
+            shift_at = _norm_vector(t, name, shape)
+        else:
+            if t.shape != (K,) or not t.is_contiguous():
+                _check(False, "{} must be contiguous of [{}]", name, K)
+            if name == "weight":
+                weight_ptr = t.data_ptr()
+            else:
+                post_ptr = t.data_ptr()
     residual_ptr = sum_ptr = None
     residual_step = sum_step = 0
     if residual is not None:
@@ -1060,7 +1071,6 @@ def block_norm(out, sf, global_scale, given_scale: bool, x, residual, residual_o
             ws = x.new_empty((nbytes,), dtype=torch.uint8)
             ws_ptr = ws.data_ptr()
     _lib.check(_L.ac4k_block_norm(out.data_ptr(), out_step, None if sf is None else sf.data_ptr(), None if global_scale is None else global_scale.data_ptr(),
-                                  int(given_scale), x.data_ptr(), x_step, residual_ptr, residual_step, sum_ptr, sum_step,
-                                  None if weight is None else weight.data_ptr(), None if post_weight is None else post_weight.data_ptr(), *gate_at, *scale_at,
-                                  *shift_at, tag if vector_tag is None else vector_tag, rows, K, tag, number, kind_number, residual_scale, eps, ws_ptr, nbytes,
-                                  _stream()))
+                                  int(given_scale), x.data_ptr(), x_step, residual_ptr, residual_step, sum_ptr, sum_step, weight_ptr, post_ptr, *gate_at[:3],
+                                  *scale_at[:3], *shift_at[:3], 2 if vector_type is torch.float32 else tag, rows, K, tag, number, kind_number, residual_scale, eps,
+                                  ws_ptr, nbytes, _stream()))

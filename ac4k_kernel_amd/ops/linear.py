@@ -43,7 +43,7 @@ def linear(x, x_scale, x_global_scale, weight, weight_scale, weight_global_scale
         residual = residual.contiguous()
     fresh = out is None
     if fresh:
-        out = torch.empty((x.size(0), weight.size(0)), dtype=torch.bfloat16, device=x.device)
+        out = x.new_empty((x.size(0), weight.size(0)), dtype=torch.bfloat16)
     _rocm_ops.linear_nvfp4_epilogue(out, x, x_scale, x_global_scale, weight, weight_scale, weight_global_scale, bias, activation, residual, fresh)
     return out
 

@@ -110,15 +110,18 @@ def block_norm(x, residual=None, weight=None, *, gate=None, residual_scale=1.0, 
             fresh = False
     elif residual_out is not None:
         raise RuntimeError("residual_out without a residual")
-    types = set()
+    first = None
     for t in (weight, post_weight, gate, scale, shift):
         if t is not None:
             if not isinstance(t, torch.Tensor) or t.dim() < 1:
                 raise RuntimeError("weight, post_weight, gate, scale and shift must be tensors of at least one dim")
-            types.add(t.dtype)
-    if types == {x.dtype, torch.float32}:
-        weight, post_weight, gate, scale, shift = [None if t is None else t.float() for t in (weight, post_weight, gate, scale, shift)]
-    gate, scale, shift = [t if t is None or t.shape[-1] < 1 or _rocm_ops._rows_view(t, "vector") is not None else t.contiguous() for t in (gate, scale, shift)]
+            if first is None:
+                first = t.dtype
+            elif t.dtype is not first:
+                if {t.dtype, first} != {x.dtype, torch.float32}:
+                    raise RuntimeError("weight, post_weight, gate, scale and shift must have the type of x or be float")
+                weight, post_weight, gate, scale, shift = [None if v is None or not isinstance(v, torch.Tensor) else v.float() for v in (weight, post_weight, gate, scale, shift)]
+                break
     rows, k, _ = view
     sf, given = None, global_scale is not None
     if given and precision != "nvfp4":
