@@ -178,14 +178,24 @@ __global__ __launch_bounds__(64 * BW) void norm_rows_kernel(NormArgs a, int rows
   // variance is their difference; elements of 32 bits are squared without the mean.
   auto row_stats = [&](const Vec8<DT>(&v)[NV], float &m1, float &m2, float &r) {
     double s = 0.0, q = 0.0, mean = 0.0, var;
+    if (a.centred) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
+      for (int j = 0; j < NV; ++j)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const double d = (double)vec8_get(v[j], i);
-        if (a.centred) s += d;
-        q = __builtin_fma(d, d, q);
-      }
+        for (int i = 0; i < 8; ++i) {
+          const double d = (double)vec8_get(v[j], i);
+          s += d;
+          q = __builtin_fma(d, d, q);
+        }
+    } else {
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const double d = (double)vec8_get(v[j], i);
+          q = __builtin_fma(d, d, q);
+        }
+    }
     row_sums(s, q);
     var = q * a.inverse_K;
     if (a.centred) {
@@ -257,8 +267,12 @@ __global__ __launch_bounds__(64 * BW) void norm_rows_kernel(NormArgs a, int rows
           for (int i = 0; i < 8; ++i) f[i] = vec8_get(h[j], i);
           if (post) {
             row_piece(v, pp, k, false);
+            if (a.centred) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = ((f[i] - m1) - m2) * pr * vec8_get(v, i);
+              for (int i = 0; i < 8; ++i) f[i] = (f[i] - m1) - m2;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = f[i] * pr * vec8_get(v, i);
           }
           if (gated) {
             row_piece(v, gp, k, false);
@@ -341,7 +355,13 @@ __global__ __launch_bounds__(64 * BW) void norm_rows_kernel(NormArgs a, int rows
     auto values = [&](int j, float (&y)[8]) {
       const int k = (j * LPR + sub) * 8;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = (BLOCK ? (vec8_get(h[j], i) - m1) - m2 : vec8_get(h[j], i)) * r;
+      for (int i = 0; i < 8; ++i) y[i] = vec8_get(h[j], i);
+      if (BLOCK && a.centred) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = (y[i] - m1) - m2;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = y[i] * r;
       if (weighted) {
         Vec8<WT> &v = w[HELD ? j : 0];
         if constexpr (BLOCK) row_piece(v, static_cast<const W *>(a.weight), k, false);

@@ -390,7 +390,8 @@ __global__ __launch_bounds__(1024) void route_plan_kernel(RouteArgs a) {
   constexpr int THREADS = 1024;
   __shared__ int total[AC4K_ROUTE_MAX_EXPERTS];   // rows of the expert, then the start of its range
   __shared__ int before[AC4K_ROUTE_MAX_EXPERTS];  // of them, in front of this workgroup's blocks
-  __shared__ uint16_t base[ROUTE_PLAN_BLOCKS][AC4K_ROUTE_MAX_EXPERTS], mask[ROUTE_PLAN_BLOCKS][AC4K_ROUTE_MAX_EXPERTS];
+  __shared__ uint16_t base[ROUTE_PLAN_BLOCKS][AC4K_ROUTE_MAX_EXPERTS];
+  __shared__ __attribute__((aligned(16))) uint16_t mask[ROUTE_PLAN_BLOCKS * AC4K_ROUTE_MAX_EXPERTS];  // [block][Ep], as they lie in memory
   __shared__ uint32_t part[2][THREADS * 4];       // [run][pair of experts]
   __shared__ int wave_sum[THREADS / 64];
   const int tid = threadIdx.x, E = a.E, columns = a.Ep / 8, runs = THREADS / columns, pairs = columns * 4;
@@ -403,8 +404,11 @@ __global__ __launch_bounds__(1024) void route_plan_kernel(RouteArgs a) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) expert[i] = tid + i * THREADS < slots ? a.experts[t0 * a.k + tid + i * THREADS] : -1;
   for (int e = tid; e < E; e += THREADS) total[e] = before[e] = 0;
-  for (int b = tid >> 6; b < mine; b += THREADS / 64)
-    for (int e = tid & 63; e < E; e += 64) mask[b][e] = a.masks[(b0 + b) * a.Ep + e];
+  const u32x4 *masks = reinterpret_cast<const u32x4 *>(a.masks + b0 * a.Ep);
+  const int vectors = mine * a.Ep / 8;  // at most two a thread
+  u32x4 own[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) own[i] = tid + i * THREADS < vectors ? masks[tid + i * THREADS] : (u32x4){0, 0, 0, 0};
   const int run = tid / columns, column = tid - run * columns;
   if (run < runs) {
     int all[8] = {}, front[8] = {};
@@ -432,6 +436,9 @@ __global__ __launch_bounds__(1024) void route_plan_kernel(RouteArgs a) {
       part[1][run * pairs + column * 4 + i] = (uint32_t)(all[2 * i] | all[2 * i + 1] << 16);
     }
   }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (tid + i * THREADS < vectors) reinterpret_cast<u32x4 *>(mask)[tid + i * THREADS] = own[i];
   __syncthreads();
   {
     const int shares = THREADS / pairs, share = tid / pairs, pair = tid - share * pairs;
@@ -454,7 +461,7 @@ __global__ __launch_bounds__(1024) void route_plan_kernel(RouteArgs a) {
   for (int e = tid; e < E; e += THREADS) {
     int sum = 0, m[ROUTE_PLAN_BLOCKS];
 #pragma unroll
-    for (int b = 0; b < ROUTE_PLAN_BLOCKS; ++b) m[b] = b < mine ? mask[b][e] : 0;
+    for (int b = 0; b < ROUTE_PLAN_BLOCKS; ++b) m[b] = b < mine ? mask[b * a.Ep + e] : 0;
 #pragma unroll
     for (int b = 0; b < ROUTE_PLAN_BLOCKS; ++b) {
       base[b][e] = (uint16_t)sum;
@@ -470,7 +477,7 @@ __global__ __launch_bounds__(1024) void route_plan_kernel(RouteArgs a) {
   for (int i = tid, n = 0; i < slots; i += THREADS, ++n) {
     const int t = i / a.k, slot = i - t * a.k, b = t / ROUTE_TOKENS;
     const int e = n == 0 ? expert[0] : n == 1 ? expert[1] : a.experts[t0 * a.k + i];
-    route_place(a, t0 + t, slot, e, e >= 0 ? mask[b][e] : 0, t % ROUTE_TOKENS, [&](int x) { return total[x] + before[x] + base[b][x]; });
+    route_place(a, t0 + t, slot, e, e >= 0 ? mask[b * a.Ep + e] : 0, t % ROUTE_TOKENS, [&](int x) { return total[x] + before[x] + base[b][x]; });
     if (t0 * a.k + i >= rows) a.rows[t0 * a.k + i] = -1;
   }
 }
