@@ -254,10 +254,14 @@ def linear_nvfp4_epilogue(D, A, A_sf, A_global_scale, B, B_sf, B_global_scale, b
             _check(v is not None, "residual must have rows of contiguous elements, evenly apart")
             residual_ptr, residual_step = residual.data_ptr(), v[2]
         _check(fresh or _same_rows(D, residual) or not _may_overlap(D, residual), "out may be residual itself, but not overlap it otherwise")
-    if not fresh:
-        _check(not any(_may_overlap(D, t) for t in (A, A_sf, A_global_scale, B, B_sf, B_global_scale, bias) if t is not None), "out must not overlap an operand")
     if M == 0 or N == 0:
         return
+    if not fresh:  # all contiguous
+        first = D.data_ptr()
+        end = first + M * N * D.element_size()
+        for t in (A, A_sf, A_global_scale, B, B_sf, B_global_scale, bias):
+            if t is not None and t.data_ptr() < end and first < t.data_ptr() + t.nbytes:
+                _check(False, "out must not overlap an operand")
     nbytes = _L.ac4k_linear_nvfp4_scratch_bytes(M, N, K)
     ws = D.new_empty((nbytes,), dtype=torch.uint8) if nbytes > 0 else None
     _lib.check(_L.ac4k_linear_nvfp4_epilogue(D.data_ptr(), tag, A.data_ptr(), A_sf.data_ptr(), A_global_scale.data_ptr(), B.data_ptr(), B_sf.data_ptr(),

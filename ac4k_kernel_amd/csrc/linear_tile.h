@@ -3,6 +3,7 @@
 #pragma once
 
 #include <atomic>
+#include <type_traits>
 
 #include "linear_common.h"
 
@@ -341,8 +342,9 @@ __device__ __forceinline__ void store_tile(const f32x16 (&acc)[MI][NJ], char *ld
   }
 }
 
-// The same with what BIAS_EPILOGUE adds.  The sums are staged in 32 bits, and everything else happens where the rows leave: a lane has the same columns in all
-// rows, so that its bias stays in registers, and reads the residual in the 16 bytes that it stores, G steps of rows ahead.
+// The same with what BIAS_EPILOGUE adds.  The sums are staged in 32 bits, 32 rows of the wave at a time, and everything else happens where the rows leave: a
+// lane has the same columns in all rows, so that its bias stays in registers, and it reads the residual in the 16 bytes that it stores, one pass ahead.  The passes are
+// a loop, in which only the staging is written out for each: what follows, three times for the activations, is most of the code.
 template <int OUT_DT, int MI, int NJ, int LDS_BYTES>
 __device__ __forceinline__ void store_tile_epilogue(const f32x16 (&acc)[MI][NJ], char *lds, const LinearArgs &a, float scale, int64_t m0, int64_t n0) {
   using DE = Elem<OUT_DT>;
@@ -350,7 +352,7 @@ __device__ __forceinline__ void store_tile_epilogue(const f32x16 (&acc)[MI][NJ],
   constexpr int S = sizeof(DT), V = 16 / S, WN = 32 * NJ, RP = 32;
   constexpr int PITCH = WN * 4 + 16;
   static_assert(4 * RP * PITCH <= LDS_BYTES, "epilogue staging must fit in LDS");
-  constexpr int CPR = WN / V, RS = 64 / CPR, IT = RP / RS, G = IT < 4 ? IT : 4;
+  constexpr int CPR = WN / V, RS = 64 / CPR, IT = RP / RS;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
   const int lrow = lane / CPR, lq = lane % CPR;
   char *stg = lds + wave * (RP * PITCH);
@@ -358,37 +360,36 @@ __device__ __forceinline__ void store_tile_epilogue(const f32x16 (&acc)[MI][NJ],
   const int64_t cl = a.N - n;
   const int cols = cl > V ? V : (int)cl;  // columns of this lane's piece inside the matrix
   const int64_t rl = a.M - m0 - lrow;
-  const int rows_left = cols <= 0 ? 0 : rl > 32 * MI ? 32 * MI : (int)rl;
+  const int rows_left = cols <= 0 ? 0 : rl > 32 * MI ? 32 * MI : (int)rl;  // rows of the block below this lane's first one
+  const bool interior = m0 + 32 * MI <= a.M && n0 + WN <= a.N;
   float bias[V];
 #pragma unroll
   for (int q = 0; q < V; ++q) bias[q] = a.ep.bias && q < cols ? epilogue_bias(a.ep, n + q) : 0.0f;
   const char *res = static_cast<const char *>(a.ep.residual) + ((m0 + lrow) * a.ep.residual_stride + n) * S;
   const int64_t res_step = RS * a.ep.residual_stride * S, out_step = RS * a.N * S;
   char *out = static_cast<char *>(a.D) + ((m0 + lrow) * a.N + n) * S;
-  u32x4 ahead[G];
-  auto fetch = [&](int step) {
+  u32x4 ahead[IT];
+  auto fetch = [&](int row0) {  // the residual of the pass from row0 on
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-      ahead[g] = (u32x4){0, 0, 0, 0};
-      if (a.ep.residual && (step + g) * RS < rows_left) {
-        const char *p = res + (step + g) * res_step;
-        if (cols == V) {
-          ahead[g] = *reinterpret_cast<const u32x4_elem *>(p);
-        } else {
+    for (int it = 0; it < IT; ++it) {
+      const char *p = res + it * res_step;
+      if (interior || (row0 + it * RS < rows_left && cols == V)) {
+        ahead[it] = *reinterpret_cast<const u32x4_elem *>(p);
+      } else if (row0 + it * RS < rows_left) {
+        ahead[it] = (u32x4){0, 0, 0, 0};
 #pragma unroll
-          for (int q = 0; q < V; ++q)
-            if (q < cols) {
-              if constexpr (S == 4) ahead[g][q] = reinterpret_cast<const uint32_t *>(p)[q];
-              else ahead[g][q / 2] |= (uint32_t)reinterpret_cast<const uint16_t *>(p)[q] << (16 * (q & 1));
-            }
-        }
+        for (int q = 0; q < V; ++q)
+          if (q < cols) {
+            if constexpr (S == 4) ahead[it][q] = reinterpret_cast<const uint32_t *>(p)[q];
+            else ahead[it][q / 2] |= (uint32_t)reinterpret_cast<const uint16_t *>(p)[q] << (16 * (q & 1));
+          }
       }
     }
+    res += IT * res_step;
   };
-  fetch(0);
-#pragma unroll
-  for (int i = 0; i < MI; ++i) {
-    asm volatile("" ::: "memory");
+  if (a.ep.residual) fetch(0);
+  auto stage = [&](auto index) {
+    constexpr int i = decltype(index)::value;
 #pragma unroll
     for (int j = 0; j < NJ; ++j)
 #pragma unroll
@@ -401,44 +402,50 @@ __device__ __forceinline__ void store_tile_epilogue(const f32x16 (&acc)[MI][NJ],
         }
         *reinterpret_cast<float4 *>(stg + (lane & 31) * PITCH + (j * 32 + g * 8 + half * 4) * 4) = make_float4(v[0] * scale, v[1] * scale, v[2] * scale, v[3] * scale);
       }
+  };
+  const float4 *src = reinterpret_cast<const float4 *>(stg + lrow * PITCH + lq * V * 4);
+  constexpr int UNROLL = MI * NJ == 16 ? 1 : MI;
+#pragma unroll UNROLL
+  for (int pass = 0; pass < MI; ++pass) {
+    if (pass == 0) stage(std::integral_constant<int, 0>{});
+    else if (pass == 1) stage(std::integral_constant<int, 1 % MI>{});
+    else if (pass == 2) stage(std::integral_constant<int, 2 % MI>{});
+    else stage(std::integral_constant<int, 3 % MI>{});
+    u32x4 now[IT];
+    if (a.ep.residual) {
+#pragma unroll
+      for (int it = 0; it < IT; ++it) now[it] = ahead[it];
+      if (pass + 1 < MI) fetch((pass + 1) * RP);
+    }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the staging block is private to the wave
     with_activation(a.ep.activation, [&](auto act) {
-#pragma unroll 1
-      for (int it = 0; it < IT; it += G) {
-        u32x4 now[G];
 #pragma unroll
-        for (int g = 0; g < G; ++g) now[g] = ahead[g];
-        if (i * IT + it + G < MI * IT) fetch(i * IT + it + G);
+      for (int it = 0; it < IT; ++it) {
+        float v[V];
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-          const int step = i * IT + it + g;
-          const float4 *src = reinterpret_cast<const float4 *>(stg + ((it + g) * RS + lrow) * PITCH + lq * V * 4);
-          float v[V];
-#pragma unroll
-          for (int q = 0; q < V; q += 4) {
-            const float4 f = src[q / 4];
-            v[q] = f.x, v[q + 1] = f.y, v[q + 2] = f.z, v[q + 3] = f.w;
-          }
-          u32x4 o;
-#pragma unroll
-          for (int q = 0; q < V; ++q) v[q] = act(v[q] + bias[q]);
-          if (a.ep.residual) {
-#pragma unroll
-            for (int q = 0; q < V; ++q) {
-              DT r[16 / S];
-              __builtin_memcpy(r, &now[g], 16);
-              v[q] += DE::load(r, q);
-            }
-          }
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            if constexpr (S == 2) o[q] = DE::cvt2(v[2 * q], v[2 * q + 1]);
-            else o[q] = __float_as_uint(v[q]);
-          }
-          if (step * RS < rows_left) store_piece<S>(out + step * out_step, o, cols);
+        for (int q = 0; q < V; q += 4) {
+          const float4 f = src[(it * RS * PITCH) / 16 + q / 4];
+          v[q] = f.x, v[q + 1] = f.y, v[q + 2] = f.z, v[q + 3] = f.w;
         }
+#pragma unroll
+        for (int q = 0; q < V; ++q) v[q] = act(v[q] + bias[q]);
+        if (a.ep.residual) {
+          DT r[V];
+          __builtin_memcpy(r, &now[it], 16);
+#pragma unroll
+          for (int q = 0; q < V; ++q) v[q] += DE::load(r, q);
+        }
+        u32x4 o;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          if constexpr (S == 2) o[q] = DE::cvt2(v[2 * q], v[2 * q + 1]);
+          else o[q] = __float_as_uint(v[q]);
+        }
+        if (interior) *reinterpret_cast<u32x4_elem *>(out + it * out_step) = o;
+        else if (pass * RP + it * RS < rows_left) store_piece<S>(out + it * out_step, o, cols);
       }
     });
+    out += IT * out_step;
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
 }

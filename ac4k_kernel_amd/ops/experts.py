@@ -2,6 +2,8 @@
 experts' rows back to their tokens.  Neither has a counterpart in the reference.  Inference only, as every operator here."""
 from __future__ import annotations
 
+from operator import index
+
 import torch
 
 from .. import _rocm_ops
@@ -27,9 +29,12 @@ def route_experts(logits, top_k, scoring="softmax", bias=None, groups=1, top_gro
     if view is None:
         logits = logits.contiguous()
         view = _rocm_ops._rows_view(logits, "logits")
-    groups = int(groups)
-    return _rocm_ops.route_experts(logits, int(top_k), bias, scoring, groups, groups if top_groups is None else int(top_groups), int(group_best), renormalize,
-                                   float(scale), view)
+    try:
+        top_k, groups, group_best = index(top_k), index(groups), index(group_best)
+        top_groups = groups if top_groups is None else index(top_groups)
+    except TypeError:
+        raise RuntimeError("top_k, groups, top_groups and group_best must be whole numbers") from None
+    return _rocm_ops.route_experts(logits, top_k, bias, scoring, groups, top_groups, group_best, renormalize, float(scale), view)
 
 
 def combine_experts(y, weights, places, residual=None, out=None):

@@ -82,7 +82,7 @@ def bias_of(e, seed=0, std=0.1):
 
 
 SHAPES = [(1, 1, 1), (1, 8, 2), (3, 5, 5), (16, 64, 8), (17, 60, 4), (64, 128, 8), (65, 128, 16), (64, 33, 17), (63, 1000, 64), (130, 256, 8), (129, 97, 6),
-          (200, 512, 6), (66, 1024, 8), (257, 16, 2), (1025, 32, 4)]
+          (200, 512, 6), (66, 1024, 8), (257, 16, 2), (1025, 32, 4), (100, 1, 1), (100, 3, 2), (70, 9, 4), (65, 7, 7)]
 
 
 @pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
@@ -328,7 +328,7 @@ def test_python_refusals_of_combine():
 def test_python_refusals_of_route():
     x = torch.zeros((4, 64), device="cuda")
     r = ops().route_experts
-    for kw in (dict(logits=x.cpu()), dict(logits=x.double()), dict(logits=[1.0]), dict(logits=x[:, :0]), dict(top_k=0), dict(top_k=65), dict(logits=x[:, :4], top_k=5), dict(scoring="relu"),
+    for kw in (dict(logits=x.cpu()), dict(logits=x.double()), dict(logits=[1.0]), dict(logits=x[:, :0]), dict(top_k=0), dict(top_k=65), dict(top_k=2.0), dict(top_k=None), dict(groups="2"), dict(logits=x[:, :4], top_k=5), dict(scoring="relu"),
                dict(bias=torch.zeros(63, device="cuda")), dict(bias=torch.zeros(64)), dict(bias=torch.zeros(64, device="cuda").half()), dict(bias=0.0), dict(groups=3),
                dict(groups=0), dict(groups=4, top_groups=5), dict(groups=4, top_groups=0), dict(groups=4, top_groups=1, top_k=17), dict(group_best=3),
                dict(logits=torch.zeros((2, 1025), device="cuda"))):
