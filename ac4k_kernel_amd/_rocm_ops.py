@@ -234,9 +234,14 @@ def linear_nvfp4_epilogue(D, A, A_sf, A_global_scale, B, B_sf, B_global_scale, b
     number = _ACTIVATIONS.get(activation) if activation is None or isinstance(activation, str) else None
     if number is None:
         _check(False, "activation must be one of {}", list(_ACTIVATIONS))
-    if A is None or A_sf is None or A_global_scale is None or B is None or B_sf is None or B_global_scale is None:
-        _check(False, "operands must be tensors, not NoneType")
-    _same_device(D, A, A_sf, A_global_scale, B, B_sf, B_global_scale, bias, residual)
+    operands = (A, A_sf, A_global_scale, B, B_sf, B_global_scale)
+    dev = _current_device()
+    for t in operands:
+        if not isinstance(t, torch.Tensor) or t.get_device() != dev:
+            _check(t is not None, "operands must be tensors, not NoneType")
+            _same_device(t)
+    if not fresh or bias is not None or residual is not None:
+        _same_device(D, bias, residual)
     _check(A.dim() == 2 and A.size(0) == M, "A size(0) must be {}", M)
     K = _check_linear_operand(A, A_sf, A_global_scale, M, "a")
     if K % 16 != 0:
@@ -259,7 +264,7 @@ def linear_nvfp4_epilogue(D, A, A_sf, A_global_scale, B, B_sf, B_global_scale, b
     if not fresh:  # all contiguous
         first = D.data_ptr()
         end = first + M * N * D.element_size()
-        for t in (A, A_sf, A_global_scale, B, B_sf, B_global_scale, bias):
+        for t in (*operands, bias):
             if t is not None and t.data_ptr() < end and first < t.data_ptr() + t.nbytes:
                 _check(False, "out must not overlap an operand")
     nbytes = _L.ac4k_linear_nvfp4_scratch_bytes(M, N, K)
@@ -926,10 +931,12 @@ def combine_experts(out, y, weights, places, residual=None):
         _check(False, "weights must have the shape of places")
     *lead, k = places.shape
     T = places.numel() // k
-    _same_device(y, weights, places, residual, out)
+    dev = _current_device()
+    if y.get_device() != dev or weights.get_device() != dev or places.get_device() != dev or residual is not None or out is not None:
+        _same_device(y, weights, places, residual, out)
     residual_ptr, residual_step, out_step = None, 0, N
     if residual is not None:
-        if _check_float(residual, "residual") != tag or residual.shape != (*lead, N):
+        if residual.dtype is not y.dtype or residual.shape != (*lead, N):
             _check(False, "residual must have the type of y and shape {}", [*lead, N])
         v = _rows_view(residual, "residual")
         if v is None:
@@ -952,6 +959,16 @@ def combine_experts(out, y, weights, places, residual=None):
 
 _KINDS = {"rms": 0, "layer": 1}
 _NO_VECTOR = (None, 0, 0, None)
+
+
+def _vector_type(t, name: str, x, dev, before):
+    """The type of one of a block's vectors, which is x's or fp32 and that of those before it."""
+    if not isinstance(t, torch.Tensor) or t.get_device() != dev or t.dtype is not before and (before is not None or t.dtype is not x.dtype and t.dtype is not torch.float32):
+        _check_float(t, name)
+        _same_device(t)
+        _check(t.dtype in (x.dtype, torch.float32), "{} must have the type of x or be float", name)
+        _check(False, "weight, post_weight, gate, scale and shift must have one type")
+    return t.dtype
 
 
 def _norm_vector(t, name: str, shape):
@@ -1004,32 +1021,30 @@ def block_norm(out, sf, global_scale, given_scale: bool, x, residual, residual_o
         _check(False, "a residual comes with residual_out, and the other way round")
     vector_type, shape, weight_ptr, post_ptr = None, x.shape, None, None
     gate_at = scale_at = shift_at = _NO_VECTOR
-    for name, t in (("weight", weight), ("post_weight", post_weight), ("gate", gate), ("scale", scale), ("shift", shift)):
-        if t is None:
-            continue
-        if not isinstance(t, torch.Tensor) or t.get_device() != dev or (t.dtype is not x.dtype and t.dtype is not torch.float32) or vector_type not in (None, t.dtype):
-            _check_float(t, name)
-            _same_device(t)
-            _check(t.dtype in (x.dtype, torch.float32), "{} must have the type of x or be float", name)
-            _check(False, "weight, post_weight, gate, scale and shift must have one type")
-        vector_type = t.dtype
-        if name == "gate":
-            gate_at = _norm_vector(t, name, shape)
-        elif name == "scale":
-            scale_at = _norm_vector(t, name, shape)
-        elif name == "shift":
-            shift_at = _norm_vector(t, name, shape)
-        else:
-            if t.shape != (K,) or not t.is_contiguous():
-                _check(False, "{} must be contiguous of [{}]", name, K)
-            if name == "weight":
-                weight_ptr = t.data_ptr()
-            else:
-                post_ptr = t.data_ptr()
+    if weight is not None:
+        vector_type = _vector_type(weight, "weight", x, dev, None)
+        if weight.shape != (K,) or not weight.is_contiguous():
+            _check(False, "weight must be contiguous of [{}]", K)
+        weight_ptr = weight.data_ptr()
+    if post_weight is not None:
+        vector_type = _vector_type(post_weight, "post_weight", x, dev, vector_type)
+        if post_weight.shape != (K,) or not post_weight.is_contiguous():
+            _check(False, "post_weight must be contiguous of [{}]", K)
+        post_ptr = post_weight.data_ptr()
+    if gate is not None:
+        vector_type = _vector_type(gate, "gate", x, dev, vector_type)
+        gate_at = _norm_vector(gate, "gate", shape)
+    if scale is not None:
+        vector_type = _vector_type(scale, "scale", x, dev, vector_type)
+        scale_at = _norm_vector(scale, "scale", shape)
+    if shift is not None:
+        vector_type = _vector_type(shift, "shift", x, dev, vector_type)
+        shift_at = _norm_vector(shift, "shift", shape)
     residual_ptr = sum_ptr = None
     residual_step = sum_step = 0
     if residual is not None:
-        if _check_float(residual, "residual") != tag or residual.shape != shape or residual.get_device() != dev:
+        if not isinstance(residual, torch.Tensor) or residual.dtype is not x.dtype or residual.shape != shape or residual.get_device() != dev:
+            _check_float(residual, "residual")
             _same_device(residual)
             _check(False, "residual must have the type and shape of x")
         v = _rows_view(residual, "residual")

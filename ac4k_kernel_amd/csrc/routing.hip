@@ -24,7 +24,8 @@ struct RouteArgs {
   int32_t *offsets;         // [E + 1]
   int32_t *rows;            // [T * k]
   int32_t *places;          // [T, k]
-  uint16_t *masks;          // [blocks, Ep]: tokens of the block that take the expert; rows of whole vectors of eight
+  uint16_t *masks;          // [blocks, Ep]: tokens of the block that take the expert; rows of whole vectors
+  uint8_t *counts;          // [blocks, Ep]: how many
   int32_t *bases;           // [blocks, E]: rows of the expert in front of the block
   int32_t *totals;          // [E]
   int64_t T, blocks;
@@ -35,7 +36,7 @@ struct RouteArgs {
 
 constexpr int ROUTE_TOKENS = 16;        // of a block
 constexpr int ROUTE_ONE_TOKENS = 64;    // of a call that one workgroup takes
-constexpr int ROUTE_PLAN_BLOCKS = 16;   // of a workgroup that makes the plan in one launch, where all of them read at most so many masks
+constexpr int ROUTE_PLAN_BLOCKS = 16;   // of a workgroup that makes the plan in one launch, where all of them read at most so many counts
 constexpr int64_t ROUTE_PLAN_MASKS = 1 << 25;
 constexpr int ROUTE_SCAN_EXPERTS = 16;  // of a workgroup of the scan
 
@@ -334,7 +335,10 @@ __global__ __launch_bounds__(ROUTE_TOKENS * L) void route_kernel(RouteArgs a) {
     if (e >= 0) atomicOr(&mask[e], 1u << b);
   }
   __syncthreads();
-  for (int e = tid; e < a.Ep; e += THREADS) a.masks[(int64_t)blockIdx.x * a.Ep + e] = (uint16_t)mask[e];
+  for (int e = tid; e < a.Ep; e += THREADS) {
+    a.masks[(int64_t)blockIdx.x * a.Ep + e] = (uint16_t)mask[e];
+    a.counts[(int64_t)blockIdx.x * a.Ep + e] = (uint8_t)__popc(mask[e]);
+  }
 }
 
 // Counts of each expert in the blocks in front of each block: 64 runs of blocks and 16 experts a workgroup
@@ -346,7 +350,7 @@ __global__ __launch_bounds__(64 * ROUTE_SCAN_EXPERTS) void route_scan_kernel(Rou
   int sum = 0;
   if (e < a.E) {
 #pragma unroll 8
-    for (int64_t b = b0; b < b1; ++b) sum += __popc((uint32_t)a.masks[b * a.Ep + e]);
+    for (int64_t b = b0; b < b1; ++b) sum += a.counts[b * a.Ep + e];
   }
   part[run][x] = sum;
   __syncthreads();
@@ -357,7 +361,7 @@ __global__ __launch_bounds__(64 * ROUTE_SCAN_EXPERTS) void route_scan_kernel(Rou
 #pragma unroll 8
   for (int64_t b = b0; b < b1; ++b) {
     a.bases[b * a.E + e] = before;
-    before += __popc((uint32_t)a.masks[b * a.Ep + e]);
+    before += a.counts[b * a.Ep + e];
   }
 }
 
@@ -383,18 +387,19 @@ __global__ __launch_bounds__(256) void route_place_kernel(RouteArgs a) {
   }
 }
 
-// The same in one launch where there are few masks: every workgroup counts all of them itself and places the tokens of ROUTE_PLAN_BLOCKS
-// blocks.  A thread counts eight experts in every runs-th block; a thread's counts are under 2^16 (16 tokens a mask, at most 2^25 masks in all workgroups),
-// and the runs' counts meet as pairs.  (By an atomic add for each thread and expert the launch took 8.5 us at 16384 x 128.)
+// The same in one launch where there are few blocks: every workgroup counts all of them itself and places the tokens of ROUTE_PLAN_BLOCKS
+// blocks.  A thread adds the counts of 16 experts in every runs-th block, as bytes (eight blocks of 16 tokens at a time) and then as pairs of 16 bits (at most 2^25 masks
+// read in all workgroups: under 1500 a thread).  (With the bits counted here, a vector's eight experts one by one, 1164 vector instructions a wave took 11.4 us at
+// 16384 x 128.)
 __global__ __launch_bounds__(1024) void route_plan_kernel(RouteArgs a) {
   constexpr int THREADS = 1024;
   __shared__ int total[AC4K_ROUTE_MAX_EXPERTS];   // rows of the expert, then the start of its range
   __shared__ int before[AC4K_ROUTE_MAX_EXPERTS];  // of them, in front of this workgroup's blocks
   __shared__ uint16_t base[ROUTE_PLAN_BLOCKS][AC4K_ROUTE_MAX_EXPERTS];
   __shared__ __attribute__((aligned(16))) uint16_t mask[ROUTE_PLAN_BLOCKS * AC4K_ROUTE_MAX_EXPERTS];  // [block][Ep], as they lie in memory
-  __shared__ uint32_t part[2][THREADS * 4];       // [run][pair of experts]
+  __shared__ uint32_t part[2][THREADS * 8];       // [run][pair of experts e, e + 2]
   __shared__ int wave_sum[THREADS / 64];
-  const int tid = threadIdx.x, E = a.E, columns = a.Ep / 8, runs = THREADS / columns, pairs = columns * 4;
+  const int tid = threadIdx.x, E = a.E, columns = a.Ep / 16, runs = THREADS / columns, pairs = columns * 8;
   const int64_t b0 = (int64_t)blockIdx.x * ROUTE_PLAN_BLOCKS;
   const int mine = (int)(a.blocks - b0 < ROUTE_PLAN_BLOCKS ? a.blocks - b0 : ROUTE_PLAN_BLOCKS);
   // the experts of the first slots are under way while the masks are counted
@@ -411,29 +416,30 @@ __global__ __launch_bounds__(1024) void route_plan_kernel(RouteArgs a) {
   for (int i = 0; i < 2; ++i) own[i] = tid + i * THREADS < vectors ? masks[tid + i * THREADS] : (u32x4){0, 0, 0, 0};
   const int run = tid / columns, column = tid - run * columns;
   if (run < runs) {
-    int all[8] = {}, front[8] = {};
-    constexpr int CHUNK = 8;  // loads under way at once: the masks come from other XCDs, a microsecond away
+    uint32_t all[8] = {}, front[8] = {};
+    constexpr int CHUNK = 8;  // loads under way at once: the counts come from other XCDs, a microsecond away
     for (int64_t b = run; b < a.blocks; b += CHUNK * runs) {
-      u32x4 v[CHUNK];
+      u32x4 v[CHUNK], bytes = {0, 0, 0, 0}, front_bytes = {0, 0, 0, 0};
 #pragma unroll
       for (int c = 0; c < CHUNK; ++c) {
         const int64_t at = b + c * runs;
-        v[c] = at < a.blocks ? *reinterpret_cast<const u32x4 *>(a.masks + at * a.Ep + column * 8) : (u32x4){0, 0, 0, 0};
+        v[c] = at < a.blocks ? *reinterpret_cast<const u32x4 *>(a.counts + at * a.Ep + column * 16) : (u32x4){0, 0, 0, 0};
       }
 #pragma unroll
       for (int c = 0; c < CHUNK; ++c) {
-        const u32x4 f = b + c * runs < b0 ? v[c] : (u32x4){0, 0, 0, 0};
+        bytes += v[c];
+        if (b + c * runs < b0) front_bytes += v[c];
+      }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          all[i] += __popc(i & 1 ? v[c][i / 2] >> 16 : v[c][i / 2] & 0xffffu);
-          front[i] += __popc(i & 1 ? f[i / 2] >> 16 : f[i / 2] & 0xffffu);
-        }
+      for (int i = 0; i < 8; ++i) {
+        all[i] += bytes[i / 2] >> (8 * (i & 1)) & 0x00ff00ffu;
+        front[i] += front_bytes[i / 2] >> (8 * (i & 1)) & 0x00ff00ffu;
       }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      part[0][run * pairs + column * 4 + i] = (uint32_t)(front[2 * i] | front[2 * i + 1] << 16);
-      part[1][run * pairs + column * 4 + i] = (uint32_t)(all[2 * i] | all[2 * i + 1] << 16);
+    for (int i = 0; i < 8; ++i) {
+      part[0][run * pairs + column * 8 + i] = front[i];
+      part[1][run * pairs + column * 8 + i] = all[i];
     }
   }
 #pragma unroll
@@ -448,13 +454,14 @@ __global__ __launch_bounds__(1024) void route_plan_kernel(RouteArgs a) {
         const uint32_t f = part[0][r * pairs + pair], t = part[1][r * pairs + pair];
         f0 += f & 0xffffu, f1 += f >> 16, t0 += t & 0xffffu, t1 += t >> 16;
       }
-      if (2 * pair < E) {
-        atomicAdd(&before[2 * pair], (int)f0);
-        atomicAdd(&total[2 * pair], (int)t0);
+      const int e = pair / 8 * 16 + pair % 8 / 2 * 4 + pair % 2;
+      if (e < E) {
+        atomicAdd(&before[e], (int)f0);
+        atomicAdd(&total[e], (int)t0);
       }
-      if (2 * pair + 1 < E) {
-        atomicAdd(&before[2 * pair + 1], (int)f1);
-        atomicAdd(&total[2 * pair + 1], (int)t1);
+      if (e + 2 < E) {
+        atomicAdd(&before[e + 2], (int)f1);
+        atomicAdd(&total[e + 2], (int)t1);
       }
     }
   }
@@ -566,7 +573,7 @@ static int route_width(const RouteArgs &a, hipStream_t st) {
 static int64_t route_workspace(int64_t T, int64_t E) {
   if (T <= ROUTE_ONE_TOKENS) return 0;
   const int64_t blocks = ceil_div(T, ROUTE_TOKENS);
-  return 4 * align_up(E, 4) + 4 * align_up(blocks * E, 4) + 2 * blocks * align_up(E, 8);
+  return 4 * align_up(E, 4) + 4 * align_up(blocks * E, 4) + 3 * blocks * align_up(E, 16);
 }
 
 // ---------------------------------------------------------------------------
@@ -650,12 +657,13 @@ extern "C" __attribute__((visibility("default"))) int ac4k_route_experts(
   AC4K_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0), "workspace of %lld bytes needed, on 16 bytes", (long long)need);
   RouteArgs a{};
   a.logits = logits, a.stride = stride, a.bias = bias, a.weights = weights, a.experts = experts, a.offsets = offsets, a.rows = rows, a.places = places;
-  a.T = T, a.blocks = ceil_div(T, ROUTE_TOKENS), a.E = (int)E, a.Ep = (int)align_up(E, 8), a.k = (int)k;
+  a.T = T, a.blocks = ceil_div(T, ROUTE_TOKENS), a.E = (int)E, a.Ep = (int)align_up(E, 16), a.k = (int)k;
   a.groups = (int)(top_groups == groups ? 1 : groups), a.top_groups = (int)top_groups, a.best = best, a.group_size = (int)(E / a.groups);
   a.sigmoid = scoring == AC4K_SCORE_SIGMOID, a.renormalize = renormalize != 0, a.scale = scale;
   a.totals = static_cast<int32_t *>(workspace);
   a.bases = a.totals + align_up(E, 4);
   a.masks = reinterpret_cast<uint16_t *>(a.bases + align_up(a.blocks * E, 4));
+  a.counts = reinterpret_cast<uint8_t *>(a.masks + a.blocks * a.Ep);
   hipStream_t st = (hipStream_t)stream;
   int rc;
   if (dtype == AC4K_DTYPE_BF16) rc = route_width<AC4K_DTYPE_BF16>(a, st);
