@@ -174,8 +174,8 @@ __global__ __launch_bounds__(64 * BW) void norm_rows_kernel(NormArgs a, int rows
       flip ^= 1;
     }
   };
-  // BLOCK: mean (in two pieces; 0 where rows are not centred) and factor of a row.  Sums of 16-bit elements and of their squares lose nothing next to 64 bits, and the
-  // variance is their difference; elements of 32 bits are squared without the mean.
+  // BLOCK: mean (in two pieces; 0 where rows are not centred) and factor of a row.  Sums of 16-bit elements and of their squares lose nothing in 64 bits
+  // where the elements are of one size, and K^2 times the variance is K times the second less the square of the first; elements of 32 bits are squared without the mean.
   auto row_stats = [&](const Vec8<DT>(&v)[NV], float &m1, float &m2, float &r) {
     double s = 0.0, q = 0.0, mean = 0.0, var;
     if (a.centred) {
@@ -214,8 +214,8 @@ __global__ __launch_bounds__(64 * BW) void norm_rows_kernel(NormArgs a, int rows
         row_sums(s, q);
         var = q * a.inverse_K;
       } else {
-        var = __builtin_fma(-mean, s, q);
-        var = var < 0.0 ? 0.0 : var * a.inverse_K;  // (NaN stays)
+        var = __builtin_fma(-s, s, (double)a.K * q);
+        var = var < 0.0 ? 0.0 : var * (a.inverse_K * a.inverse_K);  // (NaN stays)
       }
     }
     m1 = (float)mean;

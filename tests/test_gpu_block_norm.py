@@ -193,6 +193,17 @@ def test_rows_of_one_value():
     assert (y == 0).all()
 
 
+@pytest.mark.parametrize("dtype,value,other", [("fp16", 1000.0, 1000.5), ("bf16", 1000.0, 1004.0), ("bf16", -3.0, -3.015625), ("fp16", 0.25, 0.250244140625)])
+def test_rows_of_one_value_but_for_one_element(dtype, value, other):
+    """The variance is a 2^-37th of the square of the mean at the least: what 64 bits hold of the difference has to do."""
+    for k in (3000, 32768):
+        x = torch.full((4, k), value)
+        x[torch.arange(4), torch.tensor([0, 7, 1000, k - 1])] = other
+        a = dict(x=x.to(DTYPES[dtype]), kind="layer", eps=0.0)
+        Reference(**a).check(run(a))
+        Reference(**a).check(run(a, "int8"), "int8")
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
 def test_values_near_the_largest_of_the_type(dtype):
     big = 2.0 ** 126
