@@ -4,7 +4,13 @@
 //   h = round(residual_scale * residual + gate * u)                     (x's type; x itself without a residual)
 //   y = (h - mean(h)) / sqrt(var(h) + eps) * weight * (1 + scale) + shift
 // and y leaves as from rms_norm, with whose kernel it is computed (norm_rows.h): in x's type or in the format of a quantizer, from 32 bits.  Sums, means and
-// squares are held in 64 bits, the squares of what is left without the mean; the mean is taken off in two pieces of 32 bits.
+// squares are held in 64 bits; the mean is taken off in two pieces of 32 bits.
+//
+// Bound by memory where rows have whole vectors: 75600 x 5120 bf16, layer norm with gate, scale and shift of one sequence, 600 us, 5.2 TB/s, the rate of a copy (1477 MiB
+// read, 1477 written; the vector port is busy for 50 %).  8192 x 4096 with post norm and gate to nvfp4 53 + 25 us, where one pass over its bytes takes 42: the second launch reads h
+// again, and the first one's port is busy for 65 %.  Rows that end inside a vector, 4002 x 5003 layer norm to int8 with vectors in fp32, 53 us where the bytes need 27:
+// every row reads its three vectors of 20 KB through the caches, at no alignment.  One row of 8192 with post norm to e4m3 5.4 us (rms_norm 3.7).
+// As first built, with all vectors held in registers ahead of their use, 198 to 256 registers left one or two waves on a SIMD: 983, 65 + 25 and 124 us.
 #include "norm_rows.h"
 
 using namespace ac4k;

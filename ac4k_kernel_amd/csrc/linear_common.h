@@ -1,4 +1,4 @@
-// What the linear kernels of linear.hip and linear_fused.hip share.
+// What the linear kernels of linear_kernels.h, linear_fused.hip and linear_grouped.hip share.
 #pragma once
 
 #include "ac4k_common.h"

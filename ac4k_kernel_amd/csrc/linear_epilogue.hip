@@ -1,5 +1,9 @@
 // The linear with an activation and a residual in its epilogue:  D = round(act((A . B^T) * (gsA*gsB) + bias) + residual).  The kernels, plans and scratch are those of
 // the plain linear (linear_kernels.h); bias, activation and residual follow the sums in 32 bits, and there is one rounding, to D's type.
+//
+// What it costs over the plain linear on the same card, us (plain / relu / silu / gelu / residual / gelu and residual): 8192 x 14336 x 4096 bf16 654 / 677 / 696 / 727 / 703 /
+// 754 - gelu is 24 instructions' time an output, which nothing hides with one wave on a SIMD, the residual 235 MB -; 1001 x 5003 x 2880 fp32 35.9 / 36.8 / 38.1 / 39.3 / 40.4 /
+// 43.4.  1 x 14336 x 4096 10.7 alone, as the plain one.  Activations on the sums where they are, in the accumulation registers, spilled them: 1050 to 1150 us.
 #include "linear_kernels.h"
 
 namespace ac4k {

@@ -1,4 +1,4 @@
-// The tile kernel of the NVFP4 linears, as a function of a workgroup: linear.hip runs it on the tiles of one matrix, linear_grouped.hip on those of
+// The tile kernel of the NVFP4 linears, as a function of a workgroup: linear_kernels.h runs it on the tiles of one matrix, linear_grouped.hip on those of
 // the experts' ones.
 #pragma once
 

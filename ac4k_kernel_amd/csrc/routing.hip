@@ -11,6 +11,10 @@
 // The plan is a counting sort by expert that keeps the order of the tokens: a block of 16 tokens keeps, for each expert, the set of its tokens as bits;
 // counts of the blocks in front and bits below a token's own are its place.  Bits are set by atomic ors, whose order does not matter, so every
 // call gives the same plan.
+//
+// Bound by launches and by vector instructions, not by bytes: 16 tokens of 64 experts 3.7 us in one workgroup; 16384 tokens to 4 of 128 experts 6.0 + 7.1 us (choice, plan)
+// where 5.2 MB of bytes need one; 4001 to 8 of 256 with groups and a bias 11.1 + 6.7: 940 vector instructions a wave, a third of them the choice's eight rounds, a
+// quarter scores in 64 bits (the port busy for 72 %).  Scores in 64 bits take 2.3 us there, each round 0.35 to 0.43.
 #include "elements.h"
 
 namespace ac4k {
@@ -588,7 +592,8 @@ struct CombineArgs {
   int k;
 };
 
-// A thread takes eight columns of a token; its places and weights are scalars of the wave.  Rows are read eight at a time.
+// A thread takes eight columns of a token; its places and weights are scalars of the wave.  Rows are read eight at a time.  Bound by memory: 8192 tokens of 8 rows of 4096
+// with a residual 130 us, 5.2 TB/s, the rate of a copy; every row is read once, whole.  16 tokens 3.7 us, a chain of places, rows and store.
 template <int DT>
 __global__ __launch_bounds__(256) void combine_kernel(CombineArgs a, uint32_t spans) {
   using T = typename Elem<DT>::T;
