@@ -281,6 +281,24 @@ def test_outputs_in_place(kind):
     assert (buffer[..., :11] == 7).all() and (buffer[..., 344:] == 7).all()
 
 
+def test_one_tensor_as_both_operands_and_shared_rows():
+    a = problem((30, 1000), kind="layer", gate="vector", post=True)
+    a["residual"] = a["x"]
+    y, h = run(a)
+    Reference(**a).check((y, h))
+    g = on_gpu(a)
+    x = g["x"]
+    got = ops().block_norm(**{**g, "residual": x}, residual_out=x)
+    assert got[1] is x and torch.equal(got[0], y) and torch.equal(x, h)
+    # one row for all of the residual; windows of one buffer as rows
+    a = problem((30, 1000))
+    a["residual"] = a["residual"][:1].expand(30, 1000)
+    Reference(**a).check(run(a))
+    buffer = data((5000,), torch.bfloat16).cuda()
+    windows = buffer.as_strided((64, 1000), (50, 1))
+    assert torch.equal(ops().block_norm(windows, kind="layer"), ops().block_norm(windows.contiguous(), kind="layer"))
+
+
 def test_no_rows():
     for precision in PRECISIONS:
         x = torch.zeros((2, 0, 96), device="cuda")

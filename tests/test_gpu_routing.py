@@ -314,6 +314,24 @@ def test_combine_into_the_residual_and_strided_operands():
     assert torch.equal(ops().combine_experts(y.t().contiguous().t(), weights, places, residual=before[:, 5:205].t().contiguous().t().unflatten(0, (2, 4))), out)
 
 
+def test_combine_on_rows_that_are_read_often():
+    y = torch.randn((7, 520), device="cuda", dtype=torch.float16)
+    places = torch.zeros((50, 4), dtype=torch.int32, device="cuda")
+    places[:, 2] = 6
+    weights = torch.full((50, 4), 0.25, device="cuda")
+    r = torch.randn((1, 520), device="cuda", dtype=torch.float16).expand(50, 520)
+    got = ops().combine_experts(y, weights, places, residual=r)
+    close(got, *combined(y, weights, places, r), 4)
+    assert (got == got[0]).all()
+
+
+def test_routing_of_an_output_that_records_gradients():
+    x = torch.randn((20, 32), device="cuda", requires_grad=True)
+    got = ops().route_experts(x * 2, 3)
+    check(got, reference(x * 2, 3))
+    assert not any(t.requires_grad for t in got)
+
+
 def test_python_refusals_of_combine():
     y, w, p = torch.zeros((8, 64), device="cuda"), torch.zeros((4, 2), device="cuda"), torch.zeros((4, 2), dtype=torch.int32, device="cuda")
     r = torch.zeros((4, 64), device="cuda")
