@@ -7,8 +7,8 @@
 // squares are held in 64 bits; the mean is taken off in two pieces of 32 bits.
 //
 // Bound by memory where rows have whole vectors: 75600 x 5120 bf16, layer norm with gate, scale and shift of one sequence, 600 us, 5.2 TB/s, the rate of a copy (1477 MiB
-// read, 1477 written; the vector port is busy for 50 %).  8192 x 4096 with post norm and gate to nvfp4 53 + 25 us, where one pass over its bytes takes 42: the second launch reads h
-// again, and the first one's port is busy for 65 %.  Rows that end inside a vector, 4002 x 5003 layer norm to int8 with vectors in fp32, 53 us where the bytes need 27:
+// read, 1477 written; the vector port is busy for 50 %).  8192 x 4096 with post norm and gate to nvfp4 49 + 25 us, where one pass over its bytes takes 42: the second launch reads h
+// again, and the first one's port is busy for 72 %.  Rows that end inside a vector, 4002 x 5003 layer norm to int8 with vectors in fp32, 48 us where the bytes need 27:
 // every row reads its three vectors of 20 KB through the caches, at no alignment.  One row of 8192 with post norm to e4m3 5.4 us (rms_norm 3.7).
 // As first built, with all vectors held in registers ahead of their use, 198 to 256 registers left one or two waves on a SIMD: 983, 65 + 25 and 124 us.
 #include "norm_rows.h"
@@ -19,7 +19,7 @@ static bool float_tag(int d) { return d == AC4K_DTYPE_BF16 || d == AC4K_DTYPE_FP
 
 extern "C" __attribute__((visibility("default"))) int64_t ac4k_block_norm_workspace_bytes(int64_t rows, int64_t K, int dtype, int precision, int given_scale) {
   if (rows < 1 || K < 1 || K > AC4K_BLOCK_NORM_MAX_COLS || !float_tag(dtype) || precision != AC4K_PRECISION_NVFP4 || given_scale) return 0;
-  const int64_t factors = norm_workspace(rows, K, dtype);
+  const int64_t factors = norm_workspace(rows, K, dtype, NORM_BLOCK);
   return factors ? factors + 8 * rows : 0;  // the means behind them
 }
 

@@ -137,7 +137,7 @@ static bool float_tag(int d) { return d == AC4K_DTYPE_BF16 || d == AC4K_DTYPE_FP
 extern "C" __attribute__((visibility("default"))) int64_t ac4k_rms_norm_workspace_bytes(int64_t rows, int64_t K, int dtype, int precision,
                                                                                        int given_scale) {
   if (rows < 1 || K < 1 || K > AC4K_NORM_MAX_COLS || !float_tag(dtype) || precision != AC4K_PRECISION_NVFP4 || given_scale) return 0;
-  return norm_workspace(rows, K, dtype);
+  return norm_workspace(rows, K, dtype, NORM_ROWS);
 }
 
 extern "C" __attribute__((visibility("default"))) int ac4k_rms_norm(
