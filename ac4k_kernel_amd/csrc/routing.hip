@@ -657,7 +657,8 @@ extern "C" __attribute__((visibility("default"))) int ac4k_route_experts(
   AC4K_REQUIRE(best == 1 || best == 2, "a group's score is that of its best one or two, not %d", best);
   AC4K_REQUIRE(k >= 1 && k <= AC4K_ROUTE_MAX_K && k <= E / groups * top_groups, "k must be 1 to %d and at most the %lld experts of the groups taken, got %lld",
                (int)AC4K_ROUTE_MAX_K, (long long)(E / groups * top_groups), (long long)k);
-  AC4K_REQUIRE(T * k < (1ll << 27) && T < (1ll << 26), "too many tokens (%lld of %lld experts)", (long long)T, (long long)k);
+  AC4K_REQUIRE(T * k < (1ll << 27) && T <= (1ll << 26) - ROUTE_TOKENS, "too many tokens (%lld of %lld experts)", (long long)T,
+               (long long)k);  // 2^32 threads a launch
   const int64_t need = route_workspace(T, E);
   AC4K_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0), "workspace of %lld bytes needed, on 16 bytes", (long long)need);
   RouteArgs a{};

@@ -42,6 +42,7 @@ def test_route_at_the_c_abi():
     refused(route(k=65), b"k must be")
     refused(route(groups=16, top_groups=1, k=5), b"k must be")
     refused(route(T=1 << 26, k=2), b"too many tokens")
+    refused(route(T=(1 << 26) - 15, k=1), b"too many tokens")  # 2^22 workgroups of 1024 threads
     refused(route(T=1000), b"workspace")
     need = lib().ac4k_route_experts_workspace_bytes(1000, 64, 4)
     assert need > 0
