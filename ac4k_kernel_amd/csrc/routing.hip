@@ -41,7 +41,7 @@ struct RouteArgs {
 constexpr int ROUTE_TOKENS = 16;        // of a block
 constexpr int ROUTE_ONE_TOKENS = 64;    // of a call that one workgroup takes
 constexpr int ROUTE_PLAN_BLOCKS = 16;   // of a workgroup that makes the plan in one launch, where all of them read at most so many counts
-constexpr int64_t ROUTE_PLAN_MASKS = 1 << 25;
+constexpr int64_t ROUTE_PLAN_COUNTS = 1 << 25;
 constexpr int ROUTE_SCAN_EXPERTS = 16;  // of a workgroup of the scan
 
 // Floats and doubles as unsigned numbers of the same order; 0 is -inf (not to be taken), all ones NaN
@@ -540,7 +540,7 @@ static void launch_route(const RouteArgs &a, hipStream_t st) {
   }
   hipLaunchKernelGGL((route_kernel<DT, L, PER, WIDE>), dim3((unsigned)a.blocks), dim3(ROUTE_TOKENS * L), 0, st, a);
   const int64_t groups = ceil_div(a.blocks, ROUTE_PLAN_BLOCKS);
-  if (groups * a.blocks * a.E <= ROUTE_PLAN_MASKS) {
+  if (groups * a.blocks * a.E <= ROUTE_PLAN_COUNTS) {
     hipLaunchKernelGGL(route_plan_kernel, dim3((unsigned)groups), dim3(1024), 0, st, a);
     return;
   }

@@ -13,7 +13,8 @@ def route_experts(logits, top_k, scoring="softmax", bias=None, groups=1, top_gro
     """Each token's top_k experts by router logits [.., E] (bf16, fp16 or fp32, E up to 1024, top_k up to 64), and the plan of the linears behind.
 
     The score of an expert is the softmax over all E logits, or with scoring="sigmoid" 1 / (1 + exp(-logit)); its key is the score plus bias
-    (fp32 [E], for balance).  A token takes the experts of the largest keys, ties to the lowest index.  With top_groups, E is cut into `groups` equal
+    (fp32 [E], for balance), both in 64 bits; without a bias (and with group_best=1) the logits themselves are compared, whose order is the same.  A token
+    takes the experts of the largest keys, ties to the lowest index.  With top_groups, E is cut into `groups` equal
     ranges, and only experts of those top_groups ranges are taken whose group_best (1 or 2) largest keys have the largest sum.  Its weights are the
     scores, without the bias, over their sum with renormalize, times scale.
     An expert with a logit of -inf is not taken: a token with fewer than top_k others has expert -1, weight 0 and place -1 in its last slots, a
