@@ -69,7 +69,7 @@ SIGNATURES = {
                          _vp, _int, _i64, _i64, _i64, ctypes.POINTER(_i64), _int, _int, _vp]),
     "ac4k_linear_grouped_nvfp4_workspace_bytes": (_i64, [_i64] * 5 + [_int]),
     "ac4k_debug_last_grouped_kernel": (_int, []),
-    "ac4k_route_experts_workspace_bytes": (_i64, [_i64] * 3),
+    "ac4k_route_experts_workspace_bytes": (_i64, [_i64] * 5),
     "ac4k_route_experts": (_int, [_vp] * 6 + [_int, _i64, _vp] + [_i64] * 3 + [_int, _i64, _i64, _int, _int, ctypes.c_double, _vp, _i64, _vp]),
     "ac4k_block_norm_workspace_bytes": (_i64, [_i64, _i64, _int, _int, _int]),
     "ac4k_block_norm": (_int, [_vp, _i64, _vp, _vp, _int] + [_vp, _i64] * 3 + [_vp, _vp] + [_vp, _i64, _i64] * 3 + [_int, _i64, _i64] + [_int] * 3 +

@@ -905,7 +905,7 @@ def route_experts(logits, k: int, bias, scoring, groups: int, top_groups: int, b
     if T == 0:
         offsets.zero_()
         return weights, experts, offsets, rows, places
-    nbytes = _L.ac4k_route_experts_workspace_bytes(T, E, k) if T > 64 else 0
+    nbytes = _L.ac4k_route_experts_workspace_bytes(T, E, k, groups, top_groups) if T > 64 else 0
     ws_ptr = None
     if nbytes > 0:
         ws = new((nbytes,), dtype=torch.uint8)

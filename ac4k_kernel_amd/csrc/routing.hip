@@ -39,7 +39,11 @@ struct RouteArgs {
 };
 
 constexpr int ROUTE_TOKENS = 16;        // of a block
-constexpr int ROUTE_ONE_TOKENS = 64;    // of a call that one workgroup takes
+constexpr int ROUTE_ROW_EXPERTS = 128;  // up to so many, without groups and up to 16 a token, 16 lanes take a token; otherwise a wave
+static int route_lanes(int64_t E, int64_t k, int64_t groups) { return groups == 1 && k <= 16 && E <= ROUTE_ROW_EXPERTS ? 16 : 64; }
+// Tokens of a call that one workgroup takes: 128 to 8 of 64 experts 9.4 us on the GPU and 13.4 for the caller, where two launches of 129 need 8.2 and 17.3;
+// 256 would need 16.8 and 16.8.
+constexpr int route_one_tokens(int lanes) { return lanes == 16 ? 128 : 64; }
 constexpr int ROUTE_PLAN_BLOCKS = 16;   // of a workgroup that makes the plan in one launch, where all of them read at most so many counts
 constexpr int64_t ROUTE_PLAN_COUNTS = 1 << 25;
 constexpr int ROUTE_SCAN_EXPERTS = 16;  // of a workgroup of the scan
@@ -493,47 +497,63 @@ __global__ __launch_bounds__(1024) void route_plan_kernel(RouteArgs a) {
   }
 }
 
-// All of a small call in one workgroup
+// All of a small call in one workgroup, THREADS / L tokens at a time
 template <int DT, int L, int PER, bool WIDE, int THREADS>
 __global__ __launch_bounds__(THREADS) void route_one_kernel(RouteArgs a) {
-  __shared__ unsigned long long mask[AC4K_ROUTE_MAX_EXPERTS];
-  __shared__ int start[AC4K_ROUTE_MAX_EXPERTS];
+  constexpr int AT_ONCE = THREADS / L, TURNS = THREADS == 256 ? 1 : route_one_tokens(L) / AT_ONCE, WORDS = (AT_ONCE * TURNS + 63) / 64;
+  constexpr int EXPERTS = L == 16 ? ROUTE_ROW_EXPERTS : AC4K_ROUTE_MAX_EXPERTS;
+  __shared__ unsigned long long mask[WORDS][EXPERTS];  // tokens of each expert
+  __shared__ int start[EXPERTS];
+  __shared__ int16_t chosen[TURNS * THREADS];
   __shared__ int wave_sum[THREADS / 64];
-  constexpr int AT_ONCE = THREADS / L, TURNS = THREADS == 256 ? 1 : ROUTE_ONE_TOKENS / AT_ONCE;
   const int tid = threadIdx.x, sub = tid % L;
-  for (int e = tid; e < a.E; e += THREADS) mask[e] = 0;
-  __syncthreads();
-  int mine[TURNS];
+  for (int e = tid; e < a.E; e += THREADS) {
 #pragma unroll
-  for (int i = 0; i < TURNS; ++i) {
-    const int t = i * AT_ONCE + tid / L;
-    mine[i] = -1;
-    if (i * AT_ONCE + (tid & ~63) / L >= a.T) continue;  // a whole wave
-    float w;
-    route_token<DT, L, PER, WIDE>(a, t, t < a.T, sub, mine[i], w);
-    if (t < a.T && sub < a.k) {
-      a.experts[(int64_t)t * a.k + sub] = mine[i];
-      a.weights[(int64_t)t * a.k + sub] = w;
-      if (mine[i] >= 0) atomicOr(&mask[mine[i]], 1ull << t);
-    }
+    for (int w = 0; w < WORDS; ++w) mask[w][e] = 0;
   }
   __syncthreads();
-  for (int e = tid; e < a.E; e += THREADS) start[e] = __popcll(mask[e]);
+#pragma unroll 1
+  for (int i = 0; i * AT_ONCE < a.T && i < TURNS; ++i) {
+    const int t = i * AT_ONCE + tid / L;
+    int mine = -1;
+    if (i * AT_ONCE + (tid & ~63) / L < a.T) {  // a whole wave
+      float w;
+      route_token<DT, L, PER, WIDE>(a, t, t < a.T, sub, mine, w);
+      if (t < a.T && sub < a.k) {
+        a.experts[(int64_t)t * a.k + sub] = mine;
+        a.weights[(int64_t)t * a.k + sub] = w;
+        if (mine >= 0) atomicOr(&mask[t >> 6][mine], 1ull << (t & 63));
+      }
+    }
+    chosen[i * THREADS + tid] = (int16_t)mine;
+  }
+  __syncthreads();
+  for (int e = tid; e < a.E; e += THREADS) {
+    int sum = 0;
+#pragma unroll
+    for (int w = 0; w < WORDS; ++w) sum += __popcll(mask[w][e]);
+    start[e] = sum;
+  }
   __syncthreads();
   const int total = route_starts<THREADS>(start, a.E, wave_sum);
   for (int e = tid; e < a.E; e += THREADS) a.offsets[e] = start[e];
   if (tid == 0) a.offsets[a.E] = total;
-#pragma unroll
-  for (int i = 0; i < TURNS; ++i) {
-    const int t = i * AT_ONCE + tid / L;
-    if (t < a.T && sub < a.k) route_place(a, t, sub, mine[i], mine[i] >= 0 ? mask[mine[i]] : 0, t, [&](int x) { return start[x]; });
+#pragma unroll 1
+  for (int i = 0; i * AT_ONCE < a.T && i < TURNS; ++i) {
+    const int t = i * AT_ONCE + tid / L, e = chosen[i * THREADS + tid];
+    if (t < a.T && sub < a.k)
+      route_place(a, t, sub, e, e >= 0 ? mask[t >> 6][e] : 0, t & 63, [&](int x) {
+        int base = start[x];
+        for (int w = 0; w < t >> 6; ++w) base += __popcll(mask[w][x]);
+        return base;
+      });
   }
   for (int i = total + tid; i < a.T * a.k; i += THREADS) a.rows[i] = -1;
 }
 
 template <int DT, int L, int PER, bool WIDE>
 static void launch_route(const RouteArgs &a, hipStream_t st) {
-  if (a.T <= ROUTE_ONE_TOKENS) {
+  if (a.T <= route_one_tokens(L)) {
     if (a.T * L <= 256) hipLaunchKernelGGL((route_one_kernel<DT, L, PER, WIDE, 256>), dim3(1), dim3(256), 0, st, a);
     else hipLaunchKernelGGL((route_one_kernel<DT, L, PER, WIDE, 1024>), dim3(1), dim3(1024), 0, st, a);
     return;
@@ -549,7 +569,7 @@ static void launch_route(const RouteArgs &a, hipStream_t st) {
 }
 template <int DT, bool WIDE>
 static int route_shape(RouteArgs a, hipStream_t st) {
-  if (a.groups == 1 && a.k <= 16 && a.E <= 128) {
+  if (route_lanes(a.E, a.k, a.groups) == 16) {
     a.group_lanes = 16;
     if (a.E <= 16) launch_route<DT, 16, 1, WIDE>(a, st);
     else if (a.E <= 32) launch_route<DT, 16, 2, WIDE>(a, st);
@@ -574,8 +594,8 @@ static int route_width(const RouteArgs &a, hipStream_t st) {
   return wide ? route_shape<DT, true>(a, st) : route_shape<DT, false>(a, st);
 }
 
-static int64_t route_workspace(int64_t T, int64_t E) {
-  if (T <= ROUTE_ONE_TOKENS) return 0;
+static int64_t route_workspace(int64_t T, int64_t E, int64_t k, int64_t groups) {
+  if (T <= route_one_tokens(route_lanes(E, k, groups))) return 0;
   const int64_t blocks = ceil_div(T, ROUTE_TOKENS);
   return 4 * align_up(E, 4) + 4 * align_up(blocks * E, 4) + 3 * blocks * align_up(E, 16);
 }
@@ -638,9 +658,9 @@ using namespace ac4k;
 
 static bool float_tag(int d) { return d == AC4K_DTYPE_BF16 || d == AC4K_DTYPE_FP16 || d == AC4K_DTYPE_FP32; }
 
-extern "C" __attribute__((visibility("default"))) int64_t ac4k_route_experts_workspace_bytes(int64_t T, int64_t E, int64_t k) {
+extern "C" __attribute__((visibility("default"))) int64_t ac4k_route_experts_workspace_bytes(int64_t T, int64_t E, int64_t k, int64_t groups, int64_t top_groups) {
   if (T < 1 || E < 1 || E > AC4K_ROUTE_MAX_EXPERTS || k < 1 || k > AC4K_ROUTE_MAX_K) return 0;
-  return route_workspace(T, E);
+  return route_workspace(T, E, k, top_groups == groups ? 1 : groups);
 }
 
 extern "C" __attribute__((visibility("default"))) int ac4k_route_experts(
@@ -659,7 +679,7 @@ extern "C" __attribute__((visibility("default"))) int ac4k_route_experts(
                (int)AC4K_ROUTE_MAX_K, (long long)(E / groups * top_groups), (long long)k);
   AC4K_REQUIRE(T * k < (1ll << 27) && T <= (1ll << 26) - ROUTE_TOKENS, "too many tokens (%lld of %lld experts)", (long long)T,
                (long long)k);  // 2^32 threads a launch
-  const int64_t need = route_workspace(T, E);
+  const int64_t need = route_workspace(T, E, k, top_groups == groups ? 1 : groups);
   AC4K_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0), "workspace of %lld bytes needed, on 16 bytes", (long long)need);
   RouteArgs a{};
   a.logits = logits, a.stride = stride, a.bias = bias, a.weights = weights, a.experts = experts, a.offsets = offsets, a.rows = rows, a.places = places;

@@ -399,11 +399,11 @@ int ac4k_debug_last_grouped_kernel(void);
  *   offsets int32 [E + 1]: range of rows of each expert, in it the tokens in rising order;  rows int32 [T * k]: the token of each row, -1 from offsets[E] on;
  *   places int32 [T, k]: the row of each slot.
  * Without a bias and with best == 1, logits are compared as they are; otherwise keys in 64 bits.  Every call gives the same results again.
- * `workspace`: ac4k_route_experts_workspace_bytes(T, E, k), on 16 bytes, contents irrelevant, NULL when that is 0. */
+ * `workspace`: ac4k_route_experts_workspace_bytes(T, E, k, groups, top_groups), on 16 bytes, contents irrelevant, NULL when that is 0. */
 enum { AC4K_SCORE_SOFTMAX = 0, AC4K_SCORE_SIGMOID = 1 };
 #define AC4K_ROUTE_MAX_EXPERTS 1024
 #define AC4K_ROUTE_MAX_K 64
-int64_t ac4k_route_experts_workspace_bytes(int64_t T, int64_t E, int64_t k);
+int64_t ac4k_route_experts_workspace_bytes(int64_t T, int64_t E, int64_t k, int64_t groups, int64_t top_groups);
 int ac4k_route_experts(float *weights, int32_t *experts, int32_t *offsets, int32_t *rows, int32_t *places, const void *logits, int dtype,
                        int64_t stride, const float *bias, int64_t T, int64_t E, int64_t k, int scoring, int64_t groups, int64_t top_groups,
                        int best, int renormalize, double scale, void *workspace, int64_t workspace_bytes, ac4k_stream_t stream);

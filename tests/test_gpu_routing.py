@@ -82,7 +82,8 @@ def bias_of(e, seed=0, std=0.1):
 
 
 SHAPES = [(1, 1, 1), (1, 8, 2), (3, 5, 5), (16, 64, 8), (17, 60, 4), (64, 128, 8), (65, 128, 16), (64, 33, 17), (63, 1000, 64), (130, 256, 8), (129, 97, 6),
-          (200, 512, 6), (66, 1024, 8), (257, 16, 2), (1025, 32, 4), (100, 1, 1), (100, 3, 2), (70, 9, 4), (65, 7, 7)]
+          (200, 512, 6), (66, 1024, 8), (257, 16, 2), (1025, 32, 4), (100, 1, 1), (100, 3, 2), (70, 9, 4), (65, 7, 7),
+          (128, 64, 16), (192, 128, 4), (255, 17, 3), (256, 100, 8), (300, 1, 1), (300, 3, 2), (290, 9, 4), (270, 7, 7), (129, 64, 17)]
 
 
 @pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])

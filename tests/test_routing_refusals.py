@@ -44,7 +44,7 @@ def test_route_at_the_c_abi():
     refused(route(T=1 << 26, k=2), b"too many tokens")
     refused(route(T=(1 << 26) - 15, k=1), b"too many tokens")  # 2^22 workgroups of 1024 threads
     refused(route(T=1000), b"workspace")
-    need = lib().ac4k_route_experts_workspace_bytes(1000, 64, 4)
+    need = lib().ac4k_route_experts_workspace_bytes(1000, 64, 4, 1, 1)
     assert need > 0
     refused(route(T=1000, ws=ONE, ws_bytes=need - 1), b"workspace")
     refused(route(T=1000, ws=ODD, ws_bytes=need), b"workspace")
@@ -52,10 +52,13 @@ def test_route_at_the_c_abi():
 
 def test_workspace_sizes():
     size = lib().ac4k_route_experts_workspace_bytes
-    assert size(64, 64, 4) == 0 and size(0, 64, 4) == 0 and size(100, 1025, 4) == 0 and size(100, 64, 0) == 0
-    for t in (65, 1000, 100000):
+    assert size(64, 64, 4, 1, 1) == 0 and size(0, 64, 4, 1, 1) == 0 and size(100, 1025, 4, 1, 1) == 0 and size(100, 64, 0, 1, 1) == 0
+    # one workgroup: 128 tokens on 16 lanes each, 64 on a wave
+    assert size(128, 64, 4, 1, 1) == size(128, 128, 16, 4, 4) == 0 < size(129, 64, 4, 1, 1)
+    assert size(65, 64, 4, 4, 2) > 0 and size(65, 64, 17, 1, 1) > 0 and size(65, 129, 4, 1, 1) > 0 and size(64, 129, 4, 1, 1) == 0
+    for t in (300, 1000, 100000):
         blocks = -(-t // 16)
-        assert size(t, 64, 4) >= 4 * 64 + 6 * blocks * 64
+        assert size(t, 64, 4, 1, 1) >= 4 * 64 + 7 * blocks * 64
 
 
 def combine(**kw):
